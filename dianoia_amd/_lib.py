@@ -146,10 +146,31 @@ SIGNATURES = {
     "dnx_attention": ([_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p], _i32),
     "dnx_attention_f6panel": ([_p] * 6 + [_i64] * 6 + [_p], _i32),
     "dnx_attention_rope": ([_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _f32, _p], _i32),
+    "dnx_quantize_i8r": ([_p, _p, _p, _i64, _i64, _i64, _p], _i32),
+    "dnx_quantize_i8r_bf16": ([_p, _p, _p, _i64, _i64, _i64, _p], _i32),
+    "dnx_rms_norm_i8r": ([_p] * 6 + [_i64] * 3 + [_f32, _p], _i32),
+    "dnx_gemm_i8r": ([_p] * 5 + [_i64] * 3 + [_p], _i32),
+    "dnx_paged_append": ([_p, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _p, _i64,
+                          _i64, _f32, _p], _i32),
+    "dnx_paged_attention_workspace_bytes": ([_p, _p, _i64], _i64),
+    "dnx_paged_attention": ([_p] * 5 + [_i64, _i64, _p, _i64, _p], _i32),
     "dnx_add": ([_p, _p, _i64, _p], _i32),
     "dnx_copy": ([_p, _p, _i64, _p], _i32),
     "dnx_steer": ([_p, _p, _i64, _i64, _i64, _f32, _p], _i32),
 }
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """dnx_paged_cache."""
+    _fields_ = [("keys", _p), ("values", _p), ("pages", _i64), ("page", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("hd", ctypes.c_int32), ("type", ctypes.c_int32)]
+
+
+class PagedBatchStruct(ctypes.Structure):
+    """dnx_paged_batch."""
+    _fields_ = [("starts", _p), ("lens", _p), ("tables", _p), ("prefix_pages", _p),
+                ("table_stride", _i64), ("prefix_len", _i64), ("seqs", _i64), ("tokens", _i64),
+                ("max_tokens", _i64), ("max_len", _i64)]
 
 
 class LibraryMissing(RuntimeError):

@@ -1,7 +1,7 @@
 """Builds libdianoia_amd.so (gfx950 HIP kernels + the lab_gpu_* C ABI) in-tree.
 
 Run as ``python -m dianoia_amd.build``; ``__graft_entry__.build()`` calls
-:func:`build`. The three translation units compile in parallel and link into
+:func:`build`. The translation units compile in parallel and link into
 one shared library next to this file, so it travels with the source tree.
 """
 
@@ -22,7 +22,7 @@ LIB = os.path.join(HERE, "libdianoia_amd.so")
 UBENCH_SRC = "ubench_tile.hip"
 UBENCH_LIB = os.path.join(HERE, "libdnx_ubench.so")
 SOURCES = ["kernels.hip", "gemv.hip", "gemm.hip", "gemm_f16.hip", "gemm_f6.hip", "gemm_float.hip",
-           "layers.hip", "matmul.hip", "lab_gpu.hip"]
+           "layers.hip", "rows_i8.hip", "gemm_i8r.hip", "paged.hip", "matmul.hip", "lab_gpu.hip"]
 ARCH = "gfx950"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -40,7 +40,8 @@ FLAGS = [
 # scale epilogue reads every result with VALU instructions, which cannot
 # take accumulation registers (one v_accvgpr_read per value otherwise).
 SOURCE_FLAGS = {src: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-                for src in ("gemm.hip", "gemm_f16.hip", "gemm_f6.hip", "gemm_float.hip", UBENCH_SRC)}
+                for src in ("gemm.hip", "gemm_f16.hip", "gemm_f6.hip", "gemm_float.hip", "paged.hip",
+                            UBENCH_SRC)}
 
 
 def _compile(src: str, build_dir: str) -> str:

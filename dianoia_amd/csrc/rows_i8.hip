@@ -1,0 +1,194 @@
+// Rows as int8 with one float32 scale a row: the activations and the weights
+// of the products in gemm_i8r.hip. Per row, with y the row's values,
+//   y_j = x_j                                   (quantize: weights, any rows)
+//   y_j = w_j (s_j r), r = 1 / sqrt(mean(s^2) + eps), s = x + m or x  (norm)
+//   top = max |y_j|, scale = top / 127, code_j = y_j / scale rounded to the
+//   nearest whole number, halves away from zero; zeros past cols.
+// No counterpart in the reference, whose 8-bit rows have a scale per 32
+// values.
+//
+// The codes of a normed row do not depend on r: code_j = 127 w_j s_j / max
+// |w s|. They are formed in 64 bits, where the product of two floats is
+// exact, so a code is that of the formula, not of the order of a float sum.
+// The factor 127 / top is rounded up by 2^-50: a value on the border of two
+// codes (which bf16 weights meet: 254 x = (2 k + 1) top) then goes away from
+// zero whatever the division's last bit, and no float strictly inside reaches
+// the border: 254 x - (2 k + 1) top is a whole multiple of 2^-34 top or more.
+// 64-bit multiply-adds run at the rate of 32-bit ones on this chip, so the
+// rows stay bound by their bytes.
+
+#include "common.h"
+#include "dnx_kernels.h"
+
+#include <math.h>
+
+using namespace dnx;
+
+namespace {
+
+constexpr int kMaxThreads = 1024;
+constexpr int kMaxV = 16;                                // four values each, per thread
+constexpr int64_t kMaxCols = (int64_t)kMaxThreads * kMaxV * 4;
+
+DNX_DEV double wave_sum64(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+DNX_DEV double wave_max64(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o));
+  return v;
+}
+
+DNX_DEV float4 load4(const float* p) { return *(const float4*)p; }
+DNX_DEV float4 load4(const uint16_t* p) {
+  const uint2 b = *(const uint2*)p;
+  return make_float4(__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u),
+                     __uint_as_float(b.y << 16), __uint_as_float(b.y & 0xffff0000u));
+}
+
+// One code: the nearest whole number to y * inv, halves away from zero. The
+// limits bind only where the row holds an infinity or NaN.
+DNX_DEV int code1(double y, double inv) {
+  const double t = y * inv;
+  return (int)fmin(fmax(t + __builtin_copysign(0.5, t), -127.5), 127.5);
+}
+
+DNX_DEV int pack4(int a, int b, int c, int d) {
+  return (a & 0xff) | ((b & 0xff) << 8) | ((c & 0xff) << 16) | (int)((uint32_t)d << 24);
+}
+
+// One workgroup a row, four values per thread and step e (V steps cover the
+// row): the row stays in registers between the reduction and the codes.
+template <typename S, int V, bool kNorm, bool kAdd>
+__global__ void __launch_bounds__(kMaxThreads)
+rows_i8_kernel(const S* x, const float* __restrict__ m, float* x_out, const float* __restrict__ w,
+               int8_t* __restrict__ qs, float* __restrict__ scales, int cols, int cols_pad,
+               float eps) {
+  __shared__ double part[2][kMaxThreads / 64];
+  const int quads = cols / 4, threads = blockDim.x, tid = threadIdx.x;
+  const size_t at = (size_t)blockIdx.x * cols;
+  // Every load of the row before the first store: x_out may be x.
+  float4 xv[V], wv[V], mv[V];
+#pragma unroll
+  for (int e = 0; e < V; e++) {
+    const int i = e * threads + tid;
+    xv[e] = wv[e] = mv[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (i < quads) {
+      xv[e] = load4(x + at + 4 * i);
+      if constexpr (kNorm) wv[e] = load4(w + 4 * i);
+      if constexpr (kAdd) mv[e] = load4(m + at + 4 * i);
+    }
+  }
+  if constexpr (kAdd) {
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      const int i = e * threads + tid;
+      xv[e] = make_float4(xv[e].x + mv[e].x, xv[e].y + mv[e].y, xv[e].z + mv[e].z,
+                          xv[e].w + mv[e].w);
+      if (i < quads) *(float4*)(x_out + at + 4 * i) = xv[e];
+    }
+  }
+  // The sum of squares (finite in 64 bits for finite floats) also tells of an
+  // infinity or NaN, which has no code: the row's scale is NaN.
+  double sum = 0.0, top = 0.0;
+#pragma unroll
+  for (int e = 0; e < V; e++)
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      const double s = (&xv[e].x)[c];
+      sum = fma(s, s, sum);
+      top = fmax(top, fabs(kNorm ? s * (double)(&wv[e].x)[c] : s));
+    }
+  sum = wave_sum64(sum);
+  top = wave_max64(top);
+  if ((tid & 63) == 0) {
+    part[0][tid >> 6] = sum;
+    part[1][tid >> 6] = top;
+  }
+  __syncthreads();
+  sum = part[0][0];
+  top = part[1][0];
+  for (int k = 1; k < threads / 64; k++) {
+    sum += part[0][k];
+    top = fmax(top, part[1][k]);
+  }
+  if (tid == 0) {
+    double scale = top / 127.0;
+    if constexpr (kNorm) scale *= 1.0 / sqrt(sum / (double)cols + (double)eps);
+    scales[blockIdx.x] = sum < INFINITY ? (float)scale : NAN;
+  }
+  const double inv = top > 0.0 ? 127.0 / top * (1.0 + 0x1p-50) : 0.0;
+  int* out = (int*)(qs + (size_t)blockIdx.x * cols_pad);
+#pragma unroll
+  for (int e = 0; e < V; e++) {
+    const int i = e * threads + tid;
+    if (i >= quads) break;
+    int q[4];
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      const double s = (&xv[e].x)[c];
+      q[c] = code1(kNorm ? s * (double)(&wv[e].x)[c] : s, inv);
+    }
+    out[i] = pack4(q[0], q[1], q[2], q[3]);
+  }
+  for (int i = quads + tid; i < cols_pad / 4; i += threads) out[i] = 0;
+}
+
+template <typename S, bool kNorm, bool kAdd>
+int launch_rows(const S* x, const float* m, float* x_out, const float* w, int8_t* qs,
+                float* scales, int64_t rows, int64_t cols, int64_t cols_pad, float eps,
+                dnx_stream_t stream) {
+  if (rows < 0 || rows > 0x7fffffff || cols <= 0 || cols % 4 != 0 || cols > kMaxCols ||
+      cols_pad < cols || cols_pad % kBlock != 0 || cols_pad > kMaxCols) {
+    return DNX_EINVAL;
+  }
+  if (rows == 0) return DNX_OK;
+  if (x == nullptr || qs == nullptr || scales == nullptr ||
+      (((uintptr_t)x | (uintptr_t)m | (uintptr_t)x_out | (uintptr_t)w | (uintptr_t)qs) & 15) != 0 ||
+      ((uintptr_t)scales & 3) != 0) {
+    return DNX_EINVAL;
+  }
+  const int64_t quads = cols / 4;
+  const int64_t steps = (quads + kMaxThreads - 1) / kMaxThreads;
+  const int V = steps <= 1 ? 1 : steps <= 2 ? 2 : steps <= 4 ? 4 : kMaxV;
+  const unsigned threads = (unsigned)(((quads + V - 1) / V + 63) / 64 * 64);
+  auto k = V == 1   ? rows_i8_kernel<S, 1, kNorm, kAdd>
+           : V == 2 ? rows_i8_kernel<S, 2, kNorm, kAdd>
+           : V == 4 ? rows_i8_kernel<S, 4, kNorm, kAdd>
+                    : rows_i8_kernel<S, kMaxV, kNorm, kAdd>;
+  hipLaunchKernelGGL(k, dim3((unsigned)rows), dim3(threads), 0, (hipStream_t)stream, x, m, x_out, w,
+                     qs, scales, (int)cols, (int)cols_pad, eps);
+  return hipGetLastError() == hipSuccess ? DNX_OK : DNX_ELAUNCH;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dnx_quantize_i8r(const float* x, int8_t* qs, float* scales, int64_t rows, int64_t cols,
+                     int64_t cols_pad, dnx_stream_t stream) {
+  return launch_rows<float, false, false>(x, nullptr, nullptr, nullptr, qs, scales, rows, cols,
+                                          cols_pad, 0.0f, stream);
+}
+
+int dnx_quantize_i8r_bf16(const uint16_t* x, int8_t* qs, float* scales, int64_t rows, int64_t cols,
+                          int64_t cols_pad, dnx_stream_t stream) {
+  return launch_rows<uint16_t, false, false>(x, nullptr, nullptr, nullptr, qs, scales, rows, cols,
+                                             cols_pad, 0.0f, stream);
+}
+
+int dnx_rms_norm_i8r(const float* x, const float* m, float* x_out, const float* w, int8_t* qs,
+                     float* scales, int64_t rows, int64_t cols, int64_t cols_pad, float eps,
+                     dnx_stream_t stream) {
+  if (rows != 0 && (w == nullptr || (m == nullptr) != (x_out == nullptr))) return DNX_EINVAL;
+  if (m != nullptr) {
+    return launch_rows<float, true, true>(x, m, x_out, w, qs, scales, rows, cols, cols_pad, eps,
+                                          stream);
+  }
+  return launch_rows<float, true, false>(x, nullptr, nullptr, w, qs, scales, rows, cols, cols_pad,
+                                         eps, stream);
+}
+
+}  // extern "C"

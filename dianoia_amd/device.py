@@ -618,3 +618,173 @@ def matmul_q4(qs, scales, x, y, rows: int, cols: int, n: int, int8_inputs: bool,
     _check(_lib.load().dnx_matmul_q4(_ptr(qs), _ptr(scales), _ptr(x), _ptr(y), rows, cols, n,
                                      int(int8_inputs), _ptr(workspace), workspace.numel(),
                                      _stream(stream)), "dnx_matmul_q4")
+
+
+# ---- a batch of sequences at once: int8 rows and products, paged keys and values
+
+def quantize_i8r(x, qs, scales, rows: int, cols: int, cols_pad: int, stream=None) -> None:
+    """fp32 rows -> int8 [rows][cols_pad] with one scale a row (value = code * scale)."""
+    _need("quantize_i8r", x=(x, rows * cols * 4), qs=(qs, rows * cols_pad),
+          scales=(scales, rows * 4))
+    _check(_lib.load().dnx_quantize_i8r(_ptr(x), _ptr(qs), _ptr(scales), rows, cols, cols_pad,
+                                        _stream(stream)), "dnx_quantize_i8r")
+
+
+def quantize_i8r_bf16(x, qs, scales, rows: int, cols: int, cols_pad: int, stream=None) -> None:
+    """bf16 rows (weights as they lie in a file) -> int8 with one scale a row."""
+    _need("quantize_i8r_bf16", x=(x, rows * cols * 2), qs=(qs, rows * cols_pad),
+          scales=(scales, rows * 4))
+    _check(_lib.load().dnx_quantize_i8r_bf16(_ptr(x), _ptr(qs), _ptr(scales), rows, cols,
+                                             cols_pad, _stream(stream)), "dnx_quantize_i8r_bf16")
+
+
+def rms_norm_i8r(x, w, qs, scales, rows: int, cols: int, cols_pad: int, eps: float, m=None,
+                 x_out=None, stream=None) -> None:
+    """RMSNorm(s) * w as int8 with one scale a row; s = x, or x + m, which goes
+    to x_out (x itself, m or another tensor)."""
+    _need("rms_norm_i8r", x=(x, rows * cols * 4), w=(w, cols * 4), qs=(qs, rows * cols_pad),
+          scales=(scales, rows * 4), m=(m, rows * cols * 4), x_out=(x_out, rows * cols * 4))
+    _check(_lib.load().dnx_rms_norm_i8r(_ptr(x), _ptr(m), _ptr(x_out), _ptr(w), _ptr(qs),
+                                        _ptr(scales), rows, cols, cols_pad, eps,
+                                        _stream(stream)), "dnx_rms_norm_i8r")
+
+
+def gemm_i8r(w, w_scale, x, x_scale, y, rows: int, cols: int, n: int, stream=None) -> None:
+    """y [n][rows] = the int8 rows x times the int8 rows w, each with its scale."""
+    _need("gemm_i8r", w=(w, rows * cols), w_scale=(w_scale, rows * 4), x=(x, n * cols),
+          x_scale=(x_scale, n * 4), y=(y, n * rows * 4))
+    _check(_lib.load().dnx_gemm_i8r(_ptr(w), _ptr(w_scale), _ptr(x), _ptr(x_scale), _ptr(y), rows,
+                                    cols, n, _stream(stream)), "dnx_gemm_i8r")
+
+
+_CACHE_TYPES = {torch.float32: 0, torch.bfloat16: 1}   # DNX_F32, DNX_BF16
+
+
+class PagedCache:
+    """Keys and values in pages: two tensors [pages][page][kv_heads][hd],
+    float32 or bfloat16 (dnx_paged_cache). Keeps the tensors, not copies."""
+
+    def __init__(self, keys: torch.Tensor, values: torch.Tensor):
+        if keys.dim() != 4 or keys.shape != values.shape or keys.dtype != values.dtype:
+            raise ValueError("PagedCache: two tensors [pages][page][kv_heads][hd] of one type")
+        if keys.dtype not in _CACHE_TYPES:
+            raise ValueError("PagedCache: float32 or bfloat16")
+        pages, page, kv_heads, hd = keys.shape
+        if page < 16 or page > 4096 or page & (page - 1):
+            raise ValueError("PagedCache: the page is a power of two from 16 to 4096")
+        if hd not in (64, 128) or not 0 < kv_heads <= 1024 or not 0 < pages * page <= 0x7fffffff:
+            raise ValueError("PagedCache: hd 64 or 128, up to 1024 heads, below 2^31 places")
+        self.keys, self.values = keys, values
+        self.kv_heads, self.hd = kv_heads, hd
+        self.struct = _lib.PagedCacheStruct(_ptr(keys), _ptr(values), pages, page, kv_heads, hd,
+                                            _CACHE_TYPES[keys.dtype])
+        self.ref = ctypes.addressof(self.struct)
+
+
+def _int32(what: str, t, *shape) -> int | None:
+    """The pointer of an int32 tensor with at least the elements of `shape`."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32:
+        raise ValueError(f"{what} is int32")
+    n = 1
+    for s in shape:
+        n *= s
+    if t.numel() < n:
+        raise ValueError(f"{what} holds {t.numel()} numbers, the batch needs {n}")
+    return _ptr(t)
+
+
+class PagedBatch:
+    """A batch over a PagedCache (dnx_paged_batch): starts [seqs + 1], lens
+    [seqs] and tables [seqs][pages] as int32 tensors, which may change between
+    calls (their values, in place); the number of rows, and the bounds that no
+    sequence's new tokens and own keys pass. prefix_pages: the pages of the
+    prefix_len keys with which every sequence begins."""
+
+    def __init__(self, starts, lens, tables, tokens: int, max_tokens: int, max_len: int,
+                 prefix_pages=None, prefix_len: int = 0):
+        seqs = lens.numel()
+        if tables.dim() != 2 or tables.shape[0] != seqs:
+            raise ValueError("PagedBatch: tables [seqs][pages]")
+        if seqs < 1 or tokens < 0 or max_tokens < 1 or max_len < 0 or prefix_len < 0:
+            raise ValueError("PagedBatch: a sequence at least, and no negative numbers")
+        self.starts, self.lens, self.tables, self.prefix_pages = starts, lens, tables, prefix_pages
+        self.tokens, self.prefix_len = tokens, prefix_len
+        self.struct = _lib.PagedBatchStruct(
+            _int32("starts", starts, seqs + 1), _int32("lens", lens, seqs),
+            _int32("tables", tables, seqs, tables.shape[1]), _int32("prefix_pages", prefix_pages, 0),
+            tables.shape[1], prefix_len, seqs, tokens, max_tokens, max_len)
+        self.ref = ctypes.addressof(self.struct)
+
+    def check(self, cache: PagedCache) -> None:
+        if self.prefix_len > 0 and (self.prefix_pages is None or self.prefix_pages.numel()
+                                    * cache.struct.page < self.prefix_len):
+            raise ValueError("PagedBatch: prefix_pages holds fewer pages than the prefix needs")
+
+
+def _head_rows(what: str, t: torch.Tensor, hd: int):
+    """(pointer, stride of a token) of float32 [n][heads][hd], heads and dims dense."""
+    if not t.is_cuda or t.dtype != torch.float32:
+        raise ValueError(f"{what} is a float32 CUDA (HIP) tensor")
+    if t.dim() != 3 or t.shape[2] != hd or t.stride(2) != 1 or t.stride(1) != hd:
+        raise ValueError(f"{what} is [n][heads][{hd}] with dense heads")
+    n = t.shape[0]
+    return t.data_ptr(), t.stride(0) if n > 1 else t.shape[1] * hd
+
+
+def paged_append(cache: PagedCache, k, v, positions, slots, rope=None, q=None, q_out=None,
+                 q_norm=None, k_norm=None, eps: float = 1e-6, stream=None) -> None:
+    """New tokens' keys [n][kv_heads][hd], normed and rotated, and values into
+    places `slots` of the cache (dnx_paged_append); with q [n][heads][hd] also
+    the queries, normed and rotated, into q_out. q, k and v may be views of one
+    projection's output. A slot of -1 leaves its token out."""
+    n, hd = k.shape[0], cache.hd
+    kp, ks = _head_rows("paged_append: k", k, hd)
+    vp, vs = _head_rows("paged_append: v", v, hd)
+    if k.shape[1] != cache.kv_heads or v.shape != k.shape:
+        raise ValueError("paged_append: k and v hold the cache's heads for the same tokens")
+    qp, qs, op, heads = None, 0, None, 0
+    if q is not None:
+        qp, qs = _head_rows("paged_append: q", q, hd)
+        heads = q.shape[1]
+        if q.shape[0] != n or q_out is None or q_out.dtype != torch.float32:
+            raise ValueError("paged_append: q of the same tokens, and a float32 q_out")
+        _need("paged_append", q_out=(q_out, n * heads * hd * 4))
+        op = _ptr(q_out)
+    _need("paged_append", q_norm=(q_norm, hd * 4), k_norm=(k_norm, hd * 4))
+    rows = 0
+    if rope is not None:
+        if rope.dim() != 2 or rope.shape[1] != hd or rope.dtype != torch.float32 or positions is None:
+            raise ValueError("paged_append: rope is float32 [positions][hd], with positions")
+        rows = rope.shape[0]
+    _check(_lib.load().dnx_paged_append(
+        cache.ref, qp, qs, op, kp, ks, vp, vs, _ptr(q_norm), _ptr(k_norm), _ptr(rope), rows,
+        _int32("positions", positions, n), _int32("slots", slots, n), heads, n, eps,
+        _stream(stream)), "dnx_paged_append")
+
+
+def paged_attention_workspace(cache: PagedCache, batch: PagedBatch, heads: int,
+                              device="cuda") -> torch.Tensor:
+    """Device workspace of paged_attention for a batch of these bounds."""
+    batch.check(cache)
+    nbytes = int(_lib.load().dnx_paged_attention_workspace_bytes(cache.ref, batch.ref, heads))
+    if nbytes < 0:
+        raise RuntimeError("dnx_paged_attention_workspace_bytes refused the batch")
+    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+
+
+def paged_attention(cache: PagedCache, batch: PagedBatch, q, out, workspace, window: int = 0,
+                    gate=None, stream=None) -> None:
+    """Attention of the batch's new tokens q [tokens][heads][hd] over the shared
+    prefix and each sequence's own pages, into out (dnx_paged_attention)."""
+    if q.dim() != 3 or q.shape[0] != batch.tokens or q.shape[2] != cache.hd:
+        raise ValueError("paged_attention: q is [tokens][heads][hd]")
+    if q.dtype != torch.float32 or out.dtype != torch.float32:
+        raise ValueError("paged_attention: q and out are float32")
+    heads = q.shape[1]
+    batch.check(cache)
+    _need("paged_attention", out=(out, q.nbytes), gate=(gate, batch.tokens * heads * 4))
+    _check(_lib.load().dnx_paged_attention(cache.ref, batch.ref, _ptr(q), _ptr(gate), _ptr(out),
+                                           heads, window, _ptr(workspace), workspace.nbytes,
+                                           _stream(stream)), "dnx_paged_attention")

@@ -513,6 +513,109 @@ int dnx_copy(const float* src, float* dst, int64_t count, dnx_stream_t stream);
 int dnx_steer(float* x, const float* v, int64_t rows, int64_t cols, int64_t mode, float scale,
               dnx_stream_t stream);
 
+// ---- A batch of sequences at once (no counterpart in the reference, which
+// serves one sequence): int8 rows and their products, and keys and values in
+// pages. Nothing here allocates or keeps state between calls, so every call
+// may be captured into a graph.
+//
+// int8 rows with one float32 scale each, value = code * scale: scale is the
+// row's largest |value| / 127, each code the nearest whole number, halves away
+// from zero, codes past `cols` zero (cols_pad a multiple of 32 >= cols, cols a
+// multiple of 4 up to 65536). Activations (rows = tokens) and weights (rows =
+// output channels) alike; _bf16 takes bf16 rows, as weights lie in a file. A
+// row that holds an infinity or NaN gets a NaN scale. Pointers 16-byte aligned
+// (scales 4).
+int dnx_quantize_i8r(const float* x, int8_t* qs, float* scales, int64_t rows, int64_t cols,
+                     int64_t cols_pad, dnx_stream_t stream);
+int dnx_quantize_i8r_bf16(const uint16_t* x, int8_t* qs, float* scales, int64_t rows, int64_t cols,
+                          int64_t cols_pad, dnx_stream_t stream);
+// The same of RMSNorm(s) * w, s = x + m (float32, written to x_out, which may
+// be x or m) or, with m and x_out both null, s = x. Sums and codes are formed
+// in 64 bits: they do not depend on an order of summation.
+int dnx_rms_norm_i8r(const float* x, const float* m, float* x_out, const float* w, int8_t* qs,
+                     float* scales, int64_t rows, int64_t cols, int64_t cols_pad, float eps,
+                     dnx_stream_t stream);
+// y[t][r] = x_scale[t] w_scale[r] sum_k x[t][k] w[r][k] on such rows: exact
+// integer sums, y [n][rows] float32 rounded from them. cols a multiple of 32
+// up to 131040 (the width the rows were written with), any n and rows; w and x
+// 16-byte aligned.
+int dnx_gemm_i8r(const int8_t* w, const float* w_scale, const int8_t* x, const float* x_scale,
+                 float* y, int64_t rows, int64_t cols, int64_t n, dnx_stream_t stream);
+
+// Keys and values in pages: each [pages][page][kv_heads][hd], of `type`, page
+// a power of two from 16 to 4096, hd 64 or 128, pages * page below 2^31,
+// kv_heads up to 1024, 16-byte aligned.
+enum { DNX_F32 = 0, DNX_BF16 = 1 };
+typedef struct {
+  void* keys;
+  void* values;
+  int64_t pages;
+  int32_t page;
+  int32_t kv_heads;
+  int32_t hd;
+  int32_t type;
+} dnx_paged_cache;
+
+// New tokens' keys and values into their places of the cache. Token t's key
+// heads (k + t * k_stride, kv_heads * hd floats) are normed per head (RMSNorm
+// over hd with k_norm; null: not) and rotated (pairs j, j + hd / 2 by
+// rope[positions[t]], a row of a table [rope_rows][cos(hd / 2), sin(hd / 2)];
+// null: not) as dnx_head_norm_rope does, its values taken as they are, and
+// both rounded to the cache's type (to nearest, ties to even) at place
+// slots[t] = page * c.page + row of the page. With q (heads per token, null:
+// none) the token's queries are normed with q_norm and rotated into q_out
+// [n][heads][hd], which may be q where that is contiguous. A token whose slot
+// lies outside the cache (-1: padding) or whose position lies outside the
+// table is left out: nothing is written for it. Two tokens of one call must
+// not have the same slot (which of them is kept, and whether whole, is open).
+// Strides in floats, multiples of 4; pointers 16-byte aligned.
+int dnx_paged_append(const dnx_paged_cache* cache, const float* q, int64_t q_stride, float* q_out,
+                     const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                     const float* q_norm, const float* k_norm, const float* rope,
+                     int64_t rope_rows, const int32_t* positions, const int32_t* slots,
+                     int64_t heads, int64_t n, float eps, dnx_stream_t stream);
+
+// A batch over such a cache. Its first prefix_len keys, in the pages listed in
+// prefix_pages, are shared: every sequence begins with them. Sequence b's own
+// keys follow, lens[b] of them (its new tokens' among them) in the pages
+// tables[b * table_stride ..]; its new tokens are the rows starts[b] ..
+// starts[b + 1] - 1 of the call (starts[0] = 0; none, one or many). tokens is
+// the number of rows, which may be more than starts[seqs]: rows behind the
+// last sequence's are neither read nor written. The arrays lie in device
+// memory and may change from call to call under one captured graph; the
+// numbers here bound them: no sequence has more than max_tokens new tokens,
+// and own keys past max_len or past the table are not seen.
+typedef struct {
+  const int32_t* starts;
+  const int32_t* lens;
+  const int32_t* tables;
+  const int32_t* prefix_pages;
+  int64_t table_stride;
+  int64_t prefix_len;
+  int64_t seqs;
+  int64_t tokens;
+  int64_t max_tokens;
+  int64_t max_len;
+} dnx_paged_batch;
+
+// Causal attention of such a batch: the i-th of a sequence's c new tokens
+// stands at position prefix_len + lens[b] - c + i and sees the keys up to its
+// own (window > 0: the last `window` of them), scores q.k / sqrt(hd). q and
+// out [tokens][heads][hd] float32, heads a multiple of kv_heads; gate [tokens]
+// [heads] or null: the output times sigmoid(gate), as dnx_attention's. The
+// prefix's keys are read once for all sequences. Keys in a page outside the
+// cache are not seen, a row without any weight (no key seen) is zeros, and
+// what lies in masked places (infinities, NaN) does not matter. float32
+// arithmetic throughout. workspace: dnx_paged_attention_workspace_bytes of
+// device memory (the partial results of runs of keys), 16-byte aligned; calls
+// that overlap need one each. The two structs are read at the call.
+int64_t dnx_paged_attention_workspace_bytes(const dnx_paged_cache* cache,
+                                            const dnx_paged_batch* batch, int64_t heads);
+int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* batch,
+                        const float* q, const float* gate, float* out, int64_t heads,
+                        int64_t window, void* workspace, int64_t workspace_bytes,
+                        dnx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
