@@ -15,6 +15,7 @@ import torch
 
 from dianoia_amd import device as D
 from gpu_util import bits, dev, host
+from test_gemm_i8r_route import SHAPES as TILES
 
 U = 2.0 ** -24
 EPS = 1e-6
@@ -169,6 +170,27 @@ def test_product(gpu_ready, n, rows, cols):
     exact = exact * xs[:, None].astype(np.float64) * ws.astype(np.float64)
     assert (np.abs(got[:n * rows].reshape(n, rows) - exact) <= 3 * U * (1 + 2 * U) * np.abs(exact)).all()
     assert (got[n * rows:] == 3.5).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", TILES)
+@pytest.mark.parametrize("shift", [0, 1])
+def test_product_every_tile(gpu_ready, shape, shift):
+    """Each tile kernel of the route, at odd sizes and at rows of a multiple of
+    4, the outputs on 16 bytes or not. Sums below 2^53 are exact in float64."""
+    n, rows, cols = shape
+    for rows in (rows, rows // 4 * 4):
+        print(f"product {n} x {rows} x {cols}", flush=True)
+        g = torch.Generator(device="cuda").manual_seed(n)
+        w, x = (torch.randint(-128, 128, (r, cols), device="cuda", generator=g).to(torch.int8)
+                for r in (rows, n))
+        ws, xs = (torch.rand(r, device="cuda", generator=g) + 0.5 for r in (rows, n))
+        y = torch.full((shift + n * rows + 64,), 3.5, device="cuda")
+        D.gemm_i8r(w, ws, x, xs, y[shift:], rows, cols, n)
+        exact = (x.double() @ w.double().t()) * xs.double()[:, None] * ws.double()
+        got = y[shift:shift + n * rows].view(n, rows).double()
+        assert ((got - exact).abs() <= 3 * U * (1 + 2 * U) * exact.abs()).all()
+        assert (y[:shift] == 3.5).all() and (y[shift + n * rows:] == 3.5).all()
 
 
 @pytest.mark.gpu
