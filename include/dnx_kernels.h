@@ -523,8 +523,8 @@ int dnx_steer(float* x, const float* v, int64_t rows, int64_t cols, int64_t mode
 // from zero, codes past `cols` zero (cols_pad a multiple of 32 >= cols, cols a
 // multiple of 4 up to 65536). Activations (rows = tokens) and weights (rows =
 // output channels) alike; _bf16 takes bf16 rows, as weights lie in a file. A
-// row that holds an infinity or NaN gets a NaN scale. Pointers 16-byte aligned
-// (scales 4).
+// row that holds an infinity or NaN gets a NaN scale (and zero codes). Pointers
+// 16-byte aligned (scales 4).
 int dnx_quantize_i8r(const float* x, int8_t* qs, float* scales, int64_t rows, int64_t cols,
                      int64_t cols_pad, dnx_stream_t stream);
 int dnx_quantize_i8r_bf16(const uint16_t* x, int8_t* qs, float* scales, int64_t rows, int64_t cols,

@@ -118,7 +118,22 @@ def test_extremes(gpu_ready):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,cols,pad", SHAPES)
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("rows", [3, 600])
+def test_norm_weight_without_a_code(gpu_ready, rows, bad):
+    """An infinity or NaN in the weight reaches every row's scale."""
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((rows, 96)).astype(np.float32)
+    w = np.ones(96, np.float32)
+    w[50] = bad
+    qs, scales = outputs(rows, 96)
+    D.rms_norm_i8r(dev(x), dev(w), qs, scales, rows, 96, 96, EPS)
+    assert np.isnan(host(scales)[:rows]).all() and (host(qs)[:rows] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,pad", SHAPES + [(600, 260, 288), (513, 4096, 4096),
+                                                    (700, 8196, 8224)])
 @pytest.mark.parametrize("add", [False, True])
 def test_norm(gpu_ready, rows, cols, pad, add):
     rng = np.random.default_rng(rows * 7 + cols + add)
