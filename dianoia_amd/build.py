@@ -22,7 +22,8 @@ LIB = os.path.join(HERE, "libdianoia_amd.so")
 UBENCH_SRC = "ubench_tile.hip"
 UBENCH_LIB = os.path.join(HERE, "libdnx_ubench.so")
 SOURCES = ["kernels.hip", "gemv.hip", "gemm.hip", "gemm_f16.hip", "gemm_f6.hip", "gemm_float.hip",
-           "layers.hip", "rows_i8.hip", "gemm_i8r.hip", "paged.hip", "matmul.hip", "lab_gpu.hip"]
+           "layers.hip", "rows_i8.hip", "gemm_i8r.hip", "paged_append.hip",
+           "paged_attention.hip", "matmul.hip", "lab_gpu.hip"]
 ARCH = "gfx950"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -40,7 +41,8 @@ FLAGS = [
 # scale epilogue reads every result with VALU instructions, which cannot
 # take accumulation registers (one v_accvgpr_read per value otherwise).
 SOURCE_FLAGS = {src: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-                for src in ("gemm.hip", "gemm_f16.hip", "gemm_f6.hip", "gemm_float.hip", "paged.hip", "gemm_i8r.hip",
+                for src in ("gemm.hip", "gemm_f16.hip", "gemm_f6.hip", "gemm_float.hip", "gemm_i8r.hip",
+                            "paged_attention.hip",
                             UBENCH_SRC)}
 
 

@@ -1,4 +1,4 @@
-// How the paged attention deals its keys to workgroups. Host code alone,
+// How the paged attention deals rows and keys to workgroups. Host code alone,
 // without HIP.
 #pragma once
 
@@ -7,40 +7,65 @@
 
 namespace dnx {
 
-// A row is one query head of one token. A workgroup takes kRowsBlock rows
-// that share a key head, and a run of the prefix's keys (`prefix_run`,
-// prefix_splits of them) or of one sequence's own keys (own_run, own_splits).
-// The rows' partial results are added by a second launch unless there is one
-// run in all.
+// A row is one query head of one token. A workgroup takes a block of rows that
+// share a key head and a run of keys: of the prefix (all tokens' rows), or of
+// one sequence's own keys (that sequence's rows). `wide` blocks hold 64 rows,
+// 16 a wave, whose waves share the keys' tiles; the others 16 rows, of which
+// each wave takes other keys. The rows' partial results are added by a second
+// launch unless there is one run in all.
+struct PagedPart {
+  bool wide;
+  int64_t blocks, runs, keys;   // blocks of rows, runs of that many keys
+};
 struct PagedSplit {
-  int64_t prefix_rows, own_rows;     // blocks of rows: all tokens', one sequence's
-  int64_t prefix_splits, prefix_run;
-  int64_t own_splits, own_run;
-  int64_t splits() const { return prefix_splits + own_splits; }
+  PagedPart prefix, own;
+  int64_t splits() const { return prefix.runs + own.runs; }
 };
 
-constexpr int kPagedRows = 16;       // rows of a workgroup
-constexpr int kPagedStep = 64;       // keys a workgroup takes at once: 16 a wave
-constexpr int kPagedMaxSplits = 32;  // of the prefix, and of a sequence
+constexpr int kPagedNarrow = 16, kPagedWide = 64;   // rows of a workgroup
+constexpr int kPagedStep = 64;       // runs are whole steps
+constexpr int kPagedMaxRuns = 32;    // of the prefix, and of a sequence
+
+// Wide blocks read the keys for 64 rows at once and take fewer products, but
+// one after another; narrow ones of the same rows run side by side and find
+// the keys in the L2. So narrow up to 32 rows, and up to 128 where the whole
+// is small (us, narrow against wide; 32 query heads over 8 key heads, hd 128):
+// f32 64 rows x 512 keys 11.6 / 13.4, 64 x 2048 18.3 / 17.7, 64 x 8192 39.6 /
+// 30.9, 128 x 512 13.7 / 15.4, 128 x 2048 25 / 22; bf16 (whose narrow blocks
+// take the bf16 matrix cores too) 64 x 8192 19.9 / 21, 128 x 2048 14.9 / 15.9,
+// 128 x 8192 28.2 / 28.4.
+inline bool paged_wide(int64_t rows, int64_t units, int64_t keys, bool f32) {
+  if (rows <= 32) return false;
+  return rows > 128 || rows * keys * units > (f32 ? 1200000 : 4000000);
+}
+
+inline PagedPart paged_part(int64_t rows, int64_t units, int64_t keys, bool f32, int64_t least,
+                            int64_t most) {
+  PagedPart p{};
+  p.wide = paged_wide(rows, units, keys, f32);
+  const int64_t block = p.wide ? kPagedWide : kPagedNarrow;
+  p.blocks = (rows + block - 1) / block;
+  p.keys = kPagedStep;
+  if (keys <= 0 || units <= 0 || rows <= 0) return p;
+  // Runs that make about 256 workgroups, of `least` to `most` keys (24 calls,
+  // geometric mean: 11.5 us; with 128 or 512 workgroups, or 128 keys at
+  // least, 11.9 to 12.2).
+  const int64_t wgs = units * p.blocks;
+  int64_t runs = (256 + wgs - 1) / wgs;
+  runs = std::min(std::max(runs, (keys + most - 1) / most), std::max<int64_t>(1, keys / least));
+  runs = std::min<int64_t>(std::max<int64_t>(runs, 1), kPagedMaxRuns);
+  p.keys = ((keys + runs - 1) / runs + kPagedStep - 1) / kPagedStep * kPagedStep;
+  p.runs = (keys + p.keys - 1) / p.keys;
+  return p;
+}
 
 inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, int64_t group,
-                              int64_t kv_heads, int64_t prefix_len, int64_t max_len) {
-  auto blocks = [](int64_t rows) { return (rows + kPagedRows - 1) / kPagedRows; };
-  PagedSplit s{blocks(tokens * group), blocks(max_tokens * group), 0, kPagedStep, 0, kPagedStep};
-  // Runs that make about `target` workgroups, of at least two steps.
-  constexpr int64_t target = 512;
-  auto deal = [&](int64_t units, int64_t keys, int64_t& splits, int64_t& run) {
-    if (keys <= 0 || units <= 0) return;
-    const int64_t steps = (keys + kPagedStep - 1) / kPagedStep;
-    int64_t want = std::min<int64_t>((target + units - 1) / units, kPagedMaxSplits);
-    want = std::max<int64_t>(1, std::min(want, steps / 2));
-    const int64_t per = (steps + want - 1) / want;
-    run = per * kPagedStep;
-    splits = (steps + per - 1) / per;
-  };
-  deal(kv_heads * s.prefix_rows, prefix_len, s.prefix_splits, s.prefix_run);
-  deal(seqs * kv_heads * s.own_rows, max_len, s.own_splits, s.own_run);
-  return s;
+                              int64_t kv_heads, int64_t prefix_len, int64_t max_len, bool f32) {
+  // Without a prefix, keys that one workgroup walks in about the time of the
+  // second launch (3 us) stay in one run: up to 256.
+  const int64_t least = prefix_len == 0 && max_len <= 256 ? 256 : kPagedStep;
+  return {paged_part(tokens * group, kv_heads, prefix_len, f32, kPagedStep, 1 << 20),
+          paged_part(max_tokens * group, seqs * kv_heads, max_len, f32, least, 2048)};
 }
 
 }  // namespace dnx

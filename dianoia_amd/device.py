@@ -621,42 +621,83 @@ def matmul_q4(qs, scales, x, y, rows: int, cols: int, n: int, int8_inputs: bool,
 
 
 # ---- a batch of sequences at once: int8 rows and products, paged keys and values
+#
+# These run for a few microseconds, less than a careless launch takes from
+# Python: sizes are compared in place, and an operand is named only once one
+# is too small.
+
+def _device_of(t: torch.Tensor) -> int:
+    """The current device, which has to be the tensor's."""
+    d = t.get_device()
+    if d < 0:
+        raise ValueError("device launchers take CUDA (HIP) tensors")
+    if d != torch._C._cuda_getDevice():
+        raise ValueError(f"the tensor is on device {d}, not on the current one")
+    return d
+
+
+def _at(t: torch.Tensor | None, device: int) -> int | None:
+    """The pointer of a contiguous tensor on that device."""
+    if t is None:
+        return None
+    if t.get_device() != device:
+        raise ValueError("device launchers take tensors of one CUDA (HIP) device")
+    if not t.is_contiguous():
+        raise ValueError("device launchers take contiguous tensors")
+    return t.data_ptr()
+
+
+def _quantize_i8r(name: str, size: int, x, qs, scales, rows, cols, cols_pad, stream) -> None:
+    if x.nbytes < rows * cols * size or qs.nbytes < rows * cols_pad or scales.nbytes < rows * 4:
+        _need(name, x=(x, rows * cols * size), qs=(qs, rows * cols_pad), scales=(scales, rows * 4))
+    d = _device_of(x)
+    rc = getattr(_lib.load(), name)(_at(x, d), _at(qs, d), _at(scales, d), rows, cols, cols_pad,
+                                    _stream(stream))
+    if rc:
+        _check(rc, name)
+
 
 def quantize_i8r(x, qs, scales, rows: int, cols: int, cols_pad: int, stream=None) -> None:
     """fp32 rows -> int8 [rows][cols_pad] with one scale a row (value = code * scale)."""
-    _need("quantize_i8r", x=(x, rows * cols * 4), qs=(qs, rows * cols_pad),
-          scales=(scales, rows * 4))
-    _check(_lib.load().dnx_quantize_i8r(_ptr(x), _ptr(qs), _ptr(scales), rows, cols, cols_pad,
-                                        _stream(stream)), "dnx_quantize_i8r")
+    _quantize_i8r("dnx_quantize_i8r", 4, x, qs, scales, rows, cols, cols_pad, stream)
 
 
 def quantize_i8r_bf16(x, qs, scales, rows: int, cols: int, cols_pad: int, stream=None) -> None:
     """bf16 rows (weights as they lie in a file) -> int8 with one scale a row."""
-    _need("quantize_i8r_bf16", x=(x, rows * cols * 2), qs=(qs, rows * cols_pad),
-          scales=(scales, rows * 4))
-    _check(_lib.load().dnx_quantize_i8r_bf16(_ptr(x), _ptr(qs), _ptr(scales), rows, cols,
-                                             cols_pad, _stream(stream)), "dnx_quantize_i8r_bf16")
+    _quantize_i8r("dnx_quantize_i8r_bf16", 2, x, qs, scales, rows, cols, cols_pad, stream)
 
 
 def rms_norm_i8r(x, w, qs, scales, rows: int, cols: int, cols_pad: int, eps: float, m=None,
                  x_out=None, stream=None) -> None:
     """RMSNorm(s) * w as int8 with one scale a row; s = x, or x + m, which goes
     to x_out (x itself, m or another tensor)."""
-    _need("rms_norm_i8r", x=(x, rows * cols * 4), w=(w, cols * 4), qs=(qs, rows * cols_pad),
-          scales=(scales, rows * 4), m=(m, rows * cols * 4), x_out=(x_out, rows * cols * 4))
-    _check(_lib.load().dnx_rms_norm_i8r(_ptr(x), _ptr(m), _ptr(x_out), _ptr(w), _ptr(qs),
-                                        _ptr(scales), rows, cols, cols_pad, eps,
-                                        _stream(stream)), "dnx_rms_norm_i8r")
+    size = rows * cols * 4
+    if (x.nbytes < size or w.nbytes < cols * 4 or qs.nbytes < rows * cols_pad
+            or scales.nbytes < rows * 4 or (m is not None and m.nbytes < size)
+            or (x_out is not None and x_out.nbytes < size)):
+        _need("rms_norm_i8r", x=(x, size), w=(w, cols * 4), qs=(qs, rows * cols_pad),
+              scales=(scales, rows * 4), m=(m, size), x_out=(x_out, size))
+    d = _device_of(x)
+    rc = _lib.load().dnx_rms_norm_i8r(_at(x, d), _at(m, d), _at(x_out, d), _at(w, d), _at(qs, d),
+                                      _at(scales, d), rows, cols, cols_pad, eps, _stream(stream))
+    if rc:
+        _check(rc, "dnx_rms_norm_i8r")
 
 
 def gemm_i8r(w, w_scale, x, x_scale, y, rows: int, cols: int, n: int, stream=None) -> None:
     """y [n][rows] = the int8 rows x times the int8 rows w, each with its scale."""
-    _need("gemm_i8r", w=(w, rows * cols), w_scale=(w_scale, rows * 4), x=(x, n * cols),
-          x_scale=(x_scale, n * 4), y=(y, n * rows * 4))
-    _check(_lib.load().dnx_gemm_i8r(_ptr(w), _ptr(w_scale), _ptr(x), _ptr(x_scale), _ptr(y), rows,
-                                    cols, n, _stream(stream)), "dnx_gemm_i8r")
+    if (w.nbytes < rows * cols or w_scale.nbytes < rows * 4 or x.nbytes < n * cols
+            or x_scale.nbytes < n * 4 or y.nbytes < n * rows * 4):
+        _need("gemm_i8r", w=(w, rows * cols), w_scale=(w_scale, rows * 4), x=(x, n * cols),
+              x_scale=(x_scale, n * 4), y=(y, n * rows * 4))
+    d = _device_of(w)
+    rc = _lib.load().dnx_gemm_i8r(_at(w, d), _at(w_scale, d), _at(x, d), _at(x_scale, d),
+                                  _at(y, d), rows, cols, n, _stream(stream))
+    if rc:
+        _check(rc, "dnx_gemm_i8r")
 
 
+_F32, _I32 = torch.float32, torch.int32
 _CACHE_TYPES = {torch.float32: 0, torch.bfloat16: 1}   # DNX_F32, DNX_BF16
 
 
@@ -675,24 +716,25 @@ class PagedCache:
         if hd not in (64, 128) or not 0 < kv_heads <= 1024 or not 0 < pages * page <= 0x7fffffff:
             raise ValueError("PagedCache: hd 64 or 128, up to 1024 heads, below 2^31 places")
         self.keys, self.values = keys, values
-        self.kv_heads, self.hd = kv_heads, hd
-        self.struct = _lib.PagedCacheStruct(_ptr(keys), _ptr(values), pages, page, kv_heads, hd,
-                                            _CACHE_TYPES[keys.dtype])
+        self.page, self.kv_heads, self.hd = page, kv_heads, hd
+        self.device = keys.get_device()
+        self.struct = _lib.PagedCacheStruct(_ptr(keys), _at(values, self.device), pages, page,
+                                            kv_heads, hd, _CACHE_TYPES[keys.dtype])
         self.ref = ctypes.addressof(self.struct)
 
+    def check_device(self) -> int:
+        if self.device != torch._C._cuda_getDevice():
+            raise ValueError(f"the cache is on device {self.device}, not on the current one")
+        return self.device
 
-def _int32(what: str, t, *shape) -> int | None:
-    """The pointer of an int32 tensor with at least the elements of `shape`."""
-    if t is None:
-        return None
-    if t.dtype != torch.int32:
+
+def _ints(what: str, t, device: int, least: int) -> int:
+    """The pointer of an int32 tensor of at least that many numbers."""
+    if t.dtype is not _I32:
         raise ValueError(f"{what} is int32")
-    n = 1
-    for s in shape:
-        n *= s
-    if t.numel() < n:
-        raise ValueError(f"{what} holds {t.numel()} numbers, the batch needs {n}")
-    return _ptr(t)
+    if t.numel() < least:
+        raise ValueError(f"{what} holds {t.numel()} numbers, the batch needs {least}")
+    return _at(t, device)
 
 
 class PagedBatch:
@@ -711,26 +753,22 @@ class PagedBatch:
             raise ValueError("PagedBatch: a sequence at least, and no negative numbers")
         self.starts, self.lens, self.tables, self.prefix_pages = starts, lens, tables, prefix_pages
         self.tokens, self.prefix_len = tokens, prefix_len
+        self.device = d = starts.get_device()
+        if d < 0:
+            raise ValueError("PagedBatch: CUDA (HIP) tensors")
+        self.prefix_places = 0 if prefix_pages is None else prefix_pages.numel()
         self.struct = _lib.PagedBatchStruct(
-            _int32("starts", starts, seqs + 1), _int32("lens", lens, seqs),
-            _int32("tables", tables, seqs, tables.shape[1]), _int32("prefix_pages", prefix_pages, 0),
+            _ints("starts", starts, d, seqs + 1), _ints("lens", lens, d, seqs),
+            _ints("tables", tables, d, 0),
+            None if prefix_pages is None else _ints("prefix_pages", prefix_pages, d, 0),
             tables.shape[1], prefix_len, seqs, tokens, max_tokens, max_len)
         self.ref = ctypes.addressof(self.struct)
 
     def check(self, cache: PagedCache) -> None:
-        if self.prefix_len > 0 and (self.prefix_pages is None or self.prefix_pages.numel()
-                                    * cache.struct.page < self.prefix_len):
+        if self.prefix_len > self.prefix_places * cache.page:
             raise ValueError("PagedBatch: prefix_pages holds fewer pages than the prefix needs")
-
-
-def _head_rows(what: str, t: torch.Tensor, hd: int):
-    """(pointer, stride of a token) of float32 [n][heads][hd], heads and dims dense."""
-    if not t.is_cuda or t.dtype != torch.float32:
-        raise ValueError(f"{what} is a float32 CUDA (HIP) tensor")
-    if t.dim() != 3 or t.shape[2] != hd or t.stride(2) != 1 or t.stride(1) != hd:
-        raise ValueError(f"{what} is [n][heads][{hd}] with dense heads")
-    n = t.shape[0]
-    return t.data_ptr(), t.stride(0) if n > 1 else t.shape[1] * hd
+        if self.device != cache.device:
+            raise ValueError("PagedBatch: on another device than the cache")
 
 
 def paged_append(cache: PagedCache, k, v, positions, slots, rope=None, q=None, q_out=None,
@@ -739,29 +777,39 @@ def paged_append(cache: PagedCache, k, v, positions, slots, rope=None, q=None, q
     places `slots` of the cache (dnx_paged_append); with q [n][heads][hd] also
     the queries, normed and rotated, into q_out. q, k and v may be views of one
     projection's output. A slot of -1 leaves its token out."""
-    n, hd = k.shape[0], cache.hd
-    kp, ks = _head_rows("paged_append: k", k, hd)
-    vp, vs = _head_rows("paged_append: v", v, hd)
-    if k.shape[1] != cache.kv_heads or v.shape != k.shape:
-        raise ValueError("paged_append: k and v hold the cache's heads for the same tokens")
-    qp, qs, op, heads = None, 0, None, 0
+    hd, d = cache.hd, cache.check_device()
+    n, kv_heads, dims = k.shape
+    ks, vs = k.stride(), v.stride()
+    if (kv_heads != cache.kv_heads or dims != hd or v.shape != k.shape or k.dtype is not _F32
+            or v.dtype is not _F32 or ks[2] != 1 or ks[1] != hd or vs[2] != 1 or vs[1] != hd):
+        raise ValueError("paged_append: k and v are float32 [n][kv_heads][hd] with dense heads")
+    if k.get_device() != d or v.get_device() != d:
+        raise ValueError("paged_append: k and v are not on the cache's device")
+    qp = qo = None
+    qs = heads = rows = 0
     if q is not None:
-        qp, qs = _head_rows("paged_append: q", q, hd)
         heads = q.shape[1]
-        if q.shape[0] != n or q_out is None or q_out.dtype != torch.float32:
-            raise ValueError("paged_append: q of the same tokens, and a float32 q_out")
-        _need("paged_append", q_out=(q_out, n * heads * hd * 4))
-        op = _ptr(q_out)
-    _need("paged_append", q_norm=(q_norm, hd * 4), k_norm=(k_norm, hd * 4))
-    rows = 0
+        st = q.stride()
+        if (q.dtype is not _F32 or q.shape[0] != n or q.shape[2] != hd or st[2] != 1
+                or st[1] != hd or q.get_device() != d):
+            raise ValueError("paged_append: q is float32 [n][heads][hd] with dense heads")
+        if q_out is None or q_out.dtype is not _F32 or q_out.nbytes < n * heads * hd * 4:
+            raise ValueError("paged_append: q needs a float32 q_out [n][heads][hd]")
+        qp, qs, qo = q.data_ptr(), st[0] if n > 1 else heads * hd, _at(q_out, d)
+    for w in (q_norm, k_norm):
+        if w is not None and (w.dtype is not _F32 or w.nbytes < hd * 4):
+            raise ValueError("paged_append: a norm's weight is float32 [hd]")
     if rope is not None:
-        if rope.dim() != 2 or rope.shape[1] != hd or rope.dtype != torch.float32 or positions is None:
+        if rope.dtype is not _F32 or rope.dim() != 2 or rope.shape[1] != hd or positions is None:
             raise ValueError("paged_append: rope is float32 [positions][hd], with positions")
         rows = rope.shape[0]
-    _check(_lib.load().dnx_paged_append(
-        cache.ref, qp, qs, op, kp, ks, vp, vs, _ptr(q_norm), _ptr(k_norm), _ptr(rope), rows,
-        _int32("positions", positions, n), _int32("slots", slots, n), heads, n, eps,
-        _stream(stream)), "dnx_paged_append")
+    rc = _lib.load().dnx_paged_append(
+        cache.ref, qp, qs, qo, k.data_ptr(), ks[0] if n > 1 else kv_heads * hd, v.data_ptr(),
+        vs[0] if n > 1 else kv_heads * hd, _at(q_norm, d), _at(k_norm, d), _at(rope, d), rows,
+        None if positions is None else _ints("positions", positions, d, n),
+        _ints("slots", slots, d, n), heads, n, eps, _stream(stream))
+    if rc:
+        _check(rc, "dnx_paged_append")
 
 
 def paged_attention_workspace(cache: PagedCache, batch: PagedBatch, heads: int,
@@ -778,13 +826,17 @@ def paged_attention(cache: PagedCache, batch: PagedBatch, q, out, workspace, win
                     gate=None, stream=None) -> None:
     """Attention of the batch's new tokens q [tokens][heads][hd] over the shared
     prefix and each sequence's own pages, into out (dnx_paged_attention)."""
-    if q.dim() != 3 or q.shape[0] != batch.tokens or q.shape[2] != cache.hd:
-        raise ValueError("paged_attention: q is [tokens][heads][hd]")
-    if q.dtype != torch.float32 or out.dtype != torch.float32:
-        raise ValueError("paged_attention: q and out are float32")
-    heads = q.shape[1]
+    d = cache.check_device()
     batch.check(cache)
-    _need("paged_attention", out=(out, q.nbytes), gate=(gate, batch.tokens * heads * 4))
-    _check(_lib.load().dnx_paged_attention(cache.ref, batch.ref, _ptr(q), _ptr(gate), _ptr(out),
-                                           heads, window, _ptr(workspace), workspace.nbytes,
-                                           _stream(stream)), "dnx_paged_attention")
+    n, heads, hd = q.shape
+    if n != batch.tokens or hd != cache.hd or q.dtype is not _F32 or out.dtype is not _F32:
+        raise ValueError("paged_attention: q and out are float32 [tokens][heads][hd]")
+    if out.nbytes < q.nbytes or (gate is not None and (gate.nbytes < n * heads * 4
+                                                       or gate.dtype is not _F32)):
+        _need("paged_attention", out=(out, q.nbytes), gate=(gate, n * heads * 4))
+        raise ValueError("paged_attention: gate is float32 [tokens][heads]")
+    rc = _lib.load().dnx_paged_attention(cache.ref, batch.ref, _at(q, d), _at(gate, d), _at(out, d),
+                                         heads, window, _at(workspace, d), workspace.nbytes,
+                                         _stream(stream))
+    if rc:
+        _check(rc, "dnx_paged_attention")

@@ -605,10 +605,11 @@ typedef struct {
 // [heads] or null: the output times sigmoid(gate), as dnx_attention's. The
 // prefix's keys are read once for all sequences. Keys in a page outside the
 // cache are not seen, a row without any weight (no key seen) is zeros, and
-// what lies in masked places (infinities, NaN) does not matter. float32
-// arithmetic throughout. workspace: dnx_paged_attention_workspace_bytes of
-// device memory (the partial results of runs of keys), 16-byte aligned; calls
-// that overlap need one each. The two structs are read at the call.
+// what lies in masked places (infinities, NaN) does not matter, but for the
+// last bits of rows that share a step with it. float32 accuracy throughout.
+// workspace: dnx_paged_attention_workspace_bytes of device memory (the partial
+// results of runs of keys), 16-byte aligned; calls that overlap need one each.
+// The two structs are read at the call.
 int64_t dnx_paged_attention_workspace_bytes(const dnx_paged_cache* cache,
                                             const dnx_paged_batch* batch, int64_t heads);
 int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* batch,

@@ -246,6 +246,9 @@ CASES = [
     ([3, 3], [3, 3], 4100, 8, 2, 128, 256),
     ([1] * 40, list(range(1, 41)), 520, 16, 2, 128, 16),
     ([1, 1], [3000, 1500], 0, 4, 4, 128, 128),
+    ([1] * 40, [30] * 40, 1500, 16, 2, 128, 64),
+    ([200, 1, 90], [333, 70, 90], 190, 4, 2, 64, 32),
+    ([150], [700], 64, 3, 1, 128, 16),
 ]
 
 
@@ -304,28 +307,33 @@ def test_keys_past_the_bounds_are_not_seen(gpu_ready):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
-def test_infinities_behind_the_mask(gpu_ready, kind):
+@pytest.mark.parametrize("heads,kv,hd,page", [(4, 2, 64, 16), (64, 2, 64, 64), (64, 1, 128, 16),
+                                              (64, 1, 128, 128)])
+def test_infinities_behind_the_mask(gpu_ready, heads, kv, hd, page, kind):
     """An infinity or NaN among the keys or values of a later token does not
-    reach the earlier ones; where it is seen, it follows the formula."""
+    reach the earlier ones; where it is seen, it follows the formula. The rows
+    next to it may be formed by other instructions (float32 products in place
+    of pieces), each within the bound of the formula on the clean cache."""
     counts, lens, prefix = [6], [40], 50
-    clean = Batch(8, counts, lens, prefix, 4, 2, 64, kind, 16)
-    want = host(clean.run()).copy()
+    make = lambda: Batch(8, counts, lens, prefix, heads, kv, hd, kind, page)
+    want, room = make().expected()
+    near = lambda got, at: (np.abs(got - want[at]) <= room[at]).all()
     for what in ("keys", "values"):
         for bad in (np.inf, -np.inf, np.nan):
             b = Batch(8, counts, lens, prefix, 4, 2, 64, kind, 16)
             j = 37                                  # seen by tokens 3, 4 and 5 (places 37 .. 39)
             getattr(b, what)[int(b.tables_h[0, j // 16]), j % 16, :, 5] = bad
             out = host(b.run())
-            assert np.array_equal(out[:3], want[:3]), (what, bad)
+            assert near(out[:3], np.s_[:3]), (what, bad)
             if what == "values":
-                assert np.array_equal(out[3:, :, :5], want[3:, :, :5])
+                assert near(out[3:, :, :5], np.s_[3:, :, :5])
                 got = out[3:, :, 5]
                 assert (np.isnan(got) if np.isnan(bad) else got == bad).all()
-    b = Batch(8, counts, lens, prefix, 4, 2, 64, kind, 16)   # a window hides the prefix's first keys
-    full = host(b.run(60)).copy()
+    b = make()                                  # a window hides the prefix's first keys
+    want, room = b.expected(60)
     for t in (b.keys, b.values):
         t[int(b.shared[0]), :2] = float("nan")
-    assert np.array_equal(host(b.run(60)), full)
+    assert near(host(b.run(60)), np.s_[:])
 
 
 def test_scores_that_overflow(gpu_ready):

@@ -14,10 +14,11 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SOURCE = """
 #include "paged_split.h"
 extern "C" void split_of(int64_t seqs, int64_t tokens, int64_t max_tokens, int64_t group,
-                         int64_t kv_heads, int64_t prefix, int64_t len, int64_t* out) {
-  const dnx::PagedSplit s = dnx::paged_split(seqs, tokens, max_tokens, group, kv_heads, prefix, len);
-  const int64_t v[] = {s.prefix_rows, s.own_rows, s.prefix_splits, s.prefix_run, s.own_splits,
-                       s.own_run, s.splits()};
+                         int64_t kv_heads, int64_t prefix, int64_t len, int64_t f32, int64_t* out) {
+  const dnx::PagedSplit s =
+      dnx::paged_split(seqs, tokens, max_tokens, group, kv_heads, prefix, len, f32 != 0);
+  const int64_t v[] = {s.prefix.blocks, s.own.blocks, s.prefix.runs, s.prefix.keys, s.own.runs,
+                       s.own.keys, s.splits()};
   for (int i = 0; i < 7; i++) out[i] = v[i];
 }
 """
@@ -31,7 +32,7 @@ def split_of(tmp_path_factory):
     subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-o", so, str(d / "s.cpp"),
                     "-I", os.path.join(ROOT, "dianoia_amd", "csrc")], check=True)
     f = ctypes.CDLL(so).split_of
-    f.argtypes, f.restype = [ctypes.c_int64] * 7 + [ctypes.c_void_p], None
+    f.argtypes, f.restype = [ctypes.c_int64] * 8 + [ctypes.c_void_p], None
 
     def call(*args):
         out = (ctypes.c_int64 * 7)()
@@ -41,11 +42,12 @@ def split_of(tmp_path_factory):
 
 
 def test_every_key_has_a_run(split_of):
-    for seqs, each, group, kv, prefix, length in itertools.product(
+    for seqs, each, group, kv, prefix, length, f32 in itertools.product(
             (1, 3, 64, 300), (1, 5, 70), (1, 3, 8, 33), (1, 2, 8), (0, 1, 63, 65, 777, 8192, 200000),
-            (0, 1, 64, 500, 2048, 100000)):
+            (0, 1, 64, 500, 2048, 100000), (0, 1)):
         tokens = seqs * each
-        pr, orows, ps, prun, os_, orun, total = split_of(seqs, tokens, each, group, kv, prefix, length)
+        pr, orows, ps, prun, os_, orun, total = split_of(seqs, tokens, each, group, kv, prefix, length,
+                                                        f32)
         assert total == ps + os_ <= 64
         for keys, splits, run in ((prefix, ps, prun), (length, os_, orun)):
             assert run % 64 == 0 and run > 0
