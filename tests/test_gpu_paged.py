@@ -320,9 +320,9 @@ def test_infinities_behind_the_mask(gpu_ready, heads, kv, hd, page, kind):
     near = lambda got, at: (np.abs(got - want[at]) <= room[at]).all()
     for what in ("keys", "values"):
         for bad in (np.inf, -np.inf, np.nan):
-            b = Batch(8, counts, lens, prefix, 4, 2, 64, kind, 16)
+            b = make()
             j = 37                                  # seen by tokens 3, 4 and 5 (places 37 .. 39)
-            getattr(b, what)[int(b.tables_h[0, j // 16]), j % 16, :, 5] = bad
+            getattr(b, what)[int(b.tables_h[0, j // page]), j % page, :, 5] = bad
             out = host(b.run())
             assert near(out[:3], np.s_[:3]), (what, bad)
             if what == "values":
