@@ -270,6 +270,24 @@ def test_window(gpu_ready, window, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [0, 70, 700])
+def test_many_sequences_of_unequal_lengths(gpu_ready, window, kind):
+    """Sequences without tokens, without keys, of one key, of whole steps, and one
+    that is most of the batch; a bound on the lengths that is far above them."""
+    rng = np.random.default_rng(17)
+    lens = rng.choice([0, 1, 5, 63, 64, 65, 128, 200, 333, 900], 130).tolist()
+    counts = [min(int(c), max(n, 1)) for c, n in zip(rng.choice([0, 1, 1, 1, 2, 8], 130), lens)]
+    Batch(20, counts, lens, 100, 4, 2, 64, kind, 16, pad=3, gate=True).check(window)
+    one = [0] * 40 + [1] + [0] * 88 + [1]
+    Batch(21, one, [2000 if c else 0 for c in one], 0, 4, 2, 128, kind, 64).check(window)
+    Batch(22, [1] * 64, list(range(64)), 0, 8, 4, 64, kind, 16, max_len=100000).check(window)
+    for seqs in (256, 257):
+        lens = [int(n) for n in rng.integers(0, 40, seqs)]
+        lens[3] = lens[-1] = 600
+        Batch(seqs, [1] * seqs, lens, 65, 2, 1, 64, kind, 32).check(window)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_rows_without_keys_are_zeros(gpu_ready, kind):
     """A token that stands before its sequence's first own key, and no prefix."""
     b = Batch(3, [1, 2, 1], [0, 1, 20], 0, 4, 2, 64, kind, 16, pad=2)
