@@ -248,6 +248,9 @@ DNX_DEV uint4 buffer_load16(i32x4 rsrc, int offset) {
   return make_uint4((uint32_t)v.x, (uint32_t)v.y, (uint32_t)v.z, (uint32_t)v.w);
 }
 
+// The threads that a launch may have, all its workgroups together.
+constexpr int64_t kLaunchThreads = 0xffffffff;
+
 // Cache-policy immediate of a buffer load on gfx950: the non-temporal bit.
 // Weights read once per call stream through the caches without being kept:
 // on the 350 MB LM head this took the GEMV from 69 to 61 us.

@@ -253,14 +253,17 @@ __global__ void __launch_bounds__(KG * WM * WN * 64) gemm_i8r_tile_kernel(I8RArg
 }
 
 template <int I, int WM, int WN, int MT, int NT, int RING>
-void launch_tile(const I8RArgs& p, hipStream_t st) {
+int launch_tile(const I8RArgs& p, hipStream_t st) {
   constexpr I8RTile T = kI8RTiles[I];
   static_assert(T.tokens == WM * MT * 32 && T.rows == WN * NT * 32, "the route's tile");
   const int64_t tiles_t = (p.n + T.tokens - 1) / T.tokens;
   const int64_t tiles = tiles_t * ((p.rows + T.rows - 1) / T.rows);
-  hipLaunchKernelGGL((gemm_i8r_tile_kernel<WM, WN, MT, NT, RING, T.parts>),
-                     dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(T.parts * WM * WN * 64), 0, st, p,
-                     (int)tiles_t, (int)tiles);
+  constexpr int kThreads = T.parts * WM * WN * 64;
+  const int64_t grid = (tiles + 7) / 8 * 8;
+  if (grid > kLaunchThreads / kThreads) return DNX_EINVAL;
+  hipLaunchKernelGGL((gemm_i8r_tile_kernel<WM, WN, MT, NT, RING, T.parts>), dim3((unsigned)grid),
+                     dim3(kThreads), 0, st, p, (int)tiles_t, (int)tiles);
+  return hipGetLastError() == hipSuccess ? DNX_OK : DNX_ELAUNCH;
 }
 
 }  // namespace
@@ -269,7 +272,7 @@ extern "C" {
 
 int dnx_gemm_i8r(const int8_t* w, const float* w_scale, const int8_t* x, const float* x_scale,
                  float* y, int64_t rows, int64_t cols, int64_t n, dnx_stream_t stream) {
-  if (rows <= 0 || rows > (1 << 30) || n < 0 || n > (1 << 22) || cols <= 0 ||
+  if (rows <= 0 || rows >= (1 << 22) || n < 0 || n >= (1 << 22) || cols <= 0 ||
       cols % kBlock != 0 || cols > kMaxK) {
     return DNX_EINVAL;
   }
@@ -282,18 +285,16 @@ int dnx_gemm_i8r(const int8_t* w, const float* w_scale, const int8_t* x, const f
   const I8RArgs p{w, w_scale, x, x_scale, y, (int)rows, (int)cols, (int)n};
   const hipStream_t st = (hipStream_t)stream;
   switch (i8r_route(n, rows, cols)) {
-    case kI8RFew:
-      hipLaunchKernelGGL(gemm_i8r_few_kernel, dim3((unsigned)((rows + kFewRows - 1) / kFewRows)),
-                         dim3(kFewWaves * 64), 0, st, p);
-      break;
-    case 0: launch_tile<0, 1, 1, 1, 1, 4>(p, st); break;
-    case 1: launch_tile<1, 2, 1, 1, 1, 4>(p, st); break;
-    case 2: launch_tile<2, 2, 2, 1, 1, 8>(p, st); break;
-    case 3: launch_tile<3, 2, 2, 2, 1, 4>(p, st); break;
-    case 4: launch_tile<4, 2, 2, 2, 2, 3>(p, st); break;
-    case 5: launch_tile<5, 4, 2, 2, 2, 3>(p, st); break;
-    default: launch_tile<6, 4, 4, 2, 2, 5>(p, st); break;
+    case 0: return launch_tile<0, 1, 1, 1, 1, 4>(p, st);
+    case 1: return launch_tile<1, 2, 1, 1, 1, 4>(p, st);
+    case 2: return launch_tile<2, 2, 2, 1, 1, 8>(p, st);
+    case 3: return launch_tile<3, 2, 2, 2, 1, 4>(p, st);
+    case 4: return launch_tile<4, 2, 2, 2, 2, 3>(p, st);
+    case 5: return launch_tile<5, 4, 2, 2, 2, 3>(p, st);
+    case 6: return launch_tile<6, 4, 4, 2, 2, 5>(p, st);
   }
+  hipLaunchKernelGGL(gemm_i8r_few_kernel, dim3((unsigned)((rows + kFewRows - 1) / kFewRows)),
+                     dim3(kFewWaves * 64), 0, st, p);
   return hipGetLastError() == hipSuccess ? DNX_OK : DNX_ELAUNCH;
 }
 

@@ -133,7 +133,7 @@ int dnx_paged_append(const dnx_paged_cache* cache, const float* q, int64_t q_str
   const int64_t units = n * ((q != nullptr ? heads : 0) + 2 * cache->kv_heads);
   const int64_t per = kThreads / (cache->hd / 8);
   const int64_t grid = (units + per - 1) / per;
-  if (grid > 0x7fffffff) return DNX_EINVAL;
+  if (grid > kLaunchThreads / kThreads) return DNX_EINVAL;
   auto k_ = cache->type == DNX_F32
                 ? (cache->hd == 128 ? append_kernel<float, 128> : append_kernel<float, 64>)
                 : (cache->hd == 128 ? append_kernel<uint16_t, 128> : append_kernel<uint16_t, 64>);

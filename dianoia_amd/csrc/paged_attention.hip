@@ -88,7 +88,8 @@ DNX_DEV Seen row_sees(const PagedArgs& a, const Item& w, int r) {
     const int mid = (lo + hi) / 2;
     if (a.starts[mid] <= token) lo = mid; else hi = mid;
   }
-  return {a.prefix_len + a.lens[lo] - a.starts[lo + 1] + token - a.window + 1, w.count};
+  const int place = a.prefix_len + a.lens[lo] - a.starts[lo + 1] + token;
+  return {max(place, 0) - a.window + 1, w.count};
 }
 
 // 16 keys of an item from kt on (a page holds whole sixteens) as resources
@@ -993,7 +994,7 @@ extern "C" {
 int64_t dnx_paged_attention_workspace_bytes(const dnx_paged_cache* cache,
                                             const dnx_paged_batch* batch, int64_t heads) {
   if (!cache_ok(cache) || !batch_ok(batch) || heads <= 0 || heads % cache->kv_heads != 0 ||
-      heads > 65535 || batch->tokens * heads > (1 << 30)) {
+      heads > 65535 || batch->tokens * heads >= (1 << 26)) {
     return -1;
   }
   const int64_t splits = split_of(cache, batch, heads).splits();
@@ -1047,7 +1048,7 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
   a.prefix_items = items(s.prefix, 1);
   a.scale = (float)(1.0 / sqrt((double)cache->hd));
   const int64_t grid = a.prefix_items + items(s.own, batch->seqs);
-  if (grid > 0x7fffffff) return DNX_EINVAL;
+  if (grid > kLaunchThreads / kThreads) return DNX_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
   if (grid > 0) {
     auto k = cache->type == DNX_F32 ? (cache->hd == 128 ? paged_attention_kernel<float, 128>
@@ -1059,7 +1060,6 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
   }
   if (a.splits != 1) {
     const int64_t blocks = (batch->tokens * heads + kWaves - 1) / kWaves;
-    if (blocks > 0x7fffffff) return DNX_EINVAL;
     auto k = cache->hd == 128 ? paged_combine_kernel<128> : paged_combine_kernel<64>;
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(kThreads), 0, st, a);
   }

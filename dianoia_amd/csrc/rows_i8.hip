@@ -29,6 +29,7 @@ namespace {
 constexpr int kMaxThreads = 1024;
 constexpr int kMaxV = 16;                                // four values each, per thread
 constexpr int64_t kManyRows = 512;
+constexpr int64_t kMaxRows = 1 << 22;                    // 2^32 threads in a launch
 constexpr int64_t kMaxCols = (int64_t)kMaxThreads * kMaxV * 4;
 
 // A wave's sum and maximum in 64 bits, and the maximum of unsigned words, on
@@ -193,7 +194,7 @@ template <typename S, bool kNorm, bool kAdd>
 int launch_rows(const S* x, const float* m, float* x_out, const float* w, int8_t* qs,
                 float* scales, int64_t rows, int64_t cols, int64_t cols_pad, float eps,
                 dnx_stream_t stream) {
-  if (rows < 0 || rows > 0x7fffffff || cols <= 0 || cols % 4 != 0 || cols > kMaxCols ||
+  if (rows < 0 || rows >= kMaxRows || cols <= 0 || cols % 4 != 0 || cols > kMaxCols ||
       cols_pad < cols || cols_pad % kBlock != 0 || cols_pad > kMaxCols) {
     return DNX_EINVAL;
   }

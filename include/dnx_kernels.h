@@ -521,10 +521,10 @@ int dnx_steer(float* x, const float* v, int64_t rows, int64_t cols, int64_t mode
 // int8 rows with one float32 scale each, value = code * scale: scale is the
 // row's largest |value| / 127, each code the nearest whole number, halves away
 // from zero, codes past `cols` zero (cols_pad a multiple of 32 >= cols, cols a
-// multiple of 4 up to 65536). Activations (rows = tokens) and weights (rows =
-// output channels) alike; _bf16 takes bf16 rows, as weights lie in a file. A
-// row that holds an infinity or NaN gets a NaN scale (and zero codes). Pointers
-// 16-byte aligned (scales 4).
+// multiple of 4 up to 65536, below 2^22 rows). Activations (rows = tokens) and
+// weights (rows = output channels) alike; _bf16 takes bf16 rows, as weights lie
+// in a file. A row that holds an infinity or NaN gets a NaN scale (and zero
+// codes). Pointers 16-byte aligned (scales 4).
 int dnx_quantize_i8r(const float* x, int8_t* qs, float* scales, int64_t rows, int64_t cols,
                      int64_t cols_pad, dnx_stream_t stream);
 int dnx_quantize_i8r_bf16(const uint16_t* x, int8_t* qs, float* scales, int64_t rows, int64_t cols,
@@ -537,8 +537,8 @@ int dnx_rms_norm_i8r(const float* x, const float* m, float* x_out, const float* 
                      dnx_stream_t stream);
 // y[t][r] = x_scale[t] w_scale[r] sum_k x[t][k] w[r][k] on such rows: exact
 // integer sums, y [n][rows] float32 rounded from them. cols a multiple of 32
-// up to 131040 (the width the rows were written with), any n and rows; w and x
-// 16-byte aligned.
+// up to 131040 (the width the rows were written with), n and rows below 2^22;
+// w and x 16-byte aligned.
 int dnx_gemm_i8r(const int8_t* w, const float* w_scale, const int8_t* x, const float* x_scale,
                  float* y, int64_t rows, int64_t cols, int64_t n, dnx_stream_t stream);
 
@@ -579,9 +579,11 @@ int dnx_paged_append(const dnx_paged_cache* cache, const float* q, int64_t q_str
 // prefix_pages, are shared: every sequence begins with them. Sequence b's own
 // keys follow, lens[b] of them (its new tokens' among them) in the pages
 // tables[b * table_stride ..]; its new tokens are the rows starts[b] ..
-// starts[b + 1] - 1 of the call (starts[0] = 0; none, one or many). tokens is
-// the number of rows, which may be more than starts[seqs]: rows behind the
-// last sequence's are neither read nor written. The arrays lie in device
+// starts[b + 1] - 1 of the call (starts[0] = 0; none, one or many). Where lens
+// is less than their number, the first of them have no own key: they see the
+// prefix alone. tokens is the number of rows (tokens * heads below 2^26), which
+// may be more than starts[seqs]: rows behind the last sequence's are neither
+// read nor written. The arrays lie in device
 // memory and may change from call to call under one captured graph; the
 // numbers here bound them: no sequence has more than max_tokens new tokens,
 // and own keys past max_len or past the table are not seen.

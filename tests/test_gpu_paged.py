@@ -298,6 +298,22 @@ def test_rows_without_keys_are_zeros(gpu_ready, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_more_tokens_than_own_keys(gpu_ready, kind):
+    """The first of them see the prefix alone, under the widest window too."""
+    b = Batch(9, [3], [1], 50, 4, 2, 64, kind, 16)
+    want, room = b.expected()                      # of the last, which sees all 51 keys
+    longer = Batch(9, [1], [0], 50, 4, 2, 64, kind, 16)
+    for window in (0, 0x7fffffff):
+        out = host(b.run(window))
+        assert (np.abs(out[2] - want[2]) <= room[2]).all()
+        for i in (0, 1):
+            longer.q.copy_(b.q[i:i + 1])
+            longer.first_kv = b.first_kv
+            got, bound = longer.expected()
+            assert (np.abs(out[i] - got[0]) <= bound[0]).all(), (window, i)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_pages_outside_the_cache_are_not_seen(gpu_ready, kind):
     b = Batch(4, [1, 3], [100, 90], 64, 8, 4, 128, kind, 16)
     b.tables[0, 2], b.tables[1, 0] = -1, b.keys.shape[0]

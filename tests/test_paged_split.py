@@ -118,6 +118,31 @@ def test_workspace_and_refusals():
     assert append(n=0) == 0
 
 
+def test_limits_of_sizes():
+    """Sizes whose products leave 32 or 64 bits, or a launch's threads, are
+    refused; none of these calls launches."""
+    from dianoia_amd import _lib
+    lib = _lib.load()
+    a = 4096
+
+    def size(tokens=8, heads=4, pages=64, prefix=100, length=64):
+        c = _lib.PagedCacheStruct(keys=a, values=a, pages=pages, page=16, kv_heads=2, hd=64, type=0)
+        b = _lib.PagedBatchStruct(starts=a, lens=a, tables=a, prefix_pages=a, table_stride=4,
+                                  prefix_len=prefix, seqs=3, tokens=tokens, max_tokens=1, max_len=length)
+        return lib.dnx_paged_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(b), heads)
+
+    assert size() > 0 and size(tokens=1 << 22, heads=14) > 0
+    assert size(tokens=1 << 22, heads=16) == -1
+    for pages in (1 << 27, 1 << 60, (1 << 60) + 1):
+        assert size(pages=pages) == -1
+    assert size(prefix=1 << 30, length=1 << 30) == -1
+    for rows in (1 << 22, 1 << 40):
+        assert lib.dnx_quantize_i8r(a, a, a, rows, 64, 64, None) == -1
+        assert lib.dnx_gemm_i8r(a, a, a, a, a, rows, 64, 2, None) == -1
+        assert lib.dnx_gemm_i8r(a, a, a, a, a, 8, 64, rows, None) == -1
+    assert lib.dnx_gemm_i8r(a, a, a, a, a, (1 << 22) - 1, 64, (1 << 22) - 1, None) == -1
+
+
 def test_python_refusals():
     import torch
 
