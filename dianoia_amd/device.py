@@ -728,13 +728,13 @@ class PagedCache:
         return self.device
 
 
-def _ints(what: str, t, device: int, least: int) -> int:
-    """The pointer of an int32 tensor of at least that many numbers."""
-    if t.dtype is not _I32:
-        raise ValueError(f"{what} is int32")
-    if t.numel() < least:
-        raise ValueError(f"{what} holds {t.numel()} numbers, the batch needs {least}")
-    return _at(t, device)
+def _numbers(what: str, t, device: int, least: int, dtype) -> int:
+    """The pointer of a contiguous tensor of that type, with that many numbers."""
+    if (t.dtype is not dtype or t.numel() < least or t.get_device() != device
+            or not t.is_contiguous()):
+        raise ValueError(f"{what}: a contiguous {dtype} tensor on device {device}, of {least} "
+                         f"numbers at least")
+    return t.data_ptr()
 
 
 class PagedBatch:
@@ -758,9 +758,9 @@ class PagedBatch:
             raise ValueError("PagedBatch: CUDA (HIP) tensors")
         self.prefix_places = 0 if prefix_pages is None else prefix_pages.numel()
         self.struct = _lib.PagedBatchStruct(
-            _ints("starts", starts, d, seqs + 1), _ints("lens", lens, d, seqs),
-            _ints("tables", tables, d, 0),
-            None if prefix_pages is None else _ints("prefix_pages", prefix_pages, d, 0),
+            _numbers("starts", starts, d, seqs + 1, _I32), _numbers("lens", lens, d, seqs, _I32),
+            _numbers("tables", tables, d, 0, _I32),
+            None if prefix_pages is None else _numbers("prefix_pages", prefix_pages, d, 0, _I32),
             tables.shape[1], prefix_len, seqs, tokens, max_tokens, max_len)
         self.ref = ctypes.addressof(self.struct)
 
@@ -777,37 +777,43 @@ def paged_append(cache: PagedCache, k, v, positions, slots, rope=None, q=None, q
     places `slots` of the cache (dnx_paged_append); with q [n][heads][hd] also
     the queries, normed and rotated, into q_out. q, k and v may be views of one
     projection's output. A slot of -1 leaves its token out."""
-    hd, d = cache.hd, cache.check_device()
-    n, kv_heads, dims = k.shape
-    ks, vs = k.stride(), v.stride()
-    if (kv_heads != cache.kv_heads or dims != hd or v.shape != k.shape or k.dtype is not _F32
-            or v.dtype is not _F32 or ks[2] != 1 or ks[1] != hd or vs[2] != 1 or vs[1] != hd):
+    d = cache.check_device()
+    shape = k.shape
+    n, kv_heads, hd = shape
+    ks, k1, k2 = k.stride()
+    vs, v1, v2 = v.stride()
+    if (kv_heads != cache.kv_heads or hd != cache.hd or v.shape != shape or k.dtype is not _F32
+            or v.dtype is not _F32 or k2 != 1 or k1 != hd or v2 != 1 or v1 != hd):
         raise ValueError("paged_append: k and v are float32 [n][kv_heads][hd] with dense heads")
     if k.get_device() != d or v.get_device() != d:
         raise ValueError("paged_append: k and v are not on the cache's device")
-    qp = qo = None
+    qp = qo = kw = qw = table = at = None
     qs = heads = rows = 0
     if q is not None:
-        heads = q.shape[1]
-        st = q.stride()
-        if (q.dtype is not _F32 or q.shape[0] != n or q.shape[2] != hd or st[2] != 1
-                or st[1] != hd or q.get_device() != d):
+        tokens, heads, dims = q.shape
+        qs, q1, q2 = q.stride()
+        if (tokens != n or dims != hd or q.dtype is not _F32 or q2 != 1 or q1 != hd
+                or q.get_device() != d):
             raise ValueError("paged_append: q is float32 [n][heads][hd] with dense heads")
-        if q_out is None or q_out.dtype is not _F32 or q_out.nbytes < n * heads * hd * 4:
+        if q_out is None:
             raise ValueError("paged_append: q needs a float32 q_out [n][heads][hd]")
-        qp, qs, qo = q.data_ptr(), st[0] if n > 1 else heads * hd, _at(q_out, d)
-    for w in (q_norm, k_norm):
-        if w is not None and (w.dtype is not _F32 or w.nbytes < hd * 4):
-            raise ValueError("paged_append: a norm's weight is float32 [hd]")
+        qp, qo = q.data_ptr(), _numbers("q_out", q_out, d, n * heads * hd, _F32)
+    if k_norm is not None:
+        kw = _numbers("k_norm", k_norm, d, hd, _F32)
+    if q_norm is not None:
+        qw = _numbers("q_norm", q_norm, d, hd, _F32)
     if rope is not None:
-        if rope.dtype is not _F32 or rope.dim() != 2 or rope.shape[1] != hd or positions is None:
+        rows, dims = rope.shape
+        if dims != hd or positions is None:
             raise ValueError("paged_append: rope is float32 [positions][hd], with positions")
-        rows = rope.shape[0]
+        table = _numbers("rope", rope, d, 0, _F32)
+    if positions is not None:
+        at = _numbers("positions", positions, d, n, _I32)
+    if n == 1:      # a lone row's stride is anything
+        qs, ks, vs = heads * hd, kv_heads * hd, kv_heads * hd
     rc = _lib.load().dnx_paged_append(
-        cache.ref, qp, qs, qo, k.data_ptr(), ks[0] if n > 1 else kv_heads * hd, v.data_ptr(),
-        vs[0] if n > 1 else kv_heads * hd, _at(q_norm, d), _at(k_norm, d), _at(rope, d), rows,
-        None if positions is None else _ints("positions", positions, d, n),
-        _ints("slots", slots, d, n), heads, n, eps, _stream(stream))
+        cache.ref, qp, qs, qo, k.data_ptr(), ks, v.data_ptr(), vs, qw, kw, table, rows, at,
+        _numbers("slots", slots, d, n, _I32), heads, n, eps, _stream(stream))
     if rc:
         _check(rc, "dnx_paged_append")
 
