@@ -27,7 +27,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr float kSlack = 8.0f;   // of a running maximum, in units of log2
 
 struct PartArgs {
-  int wide, blocks, runs, keys;
+  int wide, few, blocks, runs, keys;
 };
 
 struct PagedArgs {
@@ -335,6 +335,45 @@ DNX_DEV void write_row4(const PagedArgs& a, const Item& w, int64_t row, int hd, 
   }
 }
 
+// Rows of four waves' sums in LDS: [wave][16][kSumRow] and, behind them, each
+// wave's maxima and sums of weights [wave][2][16].
+template <int HD>
+constexpr int kSumRow = HD + 4;
+template <int HD>
+DNX_DEV float* wave_stats(uint8_t* lds, int wave) {
+  return (float*)lds + kWaves * 16 * kSumRow<HD> + wave * 32;
+}
+
+template <int HD>
+constexpr int kMergeBytes = kWaves * (16 * kSumRow<HD> + 32) * 4;
+
+// The four waves' sums of the first N rows, added in wave order.
+template <int HD, int N>
+DNX_DEV void merge_waves(const PagedArgs& a, const Item& w, uint8_t* lds) {
+  const float* all = (const float*)lds;
+  const float* ml = wave_stats<HD>(lds, 0);
+  __syncthreads();
+  for (int i = threadIdx.x; i < N * HD / 4; i += kThreads) {
+    const int r = i / (HD / 4), c = i % (HD / 4);
+    if (w.row0 + r >= w.rows) break;
+    float top = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWaves; k++) top = fmaxf(top, ml[2 * k * 16 + r]);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < kWaves; k++) {
+      const float l = ml[(2 * k + 1) * 16 + r];
+      if (l == 0.0f) continue;
+      const float f = partial_factor(ml[2 * k * 16 + r], l, top);
+      const float4 y = *(const float4*)&all[(k * 16 + r) * kSumRow<HD> + 4 * c];
+      total = fmaf(l, f, total);
+      acc = make_float4(fmaf(y.x, f, acc.x), fmaf(y.y, f, acc.y), fmaf(y.z, f, acc.z),
+                        fmaf(y.w, f, acc.w));
+    }
+    write_row4(a, w, row_at(a, w, w.row0 + r), HD, 4 * c, acc, top, total, c == 0);
+  }
+}
+
 // ---- 16 rows a workgroup, each wave other keys (decode: few rows read many
 // keys, and what it costs is to read them).
 //
@@ -490,13 +529,11 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
       exact_walk<C, HD>(a, w, qp, see, sl, first, KS, kStride, l16, g4, sums);
   }
 
-  // The four waves' sums, added in wave order.
-  constexpr int kRow = HD + 4;
-  float* all = (float*)lds;                             // [wave][16][kRow]
-  float* ml = all + kWaves * 16 * kRow;                 // [wave][2][16]
+  float* all = (float*)lds;
+  float* ml = wave_stats<HD>(lds, wave);
   if (g4 == 0) {
-    ml[(wave * 2 + 0) * 16 + l16] = sums.m;
-    ml[(wave * 2 + 1) * 16 + l16] = sums.l;
+    ml[l16] = sums.m;
+    ml[16 + l16] = sums.l;
   }
 #pragma unroll
   for (int h = 0; h < L::NH; h++)
@@ -504,29 +541,174 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
     for (int v = 0; v < 4; v++)
 #pragma unroll
       for (int c = 0; c < L::EV; c += 4)
-        *(float4*)&all[(wave * 16 + l16) * kRow + L::EV * (4 * g4 + v + 16 * h) + c] =
+        *(float4*)&all[(wave * 16 + l16) * kSumRow<HD> + L::EV * (4 * g4 + v + 16 * h) + c] =
             make_float4(sums.o[h][c][v], sums.o[h][c + 1][v], sums.o[h][c + 2][v],
                         sums.o[h][c + 3][v]);
-  __syncthreads();
-  for (int i = threadIdx.x; i < 16 * HD / 4; i += kThreads) {
-    const int r = i / (HD / 4), c = i % (HD / 4);
-    if (w.row0 + r >= w.rows) break;
-    float top = -INFINITY, total = 0.0f;
+  merge_waves<HD, 16>(a, w, lds);
+}
+
+// ---- One token's R <= 2 or 4 rows on a float32 cache, each wave other keys
+// (decode steps). The float32
+// matrix cores would form 16 rows for them; vector instructions form R.
+//
+// Lanes as above: a lane sums its dims of key l % 16 for each row, the four
+// lanes of the key are added, and the weights of keys 4 g .. 4 g + 3 are
+// fetched from their lanes. A row's sums are relative to one maximum, which
+// follows where a score has passed it by kSlack: weights up to 2^kSlack are as
+// exact as those up to one. Values that the token does not see are zeros.
+template <int HD, int R>
+DNX_DEV void few(const PagedArgs& a, const Item& w, uint8_t* lds) {
+  using L = Lanes<float, HD>;
+  constexpr int KS = 16, kStride = KS * kWaves;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float sl = a.scale * 1.44269504088896341f;   // scores in units of log2
+  const Seen see = row_sees(a, w, 0);
+  const int lo = __builtin_amdgcn_readfirstlane(see.lo);
+  const int hi = __builtin_amdgcn_readfirstlane(see.hi);
+  float m[R], l[R], o[R][L::NH][4];
 #pragma unroll
-    for (int k = 0; k < kWaves; k++) top = fmaxf(top, ml[2 * k * 16 + r]);
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int r = 0; r < R; r++) {
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kWaves; k++) {
-      const float l = ml[(2 * k + 1) * 16 + r];
-      if (l == 0.0f) continue;
-      const float f = partial_factor(ml[2 * k * 16 + r], l, top);
-      const float4 y = *(const float4*)&all[(k * 16 + r) * kRow + 4 * c];
-      total = fmaf(l, f, total);
-      acc = make_float4(fmaf(y.x, f, acc.x), fmaf(y.y, f, acc.y), fmaf(y.z, f, acc.z),
-                        fmaf(y.w, f, acc.w));
-    }
-    write_row4(a, w, row_at(a, w, w.row0 + r), HD, 4 * c, acc, top, total, c == 0);
+    for (int h = 0; h < L::NH; h++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) o[r][h][c] = 0.0f;
   }
+
+  // The queries in LDS: four rows of 32 dims a lane are more registers than
+  // there are.
+  float* q = (float*)(lds + kMergeBytes<HD>);     // [R][HD]
+  if (threadIdx.x < R * HD / 4) {
+    const int r = threadIdx.x / (HD / 4), c = threadIdx.x % (HD / 4);
+    *(float4*)&q[4 * threadIdx.x] =
+        *(const float4*)(a.q + row_at(a, w, min(w.row0 + r, w.rows - 1)) * HD + 4 * c);
+  }
+
+  // Requests as above: a step's keys and values while the step before is added.
+  Raw<float, HD> x;
+  Block block;
+  int page;
+  auto next = [&](int at) {
+    while (at < w.k_hi && (lo >= at + KS || hi <= at)) at += kStride;
+    return at;
+  };
+  int kt = next(w.k_lo + KS * wave), after = kt;
+  if (kt < w.k_hi) {
+    page = page_at(a, w, kt);
+    block = block_at<float, HD>(a, w, kt, page);
+    load_keys<float, HD>(block, a.row_bytes, l16, g4, x);
+    load_values<float, HD>(block, a.row_bytes, l16, g4, x);
+    after = next(kt + kStride);
+    page = page_at(a, w, after);
+  }
+  __syncthreads();
+  while (kt < w.k_hi) {
+    const int end = block.there ? w.k_hi : kt;       // no such page: its keys are not seen
+    const int then = next(after + kStride);
+    block = block_at<float, HD>(a, w, after, page);
+    page = page_at(a, w, then);
+    float s[R];
+    float4 y[2][R];
+    auto read = [&](int d) {
+#pragma unroll
+      for (int r = 0; r < R; r++) y[d & 1][r] = *(const float4*)&q[r * HD + 4 * (4 * d + g4)];
+    };
+    read(0);
+#pragma unroll
+    for (int d = 0; d < L::ND; d++) {
+      if (d + 1 < L::ND) read(d + 1);
+      __builtin_amdgcn_sched_barrier(0);   // or all are read at once
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const float4 z = y[d & 1][r];
+        s[r] = d == 0 ? element<float>(x.k[0], 0) * z.x : fmaf(element<float>(x.k[d], 0), z.x, s[r]);
+        s[r] = fmaf(element<float>(x.k[d], 1), z.y, s[r]);
+        s[r] = fmaf(element<float>(x.k[d], 2), z.z, s[r]);
+        s[r] = fmaf(element<float>(x.k[d], 3), z.w, s[r]);
+      }
+    }
+    asm volatile("" : : : "memory");       // nor kept for the next step
+    load_keys<float, HD>(block, a.row_bytes, l16, g4, x);
+    auto sees = [&](int key) { return key >= lo && key < min(hi, end); };
+    const bool seen = sees(kt + l16);
+    bool grows = false;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      s[r] = rows4_sum(s[r]) * sl;
+      s[r] = seen ? s[r] : -INFINITY;
+      grows |= s[r] > m[r] + kSlack;
+    }
+    if (__any(grows)) {
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        float top = s[r];
+        top = fmaxf(top, dppf<kQuadXor1>(top));
+        top = fmaxf(top, dppf<kQuadXor2>(top));
+        top = fmaxf(top, dppf<kHalfRowMirror>(top));
+        top = fmaxf(top, dppf<kRowMirror>(top));
+        top = fmaxf(top, m[r]);
+        const float alpha = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[r] - top);
+        m[r] = top;
+        l[r] *= alpha;
+#pragma unroll
+        for (int h = 0; h < L::NH; h++)
+#pragma unroll
+          for (int c = 0; c < 4; c++) o[r][h][c] *= alpha;
+      }
+    }
+    float p[R][4];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      s[r] = __builtin_amdgcn_exp2f(s[r] - (m[r] == -INFINITY ? 0.0f : m[r]));
+      l[r] += s[r];
+#pragma unroll
+      for (int v = 0; v < 4; v++) p[r][v] = __shfl(s[r], 4 * g4 + v);
+    }
+    if (lo > kt || min(hi, end) < kt + KS) {
+#pragma unroll
+      for (int v = 0; v < 4; v++)
+#pragma unroll
+        for (int h = 0; h < L::NH; h++)
+          if (!sees(kt + 4 * g4 + v)) x.v[v][h] = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int h = 0; h < L::NH; h++)
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+#pragma unroll
+          for (int r = 0; r < R; r++)
+            o[r][h][c] = fmaf(element<float>(x.v[v][h], c), p[r][v], o[r][h][c]);
+    load_values<float, HD>(block, a.row_bytes, l16, g4, x);
+    kt = after;
+    after = then;
+  }
+
+  float* all = (float*)lds;
+  float* ml = wave_stats<HD>(lds, wave);
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    l[r] += dppf<kQuadXor1>(l[r]);
+    l[r] += dppf<kQuadXor2>(l[r]);
+    l[r] += dppf<kHalfRowMirror>(l[r]);
+    l[r] += dppf<kRowMirror>(l[r]);
+    if (lane == 0) {
+      ml[r] = m[r];
+      ml[16 + r] = l[r];
+    }
+#pragma unroll
+    for (int h = 0; h < L::NH; h++) {
+#pragma unroll
+      for (int c = 0; c < 4; c++) o[r][h][c] = rows4_sum(o[r][h][c]);
+      if (g4 == 0)
+        *(float4*)&all[(wave * 16 + r) * kSumRow<HD> + 4 * (l16 + 16 * h)] =
+            make_float4(o[r][h][0], o[r][h][1], o[r][h][2], o[r][h][3]);
+    }
+  }
+  merge_waves<HD, R>(a, w, lds);
 }
 
 // ---- 64 rows a workgroup, 16 a wave, which share tiles of KT keys in LDS (a
@@ -880,7 +1062,7 @@ DNX_DEV void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
 template <typename C, int HD>
 constexpr int attention_lds() {
   using T = WideTile<C, HD>;
-  constexpr int w = T::kK + T::kV + kWaves * 8, n = (kWaves * 16 * (HD + 4) + kWaves * 32) * 4;
+  constexpr int w = T::kK + T::kV + kWaves * 8, n = kMergeBytes<HD> + 4 * HD * 4;
   return w > n ? w : n;
 }
 
@@ -921,9 +1103,13 @@ paged_attention_kernel(PagedArgs a) {
   w.k_hi = min(w.count, w.k_lo + part.keys);
   if (part.wide) {
     wide<C, HD>(a, w, lds);
-  } else {
-    narrow<C, HD>(a, w, lds);
+    return;
   }
+  if constexpr (sizeof(C) == 4) {
+    if (part.few == 2) return few<HD, 2>(a, w, lds);
+    if (part.few == 4) return few<HD, 4>(a, w, lds);
+  }
+  narrow<C, HD>(a, w, lds);
 }
 
 // A row's partial results added in order, one wave a row: lane s holds the
@@ -979,7 +1165,7 @@ __global__ void __launch_bounds__(kThreads) paged_combine_kernel(PagedArgs a) {
 }
 
 PartArgs part_of(const PagedPart& p) {
-  return {p.wide, (int)p.blocks, (int)p.runs, (int)p.keys};
+  return {p.wide, p.few, (int)p.blocks, (int)p.runs, (int)p.keys};
 }
 
 PagedSplit split_of(const dnx_paged_cache* c, const dnx_paged_batch* b, int64_t heads) {

@@ -13,8 +13,11 @@ namespace dnx {
 // 16 a wave, whose waves share the keys' tiles; the others 16 rows, of which
 // each wave takes other keys. The rows' partial results are added by a second
 // launch unless there is one run in all.
+// `few`: 2 or 4 where a block of a float32 cache holds one token's rows, at
+// most that many (a kernel of their own), else 0.
 struct PagedPart {
   bool wide;
+  int few;
   int64_t blocks, runs, keys;   // blocks of rows, runs of that many keys
 };
 struct PagedSplit {
@@ -39,10 +42,12 @@ inline bool paged_wide(int64_t rows, int64_t units, int64_t keys, bool f32) {
   return rows > 128 || rows * keys * units > (f32 ? 1200000 : 4000000);
 }
 
-inline PagedPart paged_part(int64_t rows, int64_t units, int64_t keys, bool f32, int64_t least,
+inline PagedPart paged_part(int64_t tokens, int64_t group, int64_t units, int64_t keys, bool f32, int64_t least,
                             int64_t most) {
   PagedPart p{};
+  const int64_t rows = tokens * group;
   p.wide = paged_wide(rows, units, keys, f32);
+  p.few = !f32 || tokens > 1 || rows > 4 ? 0 : rows <= 2 ? 2 : 4;
   const int64_t block = p.wide ? kPagedWide : kPagedNarrow;
   p.blocks = (rows + block - 1) / block;
   p.keys = kPagedStep;
@@ -64,8 +69,8 @@ inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, 
   // Without a prefix, keys that one workgroup walks in about the time of the
   // second launch (3 us) stay in one run: up to 256.
   const int64_t least = prefix_len == 0 && max_len <= 256 ? 256 : kPagedStep;
-  return {paged_part(tokens * group, kv_heads, prefix_len, f32, kPagedStep, 1 << 20),
-          paged_part(max_tokens * group, seqs * kv_heads, max_len, f32, least, 2048)};
+  return {paged_part(tokens, group, kv_heads, prefix_len, f32, kPagedStep, 1 << 20),
+          paged_part(max_tokens, group, seqs * kv_heads, max_len, f32, least, 2048)};
 }
 
 }  // namespace dnx
