@@ -384,6 +384,12 @@ DNX_DEV void merge_waves(const PagedArgs& a, const Item& w, uint8_t* lds) {
 // (eight keys of one dim a lane) come from rows of eight dims by one byte
 // permute for two values. An infinity or NaN has no pieces: a wave that ends
 // with one in its sums walks its keys again in exact steps.
+//
+// bf16, 64 sequences of 1088 keys, 32 / 8 heads, hd 128: 54 us, 5.3 TB/s (a
+// large copy reaches 4.6, this library's best reader 6.1): bound by the bytes.
+// Of unequal lengths (128 to 2048) 69 us, 4.1 TB/s: the longest ends last.
+// Dealing all sequences' keys to the workgroups in equal parts gave 69 too: a
+// prologue for each part and a second launch took what it saved.
 template <typename C, int HD>
 DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
   using L = Lanes<C, HD>;
@@ -556,6 +562,11 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
 // fetched from their lanes. A row's sums are relative to one maximum, which
 // follows where a score has passed it by kSlack: weights up to 2^kSlack are as
 // exact as those up to one. Values that the token does not see are zeros.
+//
+// 64 sequences of 128 to 1500 keys, 16 / 4 heads, hd 128: 52 us, 4.1 TB/s
+// (on the matrix cores 63), hd 64 33 (44); 3 sequences of up to 200, hd 128,
+// two rows 7.1 (9.5). The same scheme on bf16 caches, whose elements it has to
+// unpack, took 41 us for 29 on the matrix cores.
 template <int HD, int R>
 DNX_DEV void few(const PagedArgs& a, const Item& w, uint8_t* lds) {
   using L = Lanes<float, HD>;
@@ -720,6 +731,11 @@ DNX_DEV void few(const PagedArgs& a, const Item& w, uint8_t* lds) {
 // caches are split into three pieces on the way (PC = 3), each product formed
 // from the six largest products of pieces (below 2^-26 of it are left out). The
 // next tile is in registers meanwhile.
+//
+// A prefix of 8192 keys, bf16, for 64 tokens of 32 / 8 heads, hd 128: 40 us
+// for 16 tiles of 64 keys a wave, 0.6 PFLOP/s of bf16 products, three for each
+// of the formula's. Waits bound it, not one unit: a tile takes a lone wave of a
+// SIMD 1.8 us, and two waves 1.2 each.
 template <typename C, int HD>
 struct WideTile {
   static constexpr int PC = sizeof(C) == 4 ? 3 : 1;
@@ -1115,6 +1131,8 @@ paged_attention_kernel(PagedArgs a) {
 // A row's partial results added in order, one wave a row: lane s holds the
 // statistics of run s, lane i sums dims ND i .. (at most 64 runs), eight runs'
 // values requested at once. What runs without a weight hold does not count.
+// 4.7 us for 64 tokens of 32 heads, hd 128, 9 runs; 3.9 for 16 tokens of 16:
+// the launch and two waits for memory.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) paged_combine_kernel(PagedArgs a) {
   constexpr int ND = HD / 64, U = 8;
