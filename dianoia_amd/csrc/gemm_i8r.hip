@@ -287,9 +287,9 @@ int dnx_gemm_i8r(const int8_t* w, const float* w_scale, const int8_t* x, const f
   switch (i8r_route(n, rows, cols)) {
     case 0: return launch_tile<0, 1, 1, 1, 1, 4>(p, st);
     case 1: return launch_tile<1, 2, 1, 1, 1, 4>(p, st);
-    case 2: return launch_tile<2, 2, 2, 1, 1, 8>(p, st);
+    case 2: return launch_tile<2, 2, 2, 1, 1, 6>(p, st);
     case 3: return launch_tile<3, 2, 2, 2, 1, 4>(p, st);
-    case 4: return launch_tile<4, 2, 2, 2, 2, 3>(p, st);
+    case 4: return launch_tile<4, 2, 2, 2, 2, 4>(p, st);
     case 5: return launch_tile<5, 4, 2, 2, 2, 3>(p, st);
     case 6: return launch_tile<6, 4, 4, 2, 2, 5>(p, st);
   }

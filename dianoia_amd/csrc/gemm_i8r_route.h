@@ -2,7 +2,7 @@
 // code alone, without HIP.
 #pragma once
 
-#include <algorithm>
+#include <cmath>
 #include <stdint.h>
 
 namespace dnx {
@@ -10,27 +10,28 @@ namespace dnx {
 // A tile kernel: its tokens x weight rows, the parts of K that a workgroup's
 // wave groups share, and what it costs (us): a launch with prologue and
 // epilogue, a stage of 64 of K for a workgroup that has a CU to itself, and
-// for each of the workgroups that share one.
+// for each of the workgroups that share one; and how much of a last round of
+// workgroups that does not reach all CUs is waited for.
 struct I8RTile {
   int tokens, rows, parts;
-  float fixed, alone, shared;
+  float fixed, alone, shared, last;
 };
 
-// Fitted to 179 shapes (n 17 .. 2048, rows 512 .. 8192, K 512 .. 4096), timed
-// with weights rotated past the L2: the estimates are off by 7 to 10% (rms),
-// and the kernel they choose is 0.6% slower than the best of the seven in the
-// mean, 17% at worst (48 x 4096 x 4096: 9.2 against 7.8 us). Each is the
-// fastest somewhere: e.g. (us, in this order, n x rows x K) 17 x 512 x 4096:
-// 6.8 8.1 11.5 - - - -; 128 x 4096 x 2048: - 7.1 8.5 10.4 15.4 15.5 23.1; 256
-// x 4096 x 2048: - 10.4 9.0 10.7 15.8 19.4 25.0; 512 x 4096 x 4096: - 27.6
-// 20.9 17.5 25.3 31.8 41.7; 2048 x 2048 x 4096: - 73 40.7 31.7 27.4 33.5 41.9;
-// 1024 x 8192 x 4096: - 107 79 62 52 45.7 53.4; 2048 x 8192 x 4096: - 288 161
-// 122 93 84.5 73.5.
+// Fitted to 240 shapes (n 17 .. 2048, rows 512 .. 8192, K 512 .. 4096), timed
+// with weights rotated past the L2: the estimates are off by 8 to 12% (rms),
+// and the kernel they choose is 1.1% slower than the best of the seven (in two
+// or three depths of their rings each) in the mean, 31% at worst (777 x 4304 x
+// 4096: 33.3 against 25.5 us). Each is the fastest somewhere (us, in this
+// order, n x rows x K): 64 x 512 x 4096 7.4 9.4 12 14 19 - -; 64 x 4304 x 2048
+// 8.4 6.9 8.4 9.4 12 - -; 128 x 6144 x 4096 - 21.5 17.0 23.7 28.9 35.3 48; 256
+// x 6144 x 4096 - - 27.9 24.0 28.5 43 55; 512 x 8192 x 4096 - - 48.5 40 30.6 44
+// 54; 1024 x 6144 x 4096 - - - 57 46.8 40.5 52.7; 2048 x 8192 x 4096 - - - 135
+// 92 81 72.6.
 constexpr I8RTile kI8RTiles[] = {
-    {32, 32, 4, 3.25f, 0.200f, 0.320f},  {64, 32, 2, 3.50f, 0.148f, 0.216f},
-    {64, 64, 1, 3.90f, 0.120f, 0.152f},  {128, 64, 1, 4.20f, 0.175f, 0.217f},
-    {128, 128, 1, 5.90f, 0.282f, 0.340f}, {256, 128, 1, 5.70f, 0.351f, 0.569f},
-    {256, 256, 1, 7.75f, 0.488f, 0.867f},
+    {32, 32, 4, 3.73f, 0.154f, 0.357f, 0.52f},   {64, 32, 2, 3.53f, 0.146f, 0.256f, 0.36f},
+    {64, 64, 1, 3.91f, 0.121f, 0.173f, 0.33f},   {128, 64, 1, 4.13f, 0.154f, 0.267f, 0.28f},
+    {128, 128, 1, 5.80f, 0.206f, 0.382f, 0.34f}, {256, 128, 1, 6.45f, 0.345f, 0.602f, 0.63f},
+    {256, 256, 1, 8.70f, 0.457f, 0.987f, 0.55f},
 };
 constexpr int kI8RCount = sizeof(kI8RTiles) / sizeof(kI8RTiles[0]);
 constexpr int kI8RFew = -1;
@@ -48,8 +49,8 @@ inline int i8r_route(int64_t n, int64_t rows, int64_t cols) {
     const int64_t tiles = ((n + t.tokens - 1) / t.tokens) * ((rows + t.rows - 1) / t.rows);
     const int64_t stages = ((cols + 63) / 64 + t.parts - 1) / t.parts;
     const double fill = tiles / 256.0;   // workgroups a CU
-    const double stage = std::max(t.alone + (t.shared - t.alone) * std::min(1.0, fill),
-                                  t.shared * fill);
+    const double stage = fill <= 1.0 ? t.alone + (t.shared - t.alone) * fill
+                                     : t.shared * (fill + t.last * (std::ceil(fill) - fill));
     const double us = t.fixed + stages * stage;
     if (i == 0 || us < least) {
       best = i;

@@ -32,8 +32,9 @@ def route(tmp_path_factory):
 
 
 # A shape of odd sizes for each tile kernel, in the order of its table.
-SHAPES = [(17, 520, 4096), (127, 4100, 2048), (255, 4099, 2080), (511, 4098, 4096),
-          (2047, 2049, 4096), (1023, 8193, 1056), (2047, 8189, 1184)]
+SHAPES = [(17, 520, 4096), (63, 4300, 2048), (127, 4100, 2048), (255, 4099, 2080),
+          (511, 4098, 4096), (1023, 6145, 1056), (2047, 8189, 1184)]
+MORE = [(2047, 2049, 4096), (1023, 8193, 1056)]
 
 
 def test_each_kernel_is_taken(route):

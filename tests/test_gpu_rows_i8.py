@@ -15,7 +15,7 @@ import torch
 
 from dianoia_amd import device as D
 from gpu_util import bits, dev, host
-from test_gemm_i8r_route import SHAPES as TILES
+from test_gemm_i8r_route import MORE as MORE_TILES, SHAPES as TILES
 
 U = 2.0 ** -24
 EPS = 1e-6
@@ -188,7 +188,7 @@ def test_product(gpu_ready, n, rows, cols):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shape", TILES)
+@pytest.mark.parametrize("shape", TILES + MORE_TILES)
 @pytest.mark.parametrize("shift", [0, 1])
 def test_product_every_tile(gpu_ready, shape, shift):
     """Each tile kernel of the route, at odd sizes and at rows of a multiple of
