@@ -39,7 +39,7 @@ struct PagedArgs {
   int prefix_len, seqs, tokens, max_len;
   const float *q, *gate;
   float *out, *stat, *part;   // partials: stat [rows][splits][2], part [rows][splits][hd]
-  int window, splits;
+  int window, splits, joined;
   PartArgs prefix, own;
   int64_t prefix_items;
   float scale;
@@ -59,11 +59,13 @@ DNX_DEV float row_scale(float l, const float* gate, int64_t row) {
 }
 
 // What a workgroup takes: rows row0 .. of the `rows` of tokens t0 .. that
-// share key head kvh, and keys k_lo .. k_hi - 1 of a list of pages.
+// share key head kvh, and keys k_lo .. k_hi - 1 of a list of pages. Where the
+// prefix is joined to a sequence's own keys, these begin at key `joined`; the
+// keys from prefix_len to there do not exist.
 struct Item {
   bool own;
   int kvh, run, row0, rows, t0, first;   // first: the place of token t0 among the keys
-  int k_lo, k_hi, count;
+  int k_lo, k_hi, count, joined;
   const int32_t* table;
 };
 
@@ -80,7 +82,11 @@ DNX_DEV Seen row_sees(const PagedArgs& a, const Item& w, int r) {
   const int token = w.t0 + r / a.group;
   if (w.own) {
     const int place = w.first + token - w.t0;
-    return {a.window > 0 ? place - a.window + 1 : 0, min(w.count, place + 1)};
+    const int hi = w.joined + min(w.count, max(place + 1, 0));
+    if (a.window == 0) return {0, hi};
+    if (w.joined == 0) return {place - a.window + 1, hi};
+    const int lo = max(a.prefix_len + place, 0) - a.window + 1;
+    return {lo < a.prefix_len ? lo : lo - a.prefix_len + w.joined, hi};
   }
   if (a.window == 0) return {0, w.count};
   int lo = 0, hi = a.seqs;              // the token's sequence: starts[lo] <= token < starts[hi]
@@ -99,22 +105,29 @@ DNX_DEV Seen row_sees(const PagedArgs& a, const Item& w, int r) {
 // and without a branch, so that the loads of several do not wait in turn.
 struct Block {
   i32x4 keys, values;
-  bool there;
+  int end;      // its keys lie before this key (none: not after the first)
 };
+template <bool kJoined>
 DNX_DEV int page_at(const PagedArgs& a, const Item& w, int kt) {
-  return __builtin_amdgcn_readfirstlane(w.table[min(kt, w.k_hi - 1) >> a.page_bits]);
+  const int key = min(kt, w.k_hi - 1);
+  const bool own = !kJoined || key >= w.joined;
+  const int32_t* table = own ? w.table : a.prefix_pages;
+  const int place = !kJoined ? key : own ? key - w.joined : min(key, a.prefix_len - 1);
+  return __builtin_amdgcn_readfirstlane(table[place >> a.page_bits]);
 }
 // Blocks as seen from `behind` keys before them: the offset of key i of the
 // block is that of row behind + i.
-template <typename C, int HD>
+template <typename C, int HD, bool kJoined>
 DNX_DEV Block block_at(const PagedArgs& a, const Item& w, int kt, int page, int keys = 16,
                        int behind = 0) {
   Block b;
-  const int left = min(keys, w.k_hi - kt);
-  b.there = left > 0 && (uint32_t)page < (uint32_t)a.pages;
-  const uint32_t range = b.there ? (uint32_t)((left + behind) * a.row_bytes) : 0u;
+  const bool own = !kJoined || kt >= w.joined;
+  const int left = min(keys, (own ? w.k_hi : a.prefix_len) - kt);
+  const bool there = left > 0 && (uint32_t)page < (uint32_t)a.pages;
+  b.end = there ? kt + left : kt;
+  const uint32_t range = there ? (uint32_t)((left + behind) * a.row_bytes) : 0u;
   // Not used where the range is empty.
-  const uint32_t in_page = (uint32_t)(kt & ((1 << a.page_bits) - 1));
+  const uint32_t in_page = (uint32_t)((kJoined && own ? kt - w.joined : kt) & ((1 << a.page_bits) - 1));
   const uint64_t at = (uint64_t)(uint32_t)page * ((uint32_t)a.row_bytes << a.page_bits) +
                       (uint64_t)(in_page * (uint32_t)a.row_bytes) -
                       (uint64_t)((uint32_t)behind * (uint32_t)a.row_bytes);
@@ -302,7 +315,7 @@ DNX_DEV void load_query(const float* q, int g4, float (*x)[Lanes<C, HD>::EK]) {
 
 // Keys first .. first + width - 1, then `stride` further, to the item's end,
 // in exact steps.
-template <typename C, int HD>
+template <typename C, int HD, bool kJoined>
 DNX_DEV void exact_walk(const PagedArgs& a, const Item& w, const float* qp, Seen see, float sl,
                         int first, int width, int stride, int l16, int g4, Sums<C, HD>& sums) {
   float q[Lanes<C, HD>::ND][Lanes<C, HD>::EK];
@@ -312,12 +325,12 @@ DNX_DEV void exact_walk(const PagedArgs& a, const Item& w, const float* qp, Seen
   for (int k0 = first; k0 < w.k_hi; k0 += stride)
 #pragma unroll 1
     for (int kt = k0; kt < min(w.k_hi, k0 + width); kt += 16) {
-      const Block b = block_at<C, HD>(a, w, kt, page_at(a, w, kt));
-      if (!b.there || !__any(see.lo < kt + 16 && see.hi > kt)) continue;
+      const Block b = block_at<C, HD, kJoined>(a, w, kt, page_at<kJoined>(a, w, kt));
+      if (b.end == kt || !__any(see.lo < kt + 16 && see.hi > kt)) continue;
       Raw<C, HD> x;
       load_keys<C, HD>(b, a.row_bytes, l16, g4, x);
       load_values<C, HD>(b, a.row_bytes, l16, g4, x);
-      exact_step<C, HD>(x, q, kt, w.k_hi, see, sl, g4, sums, [] {});
+      exact_step<C, HD>(x, q, kt, b.end, see, sl, g4, sums, [] {});
     }
 }
 
@@ -390,7 +403,7 @@ DNX_DEV void merge_waves(const PagedArgs& a, const Item& w, uint8_t* lds) {
 // Of unequal lengths (128 to 2048) 69 us, 4.1 TB/s: the longest ends last.
 // Dealing all sequences' keys to the workgroups in equal parts gave 69 too: a
 // prologue for each part and a second launch took what it saved.
-template <typename C, int HD>
+template <typename C, int HD, bool kJoined>
 DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
   using L = Lanes<C, HD>;
   constexpr bool kF32 = sizeof(C) == 4;
@@ -415,11 +428,11 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
   int page[U];
   auto pages = [&](int at) {
 #pragma unroll
-    for (int u = 0; u < U; u++) page[u] = page_at(a, w, at + 16 * u);
+    for (int u = 0; u < U; u++) page[u] = page_at<kJoined>(a, w, at + 16 * u);
   };
   auto blocks = [&](int at) {
 #pragma unroll
-    for (int u = 0; u < U; u++) block[u] = block_at<C, HD>(a, w, at + 16 * u, page[u]);
+    for (int u = 0; u < U; u++) block[u] = block_at<C, HD, kJoined>(a, w, at + 16 * u, page[u]);
   };
   auto request_keys = [&] {
 #pragma unroll
@@ -446,7 +459,7 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
   }
   if constexpr (kF32) {
     while (kt < w.k_hi) {
-      const int end = block[0].there ? w.k_hi : kt;     // no such page: its keys are not seen
+      const int end = block[0].end;
       const int then = next(after + kStride);
       blocks(after);
       pages(then);
@@ -462,9 +475,9 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
       if (kt < w.k_hi) split_pieces(q[d], qf[d]);
     }
     while (kt < w.k_hi) {
-      bool ok[U];
+      int end[U];
 #pragma unroll
-      for (int u = 0; u < U; u++) ok[u] = block[u].there;
+      for (int u = 0; u < U; u++) end[u] = block[u].end;
       const int then = next(after + kStride);
       blocks(after);
       pages(then);
@@ -490,7 +503,7 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
 #pragma unroll
         for (int v = 0; v < 4; v++) {
           const int key = kt + 16 * u + 4 * g4 + v;
-          const bool sees = ok[u] && key >= see.lo && key < see.hi && key < w.k_hi;
+          const bool sees = key >= see.lo && key < see.hi && key < end[u];
           p[4 * u + v] = sees ? (s[u][v] + low[u][v]) * sl : -INFINITY;
           mt = fmaxf(mt, p[4 * u + v]);
         }
@@ -532,7 +545,7 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
 #pragma unroll
       for (int v = 0; v < 4; v++) check += sums.o[0][c][v] - sums.o[0][c][v];
     if (__builtin_expect(__any(check != check), 0))
-      exact_walk<C, HD>(a, w, qp, see, sl, first, KS, kStride, l16, g4, sums);
+      exact_walk<C, HD, kJoined>(a, w, qp, see, sl, first, KS, kStride, l16, g4, sums);
   }
 
   float* all = (float*)lds;
@@ -567,7 +580,7 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
 // (on the matrix cores 63), hd 64 33 (44); 3 sequences of up to 200, hd 128,
 // two rows 7.1 (9.5). The same scheme on bf16 caches, whose elements it has to
 // unpack, took 41 us for 29 on the matrix cores.
-template <int HD, int R>
+template <int HD, int R, bool kJoined>
 DNX_DEV void few(const PagedArgs& a, const Item& w, uint8_t* lds) {
   using L = Lanes<float, HD>;
   constexpr int KS = 16, kStride = KS * kWaves;
@@ -607,19 +620,19 @@ DNX_DEV void few(const PagedArgs& a, const Item& w, uint8_t* lds) {
   };
   int kt = next(w.k_lo + KS * wave), after = kt;
   if (kt < w.k_hi) {
-    page = page_at(a, w, kt);
-    block = block_at<float, HD>(a, w, kt, page);
+    page = page_at<kJoined>(a, w, kt);
+    block = block_at<float, HD, kJoined>(a, w, kt, page);
     load_keys<float, HD>(block, a.row_bytes, l16, g4, x);
     load_values<float, HD>(block, a.row_bytes, l16, g4, x);
     after = next(kt + kStride);
-    page = page_at(a, w, after);
+    page = page_at<kJoined>(a, w, after);
   }
   __syncthreads();
   while (kt < w.k_hi) {
-    const int end = block.there ? w.k_hi : kt;       // no such page: its keys are not seen
+    const int end = block.end;
     const int then = next(after + kStride);
-    block = block_at<float, HD>(a, w, after, page);
-    page = page_at(a, w, then);
+    block = block_at<float, HD, kJoined>(a, w, after, page);
+    page = page_at<kJoined>(a, w, then);
     float s[R];
     float4 y[2][R];
     auto read = [&](int d) {
@@ -799,7 +812,7 @@ DNX_DEV void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
   int page[NB];                                   // of the tile to load next
   auto pages = [&](int kt) {
 #pragma unroll
-    for (int i = 0; i < NB; i++) page[i] = page_at(a, w, kt + 16 * i);
+    for (int i = 0; i < NB; i++) page[i] = page_at<false>(a, w, kt + 16 * i);
   };
 
   // The offsets are those within the tile: one resource serves it where a page
@@ -821,8 +834,8 @@ DNX_DEV void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
   };
   auto load_tile = [&](int kt) {
     if ((1 << a.page_bits) >= KT) {
-      const Block b = block_at<C, HD>(a, w, kt, page[0], KT);
-      there_next = b.there ? (1u << NB) - 1 : 0u;
+      const Block b = block_at<C, HD, false>(a, w, kt, page[0], KT);
+      there_next = b.end > kt ? (1u << NB) - 1 : 0u;
 #pragma unroll
       for (int j = 0; j < T::KU; j++) load_key(j, b);
 #pragma unroll
@@ -833,8 +846,8 @@ DNX_DEV void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
       there_next = 0;
 #pragma unroll
       for (int i = 0; i < NB; i++) {
-        b[i] = block_at<C, HD>(a, w, kt + 16 * i, page[i], 16, 16 * i);
-        there_next |= b[i].there ? 1u << i : 0u;
+        b[i] = block_at<C, HD, false>(a, w, kt + 16 * i, page[i], 16, 16 * i);
+        there_next |= b[i].end > kt + 16 * i ? 1u << i : 0u;
       }
       // Of the second half of the waves the blocks of key groups 4 .. 7, and
       // where 32 keys are loaded at once those of the latter 16.
@@ -1054,7 +1067,7 @@ DNX_DEV void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
   if (__builtin_expect(__any(check != check), 0)) {
     using L = Lanes<C, HD>;
     Sums<C, HD> x;
-    exact_walk<C, HD>(a, w, qp, see, sl, w.k_lo, w.k_hi - w.k_lo, w.k_hi - w.k_lo, l16, g4, x);
+    exact_walk<C, HD, false>(a, w, qp, see, sl, w.k_lo, w.k_hi - w.k_lo, w.k_hi - w.k_lo, l16, g4, x);
 #pragma unroll
     for (int h = 0; h < L::NH; h++)
 #pragma unroll
@@ -1080,6 +1093,15 @@ constexpr int attention_lds() {
   using T = WideTile<C, HD>;
   constexpr int w = T::kK + T::kV + kWaves * 8, n = kMergeBytes<HD> + 4 * HD * 4;
   return w > n ? w : n;
+}
+
+template <typename C, int HD, bool kJoined>
+DNX_DEV void block_of_16(const PagedArgs& a, const Item& w, int rows, uint8_t* lds) {
+  if constexpr (sizeof(C) == 4) {
+    if (rows == 2) return few<HD, 2, kJoined>(a, w, lds);
+    if (rows == 4) return few<HD, 4, kJoined>(a, w, lds);
+  }
+  narrow<C, HD, kJoined>(a, w, lds);
 }
 
 // The prefix's workgroups, then the sequences' own: both kinds in one launch,
@@ -1110,22 +1132,25 @@ paged_attention_kernel(PagedArgs a) {
   const int t1 = w.own ? max(w.t0, min(s1, live)) : live;
   w.first = w.own ? len - (t1 - w.t0) : 0;
   w.table = w.own ? a.tables + seq * a.table_stride : a.prefix_pages;
-  w.count = w.own ? (int)min((int64_t)min(len, a.max_len), a.table_stride << a.page_bits)
+  w.count = w.own ? (int)max(min((int64_t)min(len, a.max_len), a.table_stride << a.page_bits),
+                             (int64_t)0)
                   : a.prefix_len;
   w.row0 = block * (part.wide ? kPagedWide : kPagedNarrow);
   w.rows = (t1 - w.t0) * a.group;
   if (w.row0 >= w.rows) return;
+  w.joined = w.own ? a.joined : 0;
   w.k_lo = w.run * part.keys;
-  w.k_hi = min(w.count, w.k_lo + part.keys);
+  w.k_hi = min(w.joined > 0 && w.count == 0 ? a.prefix_len : w.joined + w.count,
+               w.k_lo + part.keys);
   if (part.wide) {
     wide<C, HD>(a, w, lds);
     return;
   }
-  if constexpr (sizeof(C) == 4) {
-    if (part.few == 2) return few<HD, 2>(a, w, lds);
-    if (part.few == 4) return few<HD, 4>(a, w, lds);
+  if (w.joined > 0) {
+    block_of_16<C, HD, true>(a, w, part.few, lds);
+  } else {
+    block_of_16<C, HD, false>(a, w, part.few, lds);
   }
-  narrow<C, HD>(a, w, lds);
 }
 
 // A row's partial results added in order, one wave a row: lane s holds the
@@ -1243,6 +1268,7 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
   a.part = (float*)workspace;
   a.stat = a.part + batch->tokens * heads * a.splits * cache->hd;
   a.window = (int)window;
+  a.joined = (int)s.joined;
   a.prefix = part_of(s.prefix);
   a.own = part_of(s.own);
   // Whole rounds of the eight XCDs.

@@ -20,8 +20,11 @@ struct PagedPart {
   int few;
   int64_t blocks, runs, keys;   // blocks of rows, runs of that many keys
 };
+// `joined` (a multiple of kPagedStep): the prefix is walked with each
+// sequence's own keys in one run, in which the own keys begin at that place.
 struct PagedSplit {
   PagedPart prefix, own;
+  int64_t joined;
   int64_t splits() const { return prefix.runs + own.runs; }
 };
 
@@ -69,8 +72,24 @@ inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, 
   // Without a prefix, keys that one workgroup walks in about the time of the
   // second launch (3 us) stay in one run: up to 256.
   const int64_t least = prefix_len == 0 && max_len <= 256 ? 256 : kPagedStep;
-  return {paged_part(tokens, group, kv_heads, prefix_len, f32, kPagedStep, 1 << 20),
-          paged_part(max_tokens, group, seqs * kv_heads, max_len, f32, least, 2048)};
+  PagedSplit s{paged_part(tokens, group, kv_heads, prefix_len, f32, kPagedStep, 1 << 20),
+               paged_part(max_tokens, group, seqs * kv_heads, max_len, f32, least, 2048), 0};
+  // A short prefix is joined to them where a CU for each workgroup is left: its
+  // keys are then read once for each block of rows, but without the second
+  // launch. Up to 384 keys, or 256 where the float32 matrix cores take 16 rows
+  // (us, apart against joined: 1 sequence of 83 keys after 238, f32 hd 64, 8.1 /
+  // 6.8; 31 tokens each of 6 after 235, bf16 hd 128, 11.9 / 8.8; 6 tokens each of
+  // 12 after 276, f32 hd 128, 11.3 / 15.4; limits of 512 keys change nothing).
+  const auto steps = [](int64_t keys) { return (keys + kPagedStep - 1) / kPagedStep * kPagedStep; };
+  const int64_t joined = steps(prefix_len), keys = joined + steps(max_len);
+  if (joined > 0 && s.own.runs > 0 && !s.own.wide && keys <= (f32 && s.own.few == 0 ? 256 : 384) &&
+      seqs * kv_heads * s.own.blocks <= 256) {
+    s.joined = joined;
+    s.own.runs = 1;
+    s.own.keys = keys;
+    s.prefix.runs = 0;
+  }
+  return s;
 }
 
 }  // namespace dnx

@@ -16,6 +16,8 @@ and the normalised weights are off by 2 e. The sums over N keys add 2 (N + 64)
 u of the sum of |weight v|. So |error| <= (2 e + 2 (N + 64) u) sum_j p_j |v_j|
 with e for the worst key of the row; the gate adds 4 u."""
 
+import itertools
+
 import numpy as np
 import pytest
 import torch
@@ -295,6 +297,37 @@ def test_rows_without_keys_are_zeros(gpu_ready, kind):
     assert (out[0] == 0).all() and (out[1] == 0).all() and (out[2] != 0).any()
     b = Batch(3, [1], [0], 0, 4, 2, 64, kind, 16)      # no key in the whole call
     assert (b.check() == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("prefix", [1, 16, 63, 64, 65, 128, 250])
+def test_short_prefix(gpu_ready, prefix, kind):
+    """A prefix and own keys that one workgroup walks, with own keys that begin
+    at a step's start and windows that end anywhere; sequences without tokens
+    and tables with pages outside the cache."""
+    for (heads, kv, hd, page), counts in itertools.product(
+            [(2, 2, 64, 16), (6, 2, 128, 64), (8, 1, 64, 32)], [[1, 1, 0, 1], [3, 1, 2, 0]]):
+        b = Batch(prefix, counts, [60, 1, 33, 4], prefix, heads, kv, hd, kind, page, pad=1, gate=True)
+        for window in (0, 1, 5, 40, 64, prefix, prefix + 1, 100, 1000):
+            b.check(window)
+        b.batch.prefix_pages[-1] = -1
+        b.tables[0, 0] = 0x7fffffff
+        last = (prefix - 1) // page * page
+        b.check(seen=lambda s, j: j < last if j < prefix else s != 0 or j - prefix >= page)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_short_prefix_and_no_own_key(gpu_ready, kind):
+    b = Batch(10, [1, 1], [0, 2], 20, 4, 2, 64, kind, 16)
+    out = host(b.run())
+    alone = Batch(10, [1, 1], [0, 0], 20, 4, 2, 64, kind, 16)
+    alone.q.copy_(b.q)
+    for t in ("keys", "values"):
+        getattr(alone, t)[torch.from_numpy(alone.shared).cuda().long()] = \
+            getattr(b, t)[torch.from_numpy(b.shared).cuda().long()]
+    alone.first_kv = b.first_kv
+    want, room = alone.expected()       # places 19: all twenty keys
+    assert (np.abs(out[0] - want[0]) <= room[0]).all()
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])

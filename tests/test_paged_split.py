@@ -18,8 +18,8 @@ extern "C" void split_of(int64_t seqs, int64_t tokens, int64_t max_tokens, int64
   const dnx::PagedSplit s =
       dnx::paged_split(seqs, tokens, max_tokens, group, kv_heads, prefix, len, f32 != 0);
   const int64_t v[] = {s.prefix.blocks, s.own.blocks, s.prefix.runs, s.prefix.keys, s.own.runs,
-                       s.own.keys, s.splits()};
-  for (int i = 0; i < 7; i++) out[i] = v[i];
+                       s.own.keys, s.splits(), s.joined};
+  for (int i = 0; i < 8; i++) out[i] = v[i];
 }
 """
 
@@ -35,7 +35,7 @@ def split_of(tmp_path_factory):
     f.argtypes, f.restype = [ctypes.c_int64] * 8 + [ctypes.c_void_p], None
 
     def call(*args):
-        out = (ctypes.c_int64 * 7)()
+        out = (ctypes.c_int64 * 8)()
         f(*args, out)
         return list(out)
     return call
@@ -46,9 +46,13 @@ def test_every_key_has_a_run(split_of):
             (1, 3, 64, 300), (1, 5, 70), (1, 3, 8, 33), (1, 2, 8), (0, 1, 63, 65, 777, 8192, 200000),
             (0, 1, 64, 500, 2048, 100000), (0, 1)):
         tokens = seqs * each
-        pr, orows, ps, prun, os_, orun, total = split_of(seqs, tokens, each, group, kv, prefix, length,
-                                                        f32)
+        pr, orows, ps, prun, os_, orun, total, joined = split_of(seqs, tokens, each, group, kv, prefix,
+                                                                length, f32)
         assert total == ps + os_ <= 64
+        if joined:       # one run of both, in which the own keys begin at a step
+            assert (ps, os_) == (0, 1) and joined % 64 == 0 and prefix <= joined < prefix + 64
+            assert joined + length <= orun <= 384 and orows >= 1
+            continue
         for keys, splits, run in ((prefix, ps, prun), (length, os_, orun)):
             assert run % 64 == 0 and run > 0
             if keys == 0:
@@ -70,7 +74,7 @@ def test_workspace_and_refusals():
 
     def batch(**k):
         return _lib.PagedBatchStruct(**{**dict(starts=a, lens=a, tables=a, prefix_pages=a, table_stride=4,
-                                               prefix_len=100, seqs=3, tokens=8, max_tokens=1,
+                                               prefix_len=1000, seqs=3, tokens=8, max_tokens=1,
                                                max_len=64), **k})
 
     def size(c, b, heads=4):
@@ -125,7 +129,7 @@ def test_limits_of_sizes():
     lib = _lib.load()
     a = 4096
 
-    def size(tokens=8, heads=4, pages=64, prefix=100, length=64):
+    def size(tokens=8, heads=4, pages=64, prefix=1000, length=64):
         c = _lib.PagedCacheStruct(keys=a, values=a, pages=pages, page=16, kv_heads=2, hd=64, type=0)
         b = _lib.PagedBatchStruct(starts=a, lens=a, tables=a, prefix_pages=a, table_stride=4,
                                   prefix_len=prefix, seqs=3, tokens=tokens, max_tokens=1, max_len=length)
