@@ -647,12 +647,27 @@ def _at(t: torch.Tensor | None, device: int) -> int | None:
     return t.data_ptr()
 
 
+def _on(device: int, stream) -> int:
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
+
+
+def _refuse(*tensors) -> None:
+    """Names what is wrong with one of them, which a caller has seen."""
+    d = _device_of(tensors[0])
+    for t in tensors:
+        _at(t, d)
+    raise ValueError("device launchers take tensors of one CUDA (HIP) device")
+
+
 def _quantize_i8r(name: str, size: int, x, qs, scales, rows, cols, cols_pad, stream) -> None:
     if x.nbytes < rows * cols * size or qs.nbytes < rows * cols_pad or scales.nbytes < rows * 4:
         _need(name, x=(x, rows * cols * size), qs=(qs, rows * cols_pad), scales=(scales, rows * 4))
-    d = _device_of(x)
-    rc = getattr(_lib.load(), name)(_at(x, d), _at(qs, d), _at(scales, d), rows, cols, cols_pad,
-                                    _stream(stream))
+    d = torch._C._cuda_getDevice() if x.is_cuda else -2
+    if (x.get_device() != d or qs.get_device() != d or scales.get_device() != d
+            or not (x.is_contiguous() and qs.is_contiguous() and scales.is_contiguous())):
+        _refuse(x, qs, scales)
+    rc = getattr(_lib.load(), name)(x.data_ptr(), qs.data_ptr(), scales.data_ptr(), rows, cols,
+                                    cols_pad, _on(d, stream))
     if rc:
         _check(rc, name)
 
@@ -677,9 +692,14 @@ def rms_norm_i8r(x, w, qs, scales, rows: int, cols: int, cols_pad: int, eps: flo
             or (x_out is not None and x_out.nbytes < size)):
         _need("rms_norm_i8r", x=(x, size), w=(w, cols * 4), qs=(qs, rows * cols_pad),
               scales=(scales, rows * 4), m=(m, size), x_out=(x_out, size))
-    d = _device_of(x)
-    rc = _lib.load().dnx_rms_norm_i8r(_at(x, d), _at(m, d), _at(x_out, d), _at(w, d), _at(qs, d),
-                                      _at(scales, d), rows, cols, cols_pad, eps, _stream(stream))
+    d = torch._C._cuda_getDevice() if x.is_cuda else -2
+    if (x.get_device() != d or w.get_device() != d or qs.get_device() != d
+            or scales.get_device() != d or not (x.is_contiguous() and w.is_contiguous()
+                                                and qs.is_contiguous() and scales.is_contiguous())):
+        _refuse(x, w, qs, scales)
+    rc = _lib.load().dnx_rms_norm_i8r(
+        x.data_ptr(), None if m is None else _at(m, d), None if x_out is None else _at(x_out, d),
+        w.data_ptr(), qs.data_ptr(), scales.data_ptr(), rows, cols, cols_pad, eps, _on(d, stream))
     if rc:
         _check(rc, "dnx_rms_norm_i8r")
 
@@ -690,9 +710,14 @@ def gemm_i8r(w, w_scale, x, x_scale, y, rows: int, cols: int, n: int, stream=Non
             or x_scale.nbytes < n * 4 or y.nbytes < n * rows * 4):
         _need("gemm_i8r", w=(w, rows * cols), w_scale=(w_scale, rows * 4), x=(x, n * cols),
               x_scale=(x_scale, n * 4), y=(y, n * rows * 4))
-    d = _device_of(w)
-    rc = _lib.load().dnx_gemm_i8r(_at(w, d), _at(w_scale, d), _at(x, d), _at(x_scale, d),
-                                  _at(y, d), rows, cols, n, _stream(stream))
+    d = torch._C._cuda_getDevice() if w.is_cuda else -2
+    if (w.get_device() != d or w_scale.get_device() != d or x.get_device() != d
+            or x_scale.get_device() != d or y.get_device() != d
+            or not (w.is_contiguous() and w_scale.is_contiguous() and x.is_contiguous()
+                    and x_scale.is_contiguous() and y.is_contiguous())):
+        _refuse(w, w_scale, x, x_scale, y)
+    rc = _lib.load().dnx_gemm_i8r(w.data_ptr(), w_scale.data_ptr(), x.data_ptr(), x_scale.data_ptr(),
+                                  y.data_ptr(), rows, cols, n, _on(d, stream))
     if rc:
         _check(rc, "dnx_gemm_i8r")
 
@@ -813,7 +838,7 @@ def paged_append(cache: PagedCache, k, v, positions, slots, rope=None, q=None, q
         qs, ks, vs = heads * hd, kv_heads * hd, kv_heads * hd
     rc = _lib.load().dnx_paged_append(
         cache.ref, qp, qs, qo, k.data_ptr(), ks, v.data_ptr(), vs, qw, kw, table, rows, at,
-        _numbers("slots", slots, d, n, _I32), heads, n, eps, _stream(stream))
+        _numbers("slots", slots, d, n, _I32), heads, n, eps, _on(d, stream))
     if rc:
         _check(rc, "dnx_paged_append")
 
