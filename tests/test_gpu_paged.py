@@ -331,6 +331,41 @@ def test_short_prefix_and_no_own_key(gpu_ready, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_a_page_listed_more_than_once(gpu_ready, kind):
+    """By two sequences, twice by one, and among the prefix's pages."""
+    b = Batch(11, [1, 2, 1], [70, 64, 33], 300, 8, 4, 64, kind, 32)
+    b.tables[0, 1] = b.tables[0, 0]
+    b.tables[1, 0] = b.tables[2, 0]
+    b.batch.prefix_pages[3] = b.tables[2, 0]
+    for x, own in zip(b.first_kv, zip(*b.own_kv)):
+        own[0][32:64] = own[0][:32]
+        own[1][:32] = own[2][:32]
+        x[96:128] = own[2][:32]
+    b.check()
+    b.check(40)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_two_calls_at_once(gpu_ready, kind):
+    """On two streams, with a workspace each, over one cache."""
+    a = Batch(12, [1] * 9, [40 * i + 1 for i in range(9)], 700, 8, 4, 64, kind, 32)
+    b = Batch(12, [1] * 9, [40 * i + 1 for i in range(9)], 700, 8, 4, 64, kind, 32)
+    b.q.mul_(0.5)
+    b.cache = a.cache
+    want = host(a.run()), host(b.run())
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for x, s in zip((a, b), streams):
+        x.out.zero_()
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for x, s in zip((a, b), streams):
+            x.run(stream=s)
+    torch.cuda.synchronize()
+    for x, w in zip((a, b), want):
+        assert np.array_equal(host(x.out), w)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_more_tokens_than_own_keys(gpu_ready, kind):
     """The first of them see the prefix alone, under the widest window too."""
     b = Batch(9, [3], [1], 50, 4, 2, 64, kind, 16)
