@@ -36,7 +36,7 @@ struct PagedArgs {
   int kv_heads, heads, group;
   const int32_t *starts, *lens, *tables, *prefix_pages;
   int64_t table_stride;
-  int prefix_len, seqs, tokens, max_len;
+  int prefix_len, seqs, tokens, max_len;   // max_len: within the tables too
   const float *q, *gate;
   float *out, *stat, *part;   // partials: stat [rows][splits][2], part [rows][splits][hd]
   int window, splits, joined;
@@ -66,6 +66,8 @@ struct Item {
   bool own;
   int kvh, run, row0, rows, t0, first;   // first: the place of token t0 among the keys
   int k_lo, k_hi, count, joined;
+  int most;                 // of the list's keys, whatever lens says
+  int page[2];              // of a wave's first keys in a narrow block, and 16 further
   const int32_t* table;
 };
 
@@ -101,18 +103,18 @@ DNX_DEV Seen row_sees(const PagedArgs& a, const Item& w, int r) {
 // 16 keys of an item from kt on (a page holds whole sixteens) as resources
 // over one head's rows of the cache: what lies behind the last key, or in a
 // page outside the cache, reads as zeros without touching memory. The page is
-// looked up ahead of its use (page_at: the last key's, where kt lies past it)
-// and without a branch, so that the loads of several do not wait in turn.
+// looked up ahead of its use (page_at; past the list's end its last one) and
+// without a branch or the sequence's length, so that no load waits for another.
 struct Block {
   i32x4 keys, values;
   int end;      // its keys lie before this key (none: not after the first)
 };
 template <bool kJoined>
 DNX_DEV int page_at(const PagedArgs& a, const Item& w, int kt) {
-  const int key = min(kt, w.k_hi - 1);
-  const bool own = !kJoined || key >= w.joined;
+  const bool own = !kJoined || kt >= w.joined;
   const int32_t* table = own ? w.table : a.prefix_pages;
-  const int place = !kJoined ? key : own ? key - w.joined : min(key, a.prefix_len - 1);
+  const int place = own ? min(kJoined ? kt - w.joined : kt, w.most - 1)
+                        : min(kt, a.prefix_len - 1);
   return __builtin_amdgcn_readfirstlane(table[place >> a.page_bits]);
 }
 // Blocks as seen from `behind` keys before them: the offset of key i of the
@@ -449,7 +451,12 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
   float q[L::ND][L::EK];
   int kt = next(first), after = kt;
   if (kt < w.k_hi) {
-    pages(kt);
+    if (kt == first) {
+#pragma unroll
+      for (int u = 0; u < U; u++) page[u] = w.page[u];
+    } else {
+      pages(kt);
+    }
     load_query<C, HD>(qp, g4, q);
     blocks(kt);
     request_keys();
@@ -618,9 +625,10 @@ DNX_DEV void few(const PagedArgs& a, const Item& w, uint8_t* lds) {
     while (at < w.k_hi && (lo >= at + KS || hi <= at)) at += kStride;
     return at;
   };
-  int kt = next(w.k_lo + KS * wave), after = kt;
+  const int first = w.k_lo + KS * wave;
+  int kt = next(first), after = kt;
   if (kt < w.k_hi) {
-    page = page_at<kJoined>(a, w, kt);
+    page = kt == first ? w.page[0] : page_at<kJoined>(a, w, kt);
     block = block_at<float, HD, kJoined>(a, w, kt, page);
     load_keys<float, HD>(block, a.row_bytes, l16, g4, x);
     load_values<float, HD>(block, a.row_bytes, l16, g4, x);
@@ -628,6 +636,7 @@ DNX_DEV void few(const PagedArgs& a, const Item& w, uint8_t* lds) {
     page = page_at<kJoined>(a, w, after);
   }
   __syncthreads();
+  int q_at = 4 * g4;
   while (kt < w.k_hi) {
     const int end = block.end;
     const int then = next(after + kStride);
@@ -637,7 +646,7 @@ DNX_DEV void few(const PagedArgs& a, const Item& w, uint8_t* lds) {
     float4 y[2][R];
     auto read = [&](int d) {
 #pragma unroll
-      for (int r = 0; r < R; r++) y[d & 1][r] = *(const float4*)&q[r * HD + 4 * (4 * d + g4)];
+      for (int r = 0; r < R; r++) y[d & 1][r] = *(const float4*)&q[q_at + r * HD + 16 * d];
     };
     read(0);
 #pragma unroll
@@ -653,7 +662,7 @@ DNX_DEV void few(const PagedArgs& a, const Item& w, uint8_t* lds) {
         s[r] = fmaf(element<float>(x.k[d], 3), z.w, s[r]);
       }
     }
-    asm volatile("" : : : "memory");       // nor kept for the next step
+    asm("" : "+v"(q_at));                  // nor kept for the next step
     load_keys<float, HD>(block, a.row_bytes, l16, g4, x);
     auto sees = [&](int key) { return key >= lo && key < min(hi, end); };
     const bool seen = sees(kt + l16);
@@ -1106,40 +1115,47 @@ DNX_DEV void block_of_16(const PagedArgs& a, const Item& w, int rows, uint8_t* l
 
 // The prefix's workgroups, then the sequences' own: both kinds in one launch,
 // so that the matrix cores' work on the prefix runs beside the reading of the
-// sequences' keys. Workgroups go round the eight XCDs, each with an L2 of its
+// sequences' keys (64 tokens, 8192 shared keys, 128 to 2048 own, 32 / 8 heads,
+// hd 128, bf16: 93 us, alone 41 and 69; the own ones first 100, with 16384
+// shared and up to 400 own 78 against 105). Workgroups go round the eight XCDs, each with an L2 of its
 // own: the blocks of rows that read the same keys go to one of them.
 template <typename C, int HD>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 paged_attention_kernel(PagedArgs a) {
   __shared__ __align__(16) uint8_t lds[attention_lds<C, HD>()];
   Item w;
-  int64_t id = blockIdx.x;
-  w.own = id >= a.prefix_items;
-  if (w.own) id -= a.prefix_items;
+  uint32_t id = blockIdx.x;
+  w.own = id >= (uint32_t)a.prefix_items;
+  if (w.own) id -= (uint32_t)a.prefix_items;
   const PartArgs part = w.own ? a.own : a.prefix;
-  const int64_t turn = id / 8;
-  int64_t unit = turn / part.blocks * 8 + id % 8;
-  const int block = (int)(turn % part.blocks);
-  w.kvh = (int)(unit % a.kv_heads);
-  unit /= a.kv_heads;
-  w.run = (int)(unit % part.runs);
-  const int64_t b = unit / part.runs;
-  const int seq = (int)min(b, (int64_t)a.seqs - 1);
-  const int all = a.starts[a.seqs], s0 = a.starts[seq], s1 = a.starts[seq + 1], len = a.lens[seq];
-  if (b > (w.own ? a.seqs - 1 : 0)) return;
+  const uint32_t turn = id / 8, unit = turn / (uint32_t)part.blocks * 8 + id % 8;
+  const int block = (int)(turn % (uint32_t)part.blocks);
+  const uint32_t set = unit / (uint32_t)a.kv_heads, b = set / (uint32_t)part.runs;
+  w.kvh = (int)(unit % (uint32_t)a.kv_heads);
+  w.run = (int)(set % (uint32_t)part.runs);
+  if (b > (w.own ? (uint32_t)a.seqs - 1 : 0)) return;
+  w.k_lo = w.run * part.keys;
+  w.joined = w.own ? a.joined : 0;
+  w.table = w.own ? a.tables + b * a.table_stride : a.prefix_pages;
+  w.most = w.own ? a.max_len : a.prefix_len;
+  // One wait for everything that the first keys' addresses and rows need.
+  int all = a.starts[a.seqs], s0 = a.starts[b], s1 = a.starts[b + 1], len = a.lens[b];
+  {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int first = w.k_lo + (sizeof(C) == 4 ? 16 : 32) * wave;
+    w.page[0] = page_at<true>(a, w, first);
+    w.page[1] = page_at<true>(a, w, first + 16);
+    // (Not volatile: behind that the pages are no scalar loads.)
+    asm("" : "+s"(all), "+s"(s0), "+s"(s1), "+s"(len), "+s"(w.page[0]), "+s"(w.page[1]));
+  }
   const int live = max(0, min(all, a.tokens));
   w.t0 = w.own ? max(0, min(s0, live)) : 0;
   const int t1 = w.own ? max(w.t0, min(s1, live)) : live;
   w.first = w.own ? len - (t1 - w.t0) : 0;
-  w.table = w.own ? a.tables + seq * a.table_stride : a.prefix_pages;
-  w.count = w.own ? (int)max(min((int64_t)min(len, a.max_len), a.table_stride << a.page_bits),
-                             (int64_t)0)
-                  : a.prefix_len;
+  w.count = w.own ? max(min(len, a.max_len), 0) : a.prefix_len;
   w.row0 = block * (part.wide ? kPagedWide : kPagedNarrow);
   w.rows = (t1 - w.t0) * a.group;
   if (w.row0 >= w.rows) return;
-  w.joined = w.own ? a.joined : 0;
-  w.k_lo = w.run * part.keys;
   w.k_hi = min(w.joined > 0 && w.count == 0 ? a.prefix_len : w.joined + w.count,
                w.k_lo + part.keys);
   if (part.wide) {
@@ -1164,8 +1180,8 @@ __global__ void __launch_bounds__(kThreads) paged_combine_kernel(PagedArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t r = (int64_t)blockIdx.x * kWaves + wave;
+  if (r >= (int64_t)a.tokens * a.heads) return;
   const int live = max(0, min(a.starts[a.seqs], a.tokens));
-  if (r >= (int64_t)live * a.heads) return;
   // Resources that end with the row's runs: lanes and runs past them read 0.
   const i32x4 srs = buffer_rsrc(a.stat + 2 * r * a.splits, (uint32_t)a.splits * 8u);
   const i32x4 prs = buffer_rsrc(a.part + r * a.splits * HD, (uint32_t)(a.splits * HD) * 4u);
@@ -1186,6 +1202,7 @@ __global__ void __launch_bounds__(kThreads) paged_combine_kernel(PagedArgs a) {
   };
   load(0);
   __builtin_amdgcn_sched_barrier(0);   // all requested before the first wait
+  if (r >= (int64_t)live * a.heads) return;   // behind the last sequence
   const float l = __int_as_float(ml.y), m = lane < a.splits ? __int_as_float(ml.x) : -INFINITY;
   const float top = wave_max_dpp(m);
   const float f = partial_factor(m, l, top);
@@ -1211,9 +1228,14 @@ PartArgs part_of(const PagedPart& p) {
   return {p.wide, p.few, (int)p.blocks, (int)p.runs, (int)p.keys};
 }
 
+// The most own keys of a sequence that can be seen.
+int64_t most_own(const dnx_paged_cache* c, const dnx_paged_batch* b) {
+  return std::min(b->max_len, b->table_stride * c->page);
+}
+
 PagedSplit split_of(const dnx_paged_cache* c, const dnx_paged_batch* b, int64_t heads) {
   return paged_split(b->seqs, b->tokens, std::min(b->max_tokens, b->tokens), heads / c->kv_heads,
-                     c->kv_heads, b->prefix_len, b->max_len, c->type == DNX_F32);
+                     c->kv_heads, b->prefix_len, most_own(c, b), c->type == DNX_F32);
 }
 
 }  // namespace
@@ -1260,7 +1282,7 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
   a.prefix_len = (int)batch->prefix_len;
   a.seqs = (int)batch->seqs;
   a.tokens = (int)batch->tokens;
-  a.max_len = (int)batch->max_len;
+  a.max_len = (int)most_own(cache, batch);
   a.q = q;
   a.gate = gate;
   a.out = out;
