@@ -87,6 +87,111 @@ DNX_DEV int pack4(int a, int b, int c, int d) {
   return (a & 0xff) | ((b & 0xff) << 8) | ((c & 0xff) << 16) | (int)((uint32_t)d << 24);
 }
 
+// Four normed values' part of a row's sum of squares and top = max |y| without
+// r. The sum also tells of an infinity or NaN: it is finite in 64 bits for
+// finite floats, and nothing times a product is added to it, for one in w.
+DNX_DEV void norm4(float4 s4, float4 w4, double& sum, double& top) {
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    const double s = (&s4.x)[c], y = s * (double)(&w4.x)[c];
+    sum = fma(y, 0.0, fma(s, s, sum));
+    top = fmax(top, fabs(y));
+  }
+}
+
+// The workgroup's sum and top.
+DNX_DEV void norm_reduce(double& sum, double& top) {
+  __shared__ double part[2][kMaxThreads / 64];
+  const int tid = threadIdx.x;
+  sum = wave_sum64(sum);
+  top = wave_max64(top);
+  if ((tid & 63) == 0) {
+    part[0][tid >> 6] = sum;
+    part[1][tid >> 6] = top;
+  }
+  __syncthreads();
+  sum = part[0][0];
+  top = part[1][0];
+  for (int k = 1; k < (int)blockDim.x / 64; k++) {
+    sum += part[0][k];
+    top = fmax(top, part[1][k]);
+  }
+}
+
+DNX_DEV float norm_scale(double sum, double top, int cols, float eps) {
+  return (float)(top / 127.0 * (1.0 / sqrt(sum / (double)cols + (double)eps)));
+}
+
+// 127 / top, rounded up by 2^-50.
+DNX_DEV double code_factor(double top, bool fine) {
+  return fine && top > 0.0 ? 127.0 / top * (1.0 + 0x1p-50) : 0.0;
+}
+
+// A normed row of more values than registers hold: read again for the codes.
+// 512 x 32768 with addition and norm: 60 us, 3.7 TB/s (with 16 steps in registers,
+// most of them spilled, 153).
+template <bool kAdd>
+__global__ void __launch_bounds__(kMaxThreads)
+long_rows_i8_kernel(const float* x, const float* m, float* x_out, const float* __restrict__ w,
+                    int8_t* __restrict__ qs, float* __restrict__ scales, int cols, int cols_pad,
+                    float eps) {
+  constexpr int U = 4;                    // steps whose loads are in flight together
+  const int quads = cols / 4, threads = blockDim.x, tid = threadIdx.x;
+  const size_t at = (size_t)blockIdx.x * cols;
+  const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  double sum = 0.0, top = 0.0;
+  for (int i0 = tid; i0 < quads; i0 += U * threads) {
+    float4 s[U], u[U], a[U];
+#pragma unroll
+    for (int e = 0; e < U; e++) {
+      const int i = i0 + e * threads;
+      s[e] = u[e] = a[e] = zero;
+      if (i < quads) {
+        s[e] = load4(x + at + 4 * i);
+        u[e] = load4(w + 4 * i);
+        if constexpr (kAdd) a[e] = load4(m + at + 4 * i);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < U; e++) {
+      const int i = i0 + e * threads;
+      if constexpr (kAdd) {
+        s[e] = make_float4(s[e].x + a[e].x, s[e].y + a[e].y, s[e].z + a[e].z, s[e].w + a[e].w);
+        if (i < quads) *(float4*)(x_out + at + 4 * i) = s[e];
+      }
+      norm4(s[e], u[e], sum, top);
+    }
+  }
+  norm_reduce(sum, top);
+  const bool fine = sum < INFINITY;
+  const double inv = code_factor(top, fine);
+  const float* from = kAdd ? x_out : x;
+  int* out = (int*)(qs + (size_t)blockIdx.x * cols_pad);
+  for (int i0 = tid; i0 < quads; i0 += U * threads) {
+    float4 s[U], u[U];
+#pragma unroll
+    for (int e = 0; e < U; e++) {
+      const int i = i0 + e * threads;
+      s[e] = u[e] = zero;
+      if (i < quads) {
+        s[e] = load4(from + at + 4 * i);
+        u[e] = load4(w + 4 * i);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < U; e++) {
+      int q[4];
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        q[c] = code1((double)(&s[e].x)[c] * (double)(&u[e].x)[c], inv);
+      const int i = i0 + e * threads;
+      if (i < quads) out[i] = fine ? pack4(q[0], q[1], q[2], q[3]) : 0;
+    }
+  }
+  for (int i = quads + tid; i < cols_pad / 4; i += threads) out[i] = 0;
+  if (tid == 0) scales[blockIdx.x] = fine ? norm_scale(sum, top, cols, eps) : NAN;
+}
+
 // One workgroup a row, four values per thread and step e (V steps cover the
 // row): the row stays in registers between the reduction and the codes, so
 // each byte is read once. 4099 x 4096 with addition and norm: 44 us, 5.0 TB/s
@@ -123,35 +228,13 @@ rows_i8_kernel(const S* x, const float* __restrict__ m, float* x_out, const floa
     }
   }
   // top = max |y| without r; `fine`: the row holds no infinity or NaN. As they
-  // are, the rows' sizes order as their bits do, infinities and NaN above all;
-  // in the norm the sum of squares tells, finite in 64 bits for finite floats
-  // (nothing times a product is added to it, for an infinity or NaN in w).
+  // are, the rows' sizes order as their bits do, infinities and NaN above all.
   double sum = 0.0, top = 0.0;
   bool fine;
-  const int waves = threads / 64;
   if constexpr (kNorm) {
-    __shared__ double part[2][kMaxThreads / 64];
 #pragma unroll
-    for (int e = 0; e < V; e++)
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        const double s = (&xv[e].x)[c], y = s * (double)(&wv[e].x)[c];
-        sum = fma(y, 0.0, fma(s, s, sum));
-        top = fmax(top, fabs(y));
-      }
-    sum = wave_sum64(sum);
-    top = wave_max64(top);
-    if ((tid & 63) == 0) {
-      part[0][tid >> 6] = sum;
-      part[1][tid >> 6] = top;
-    }
-    __syncthreads();
-    sum = part[0][0];
-    top = part[1][0];
-    for (int k = 1; k < waves; k++) {
-      sum += part[0][k];
-      top = fmax(top, part[1][k]);
-    }
+    for (int e = 0; e < V; e++) norm4(xv[e], wv[e], sum, top);
+    norm_reduce(sum, top);
     fine = sum < INFINITY;
   } else {
     __shared__ uint32_t part[kMaxThreads / 64];
@@ -164,11 +247,11 @@ rows_i8_kernel(const S* x, const float* __restrict__ m, float* x_out, const floa
     if ((tid & 63) == 0) part[tid >> 6] = bits;
     __syncthreads();
     bits = part[0];
-    for (int k = 1; k < waves; k++) bits = max(bits, part[k]);
+    for (int k = 1; k < threads / 64; k++) bits = max(bits, part[k]);
     fine = bits < 0x7f800000u;
     top = __uint_as_float(bits);
   }
-  const double inv = fine && top > 0.0 ? 127.0 / top * (1.0 + 0x1p-50) : 0.0;
+  const double inv = code_factor(top, fine);
   int* out = (int*)(qs + (size_t)blockIdx.x * cols_pad);
 #pragma unroll
   for (int e = 0; e < V; e++) {
@@ -184,9 +267,8 @@ rows_i8_kernel(const S* x, const float* __restrict__ m, float* x_out, const floa
   }
   for (int i = quads + tid; i < cols_pad / 4; i += threads) out[i] = 0;
   if (tid == 0) {
-    double scale = top / 127.0;
-    if constexpr (kNorm) scale *= 1.0 / sqrt(sum / (double)cols + (double)eps);
-    scales[blockIdx.x] = fine ? (float)scale : NAN;
+    const float scale = kNorm ? norm_scale(sum, top, cols, eps) : (float)(top / 127.0);
+    scales[blockIdx.x] = fine ? scale : NAN;
   }
 }
 
@@ -211,12 +293,21 @@ int launch_rows(const S* x, const float* m, float* x_out, const float* w, int8_t
   const int V = rows >= kManyRows && steps <= 4 ? 4
                 : steps <= 1 ? 1 : steps <= 2 ? 2 : steps <= 4 ? 4 : kMaxV;
   const unsigned threads = (unsigned)(((quads + V - 1) / V + 63) / 64 * 64);
-  auto k = V == 1   ? rows_i8_kernel<S, 1, kNorm, kAdd>
-           : V == 2 ? rows_i8_kernel<S, 2, kNorm, kAdd>
-           : V == 4 ? rows_i8_kernel<S, 4, kNorm, kAdd>
-                    : rows_i8_kernel<S, kMaxV, kNorm, kAdd>;
-  hipLaunchKernelGGL(k, dim3((unsigned)rows), dim3(threads), 0, (hipStream_t)stream, x, m, x_out, w,
-                     qs, scales, (int)cols, (int)cols_pad, eps);
+  auto launch = [&](auto k, unsigned n) {
+    hipLaunchKernelGGL(k, dim3((unsigned)rows), dim3(n), 0, (hipStream_t)stream, x, m, x_out, w, qs,
+                       scales, (int)cols, (int)cols_pad, eps);
+  };
+  if (V == 1) {
+    launch(rows_i8_kernel<S, 1, kNorm, kAdd>, threads);
+  } else if (V == 2) {
+    launch(rows_i8_kernel<S, 2, kNorm, kAdd>, threads);
+  } else if (V == 4) {
+    launch(rows_i8_kernel<S, 4, kNorm, kAdd>, threads);
+  } else if constexpr (kNorm) {
+    launch(long_rows_i8_kernel<kAdd>, kMaxThreads);
+  } else {
+    launch(rows_i8_kernel<S, kMaxV, kNorm, kAdd>, threads);
+  }
   return hipGetLastError() == hipSuccess ? DNX_OK : DNX_ELAUNCH;
 }
 

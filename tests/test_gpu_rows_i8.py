@@ -132,6 +132,26 @@ def test_norm_weight_without_a_code(gpu_ready, rows, bad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cols", [16384, 16388, 40000])
+@pytest.mark.parametrize("at", [0, -1])
+def test_long_norm_rows_without_a_code(gpu_ready, cols, at):
+    """Rows about the length from which they are read twice."""
+    rng = np.random.default_rng(cols)
+    x = rng.standard_normal((4, cols)).astype(np.float32)
+    x[0], x[1, at], x[2, at] = 0.0, np.nan, -np.inf
+    w = np.ones(cols, np.float32)
+    pad = -(-cols // 32) * 32
+    qs, scales = outputs(4, pad)
+    D.rms_norm_i8r(dev(x), dev(w), qs, scales, 4, cols, pad, EPS)
+    q, s = host(qs), host(scales)
+    assert (q[:3] == 0).all() and s[0] == 0 and np.isnan(s[1]) and np.isnan(s[2])
+    assert np.abs(q[3].astype(int)).max() == 127 and np.isfinite(s[3])
+    w[at] = np.inf
+    D.rms_norm_i8r(dev(x), dev(w), qs, scales, 4, cols, pad, EPS)
+    assert np.isnan(host(scales)[:4]).all() and (host(qs)[:4] == 0).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,cols,pad", SHAPES + [(600, 260, 288), (513, 4096, 4096),
                                                     (700, 8196, 8224)])
 @pytest.mark.parametrize("add", [False, True])
