@@ -24,6 +24,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
+constexpr int kCombineRuns = 8;   // more of a row's are added by four waves
 constexpr float kSlack = 8.0f;   // of a running maximum, in units of log2
 
 struct PartArgs {
@@ -1169,22 +1170,25 @@ paged_attention_kernel(PagedArgs a) {
   }
 }
 
-// A row's partial results added in order, one wave a row: lane s holds the
-// statistics of run s, lane i sums dims ND i .. (at most 64 runs), eight runs'
-// values requested at once. What runs without a weight hold does not count.
-// 4.7 us for 64 tokens of 32 heads, hd 128, 9 runs; 3.9 for 16 tokens of 16:
-// the launch and two waits for memory.
-template <int HD>
+// A row's partial results added in order by W waves, an equal part of the runs
+// each (at most 64): lane s holds the statistics of the part's run s, lane i
+// sums dims ND i .., eight runs' values requested at once. What runs without a
+// weight hold does not count. 4.7 us for 64 tokens of 32 heads, hd 128, 9 runs;
+// 3.9 for 16 tokens of 16: the launch and two waits for memory.
+template <int HD, int W>
 __global__ void __launch_bounds__(kThreads) paged_combine_kernel(PagedArgs a) {
   constexpr int ND = HD / 64, U = 8;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t r = (int64_t)blockIdx.x * kWaves + wave;
+  const int64_t r = (int64_t)blockIdx.x * (kWaves / W) + wave / W;
   if (r >= (int64_t)a.tokens * a.heads) return;
   const int live = max(0, min(a.starts[a.seqs], a.tokens));
-  // Resources that end with the row's runs: lanes and runs past them read 0.
-  const i32x4 srs = buffer_rsrc(a.stat + 2 * r * a.splits, (uint32_t)a.splits * 8u);
-  const i32x4 prs = buffer_rsrc(a.part + r * a.splits * HD, (uint32_t)(a.splits * HD) * 4u);
+  const int per = (a.splits + W - 1) / W, first = W == 1 ? 0 : wave * per;
+  const int runs = max(0, min(per, a.splits - first));
+  // Resources that end with the part's runs: lanes and runs past them read 0.
+  const int64_t at0 = r * a.splits + first;
+  const i32x4 srs = buffer_rsrc(a.stat + 2 * at0, (uint32_t)runs * 8u);
+  const i32x4 prs = buffer_rsrc(a.part + at0 * HD, (uint32_t)(runs * HD) * 4u);
   const i32x2 ml = dnx_raw_buffer_load_v2i32(srs, lane * 8, 0, 0);
   float v[U][ND];
   auto load = [&](int s0) {
@@ -1203,13 +1207,13 @@ __global__ void __launch_bounds__(kThreads) paged_combine_kernel(PagedArgs a) {
   load(0);
   __builtin_amdgcn_sched_barrier(0);   // all requested before the first wait
   if (r >= (int64_t)live * a.heads) return;   // behind the last sequence
-  const float l = __int_as_float(ml.y), m = lane < a.splits ? __int_as_float(ml.x) : -INFINITY;
-  const float top = wave_max_dpp(m);
+  const float l = __int_as_float(ml.y), m = lane < runs ? __int_as_float(ml.x) : -INFINITY;
+  float top = wave_max_dpp(m);
   const float f = partial_factor(m, l, top);
-  const float total = wave_sum_dpp(l * f);
+  float total = wave_sum_dpp(l * f);
   const uint64_t with = __ballot(l != 0.0f);
   float acc[ND] = {};
-  for (int s0 = 0; s0 < a.splits; s0 += U) {
+  for (int s0 = 0; s0 < runs; s0 += U) {
     if (s0 > 0) load(s0);
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -1217,6 +1221,29 @@ __global__ void __launch_bounds__(kThreads) paged_combine_kernel(PagedArgs a) {
       const bool counts = (with >> (s0 + u)) & 1;
 #pragma unroll
       for (int i = 0; i < ND; i++) acc[i] = fmaf(counts ? v[u][i] : 0.0f, fs, acc[i]);
+    }
+  }
+  if constexpr (W > 1) {
+    __shared__ float stats[W][2], sums[W][HD];
+    if (lane == 0) stats[wave][0] = top, stats[wave][1] = total;
+#pragma unroll
+    for (int i = 0; i < ND; i++) sums[wave][ND * lane + i] = acc[i];
+    __syncthreads();
+    if (wave > 0) return;
+    top = stats[0][0];
+#pragma unroll
+    for (int k = 1; k < W; k++) top = fmaxf(top, stats[k][0]);
+    total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < ND; i++) acc[i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < W; k++) {
+      const float part = stats[k][1];
+      if (part == 0.0f) continue;
+      const float fk = partial_factor(stats[k][0], part, top);
+      total = fmaf(part, fk, total);
+#pragma unroll
+      for (int i = 0; i < ND; i++) acc[i] = fmaf(sums[k][ND * lane + i], fk, acc[i]);
     }
   }
   const float g = row_scale(total, a.gate, r);
@@ -1311,8 +1338,13 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
     if (hipGetLastError() != hipSuccess) return DNX_ELAUNCH;
   }
   if (a.splits != 1) {
-    const int64_t blocks = (batch->tokens * heads + kWaves - 1) / kWaves;
-    auto k = cache->hd == 128 ? paged_combine_kernel<128> : paged_combine_kernel<64>;
+    const int64_t rows = batch->tokens * heads;
+    const bool split = rows < kPagedManyRows && a.splits > kCombineRuns;
+    const int64_t blocks = split ? rows : (rows + kWaves - 1) / kWaves;
+    auto k = cache->hd == 128 ? (split ? paged_combine_kernel<128, kWaves>
+                                       : paged_combine_kernel<128, 1>)
+                              : (split ? paged_combine_kernel<64, kWaves>
+                                       : paged_combine_kernel<64, 1>);
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(kThreads), 0, st, a);
   }
   return hipGetLastError() == hipSuccess ? DNX_OK : DNX_ELAUNCH;

@@ -30,7 +30,12 @@ struct PagedSplit {
 
 constexpr int kPagedNarrow = 16, kPagedWide = 64;   // rows of a workgroup
 constexpr int kPagedStep = 64;       // runs are whole steps
-constexpr int kPagedMaxRuns = 32;    // of the prefix, and of a sequence
+// Runs of the prefix, and of a sequence: up to 32, and more (256 in all) where
+// they hold 256 keys each and the call has few rows (whose partial results are
+// then added by four waves each). One token after 131072 keys, 8 heads over
+// one, hd 128, bf16: 45 us with 32 runs, 19 with 128 or 256; f32 147, 46, 34.
+constexpr int kPagedRuns = 32, kPagedMaxRuns = 256, kPagedLong = 256;
+constexpr int64_t kPagedManyRows = 1 << 20;
 
 // Wide blocks read the keys for 64 rows at once and take fewer products, but
 // one after another; narrow ones of the same rows run side by side and find
@@ -45,8 +50,8 @@ inline bool paged_wide(int64_t rows, int64_t units, int64_t keys, bool f32) {
   return rows > 128 || rows * keys * units > (f32 ? 1200000 : 4000000);
 }
 
-inline PagedPart paged_part(int64_t tokens, int64_t group, int64_t units, int64_t keys, bool f32, int64_t least,
-                            int64_t most) {
+inline PagedPart paged_part(int64_t tokens, int64_t group, int64_t units, int64_t keys, bool f32,
+                            int64_t least, int64_t most, int64_t max_runs) {
   PagedPart p{};
   const int64_t rows = tokens * group;
   p.wide = paged_wide(rows, units, keys, f32);
@@ -61,7 +66,8 @@ inline PagedPart paged_part(int64_t tokens, int64_t group, int64_t units, int64_
   const int64_t wgs = units * p.blocks;
   int64_t runs = (256 + wgs - 1) / wgs;
   runs = std::min(std::max(runs, (keys + most - 1) / most), std::max<int64_t>(1, keys / least));
-  runs = std::min<int64_t>(std::max<int64_t>(runs, 1), kPagedMaxRuns);
+  runs = std::min(runs, std::max<int64_t>(kPagedRuns, keys / kPagedLong));
+  runs = std::min<int64_t>(std::max<int64_t>(runs, 1), max_runs);
   p.keys = ((keys + runs - 1) / runs + kPagedStep - 1) / kPagedStep * kPagedStep;
   p.runs = (keys + p.keys - 1) / p.keys;
   return p;
@@ -72,8 +78,10 @@ inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, 
   // Without a prefix, keys that one workgroup walks in about the time of the
   // second launch (3 us) stay in one run: up to 256.
   const int64_t least = prefix_len == 0 && max_len <= 256 ? 256 : kPagedStep;
-  PagedSplit s{paged_part(tokens, group, kv_heads, prefix_len, f32, kPagedStep, 1 << 20),
-               paged_part(max_tokens, group, seqs * kv_heads, max_len, f32, least, 2048), 0};
+  const int64_t max_runs = tokens * group * kv_heads >= kPagedManyRows ? kPagedRuns
+                           : prefix_len > 0 ? kPagedMaxRuns / 2 : kPagedMaxRuns;
+  PagedSplit s{paged_part(tokens, group, kv_heads, prefix_len, f32, kPagedStep, 1 << 20, max_runs),
+               paged_part(max_tokens, group, seqs * kv_heads, max_len, f32, least, 2048, max_runs), 0};
   // A short prefix is joined to them where a CU for each workgroup is left: its
   // keys are then read once for each block of rows, but without the second
   // launch. Up to 384 keys, or 256 where the float32 matrix cores take 16 rows

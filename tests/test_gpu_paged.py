@@ -317,6 +317,17 @@ def test_short_prefix(gpu_ready, prefix, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("counts,lens,prefix,heads,hd", [
+    ([1], [70001], 0, 2, 64), ([2, 1], [33000, 5], 40000, 3, 64), ([1], [20], 66000, 9, 128)])
+def test_many_runs(gpu_ready, counts, lens, prefix, heads, hd, kind):
+    """Long caches of one key head: up to 256 runs to add, most of them empty
+    under a window."""
+    b = Batch(13, counts, lens, prefix, heads, 1, hd, kind, 256, pad=1, gate=True)
+    b.check()
+    b.check(3000)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_short_prefix_and_no_own_key(gpu_ready, kind):
     b = Batch(10, [1, 1], [0, 2], 20, 4, 2, 64, kind, 16)
     out = host(b.run())

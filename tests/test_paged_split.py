@@ -48,7 +48,7 @@ def test_every_key_has_a_run(split_of):
         tokens = seqs * each
         pr, orows, ps, prun, os_, orun, total, joined = split_of(seqs, tokens, each, group, kv, prefix,
                                                                 length, f32)
-        assert total == ps + os_ <= 64
+        assert total == ps + os_ <= 256
         if joined:       # one run of both, in which the own keys begin at a step
             assert (ps, os_) == (0, 1) and joined % 64 == 0 and prefix <= joined < prefix + 64
             assert joined + length <= orun <= 384 and orows >= 1
