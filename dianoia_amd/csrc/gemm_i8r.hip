@@ -27,49 +27,58 @@ struct I8RArgs {
 };
 
 // ---- Few tokens (a decode batch of up to 16): what it costs is to read the
-// weights once. A workgroup takes 16 weight rows and all tokens, its eight
-// waves an eighth of K each, both operands straight from memory into the
-// fragments of v_mfma_i32_16x16x64_i8 (lane l: row l % 16, the 16 bytes at k =
-// 16 (l / 16) of 64), four steps requested at once; the eight sums meet in
-// LDS. 13 x 6144 x 2048: 5.7 us, 2.3 TB/s, of which about 2.0 us are an empty
-// launch's.
+// weights once. A workgroup takes 16 or 32 weight rows (NR tiles) and all
+// tokens, its eight waves an eighth of K each, both operands straight from
+// memory into the fragments of v_mfma_i32_16x16x64_i8 (lane l: row l % 16, the
+// 16 bytes at k = 16 (l / 16) of 64), four steps requested at once; the eight
+// sums meet in LDS. 13 x 6144 x 2048: 5.1 us, 2.5 TB/s, of which about 2.0 us
+// are an empty launch's; 16 x 128256 x 4096 128 us, 4.2 TB/s.
 constexpr int kFewWaves = 8, kFewRows = 16, kFewSteps = 4;
 
+template <int NR>
 __global__ void __launch_bounds__(kFewWaves * 64) gemm_i8r_few_kernel(I8RArgs p) {
-  __shared__ int part[kFewWaves][16][16];
+  __shared__ int part[kFewWaves][NR][16][16];
   const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r0 = blockIdx.x * kFewRows;
+  const int r0 = blockIdx.x * kFewRows * NR;
   const i32x4 wrs = buffer_rsrc(p.w + (size_t)r0 * p.cols,
-                                (uint32_t)(min(kFewRows, p.rows - r0) * p.cols));
+                                (uint32_t)(min(kFewRows * NR, p.rows - r0) * p.cols));
   const i32x4 xrs = buffer_rsrc(p.x, (uint32_t)(p.n * p.cols));
   const int chunks = (p.cols + 63) / 64, per = (chunks + kFewWaves - 1) / kFewWaves;
   const int end = min(chunks, (wave + 1) * per);
-  v4i acc = {};
+  v4i acc[NR] = {};
   for (int c0 = wave * per; c0 < end; c0 += kFewSteps) {
-    i32x4 wv[kFewSteps], xv[kFewSteps];
+    i32x4 wv[kFewSteps][NR], xv[kFewSteps];
 #pragma unroll
     for (int u = 0; u < kFewSteps; u++) {
       // Past the row: past the resource (zeros), the next row's bytes follow.
       const int k = (c0 + u) * 64 + 16 * g4;
-      const int at = c0 + u < end && k < p.cols ? l16 * p.cols + k : -1;
-      wv[u] = dnx_raw_buffer_load_v4i32(wrs, at, 0, kStream);
-      xv[u] = dnx_raw_buffer_load_v4i32(xrs, at, 0, 0);
+      const bool in = c0 + u < end && k < p.cols;
+#pragma unroll
+      for (int i = 0; i < NR; i++)
+        wv[u][i] = dnx_raw_buffer_load_v4i32(wrs, in ? (16 * i + l16) * p.cols + k : -1, 0, kStream);
+      xv[u] = dnx_raw_buffer_load_v4i32(xrs, in ? l16 * p.cols + k : -1, 0, 0);
     }
     __builtin_amdgcn_sched_barrier(0);   // every load before the first product waits
 #pragma unroll
     for (int u = 0; u < kFewSteps; u++)
-      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(xv[u], wv[u], acc, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < NR; i++)
+        acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xv[u], wv[u][i], acc[i], 0, 0, 0);
   }
 #pragma unroll
-  for (int v = 0; v < 4; v++) part[wave][4 * g4 + v][l16] = acc[v];
-  __syncthreads();
-  const int t = threadIdx.x / 16, r = r0 + threadIdx.x % 16;
-  if (t >= p.n || r >= p.rows) return;
-  int sum = 0;
+  for (int i = 0; i < NR; i++)
 #pragma unroll
-  for (int w = 0; w < kFewWaves; w++) sum += part[w][t][threadIdx.x % 16];
-  p.y[(size_t)t * p.rows + r] = (float)sum * (p.x_scale[t] * p.w_scale[r]);
+    for (int v = 0; v < 4; v++) part[wave][i][4 * g4 + v][l16] = acc[i][v];
+  __syncthreads();
+  for (int o = threadIdx.x; o < NR * 256; o += kFewWaves * 64) {
+    const int c = o % (16 * NR), t = o / (16 * NR), r = r0 + c;
+    if (t >= p.n || r >= p.rows) continue;
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; w++) sum += part[w][c / 16][t][c % 16];
+    p.y[(size_t)t * p.rows + r] = (float)sum * (p.x_scale[t] * p.w_scale[r]);
+  }
 }
 
 // ---- Many tokens: tiles of TM tokens x TN weight rows through LDS. WM x WN
@@ -293,8 +302,10 @@ int dnx_gemm_i8r(const int8_t* w, const float* w_scale, const int8_t* x, const f
     case 5: return launch_tile<5, 4, 2, 2, 2, 3>(p, st);
     case 6: return launch_tile<6, 4, 4, 2, 2, 5>(p, st);
   }
-  hipLaunchKernelGGL(gemm_i8r_few_kernel, dim3((unsigned)((rows + kFewRows - 1) / kFewRows)),
-                     dim3(kFewWaves * 64), 0, st, p);
+  const int tiles = i8r_few_tiles(n, rows);
+  const int64_t wg_rows = kFewRows * tiles;
+  hipLaunchKernelGGL(tiles == 2 ? gemm_i8r_few_kernel<2> : gemm_i8r_few_kernel<1>,
+                     dim3((unsigned)((rows + wg_rows - 1) / wg_rows)), dim3(kFewWaves * 64), 0, st, p);
   return hipGetLastError() == hipSuccess ? DNX_OK : DNX_ELAUNCH;
 }
 

@@ -36,9 +36,19 @@ constexpr I8RTile kI8RTiles[] = {
 constexpr int kI8RCount = sizeof(kI8RTiles) / sizeof(kI8RTiles[0]);
 constexpr int kI8RFew = -1;
 
+// Tiles of 16 weight rows of a workgroup of the few-token kernel. Two read the
+// tokens half as often, which counts from about five of them on, but not where
+// they leave some CUs more rows than one would (us, one against two: 13 x 6144
+// x 2048 5.66 / 5.40, 16 x 128256 x 4096 139 / 128, 4 x 6144 x 2048 5.10 / 5.21,
+// 16 x 4096 x 2048 4.10 / 5.15, 16 x 12288 x 4096 16.7 / 17.7).
+inline int i8r_few_tiles(int64_t n, int64_t rows) {
+  const auto rounds = [&](int64_t wg_rows) { return ((rows + wg_rows - 1) / wg_rows + 255) / 256; };
+  return n > 4 && (2 * rounds(32) <= rounds(16) || rows > 32768) ? 2 : 1;
+}
+
 // The index of the tile kernel, or kI8RFew for batches of up to 16 tokens: the
 // kernel without LDS for its operands (13 x 1024 x 4096: 6.2 us against 6.8 of
-// the smallest tile, 1 x 6144 x 2048 5.5 against 5.8; 16 x 6144 x 2048 6.7
+// the smallest tile, 1 x 6144 x 2048 5.5 against 5.8; 16 x 6144 x 2048 5.5
 // against 6.0).
 inline int i8r_route(int64_t n, int64_t rows, int64_t cols) {
   if (n <= 16) return kI8RFew;

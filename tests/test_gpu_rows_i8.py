@@ -190,6 +190,10 @@ PRODUCTS = [(1, 1, 32), (1, 33, 64), (5, 31, 96), (13, 1000, 2048), (16, 64, 409
             (1024, 4304, 1152), (1, 9000, 4096), (3, 128, 131040)]
 
 
+# Two tiles of rows a workgroup: whole, and a last one that is partly there.
+PRODUCTS += [(5, 8192, 64), (16, 8161, 96), (9, 4113, 2080), (13, 33001, 160)]
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,rows,cols", PRODUCTS)
 def test_product(gpu_ready, n, rows, cols):
