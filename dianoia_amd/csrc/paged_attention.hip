@@ -116,7 +116,10 @@ DNX_DEV int page_at(const PagedArgs& a, const Item& w, int kt) {
   const int32_t* table = own ? w.table : a.prefix_pages;
   const int place = own ? min(kJoined ? kt - w.joined : kt, w.most - 1)
                         : min(kt, a.prefix_len - 1);
-  return __builtin_amdgcn_readfirstlane(table[place >> a.page_bits]);
+  // Constant memory to the kernel: a scalar load wherever it stands (behind a
+  // store or a barrier the compiler would wait for a vector load instead).
+  typedef const __attribute__((address_space(4))) int32_t* Constant;
+  return __builtin_amdgcn_readfirstlane(((Constant)(uintptr_t)table)[place >> a.page_bits]);
 }
 // Blocks as seen from `behind` keys before them: the offset of key i of the
 // block is that of row behind + i.
@@ -1105,6 +1108,21 @@ constexpr int attention_lds() {
   return w > n ? w : n;
 }
 
+// Whether none of an own block's rows, up to `end`, sees a key of its run: the
+// run lies behind the sequence's keys (where the bound on the lengths is far
+// above them), or the window or the rows' own places end before it. Such a run
+// only says so; its sums are not written. 64 sequences of 200 keys, bound 32768,
+// 32 / 8 heads, hd 128, bf16: 65 us without this and with a sequence's runs side
+// by side in the launch, 33 with both (13 with the bound at 200).
+DNX_DEV bool unseen(const PagedArgs& a, const Item& w, int end) {
+  int lo = w.k_lo, hi = w.k_hi;
+  if (lo < hi && (a.window > 0 || w.rows > a.group)) {
+    if (a.window > 0) lo = max(lo, w.first + w.row0 / a.group - a.window + 1);
+    hi = min(hi, w.first + (end - 1) / a.group + 1);
+  }
+  return lo >= hi;
+}
+
 template <typename C, int HD, bool kJoined>
 DNX_DEV void block_of_16(const PagedArgs& a, const Item& w, int rows, uint8_t* lds) {
   if constexpr (sizeof(C) == 4) {
@@ -1131,10 +1149,13 @@ paged_attention_kernel(PagedArgs a) {
   const PartArgs part = w.own ? a.own : a.prefix;
   const uint32_t turn = id / 8, unit = turn / (uint32_t)part.blocks * 8 + id % 8;
   const int block = (int)(turn % (uint32_t)part.blocks);
-  const uint32_t set = unit / (uint32_t)a.kv_heads, b = set / (uint32_t)part.runs;
+  // The sequences' first runs before their second ones: where the bound on the
+  // lengths is far above them, those that have keys start at once.
+  const uint32_t set = unit / (uint32_t)a.kv_heads, sets = w.own ? (uint32_t)a.seqs : 1;
+  const uint32_t b = set % sets;
   w.kvh = (int)(unit % (uint32_t)a.kv_heads);
-  w.run = (int)(set % (uint32_t)part.runs);
-  if (b > (w.own ? (uint32_t)a.seqs - 1 : 0)) return;
+  w.run = (int)(set / sets);
+  if (w.run >= part.runs) return;
   w.k_lo = w.run * part.keys;
   w.joined = w.own ? a.joined : 0;
   w.table = w.own ? a.tables + b * a.table_stride : a.prefix_pages;
@@ -1146,7 +1167,6 @@ paged_attention_kernel(PagedArgs a) {
     const int first = w.k_lo + (sizeof(C) == 4 ? 16 : 32) * wave;
     w.page[0] = page_at<true>(a, w, first);
     w.page[1] = page_at<true>(a, w, first + 16);
-    // (Not volatile: behind that the pages are no scalar loads.)
     asm("" : "+s"(all), "+s"(s0), "+s"(s1), "+s"(len), "+s"(w.page[0]), "+s"(w.page[1]));
   }
   const int live = max(0, min(all, a.tokens));
@@ -1159,6 +1179,15 @@ paged_attention_kernel(PagedArgs a) {
   if (w.row0 >= w.rows) return;
   w.k_hi = min(w.joined > 0 && w.count == 0 ? a.prefix_len : w.joined + w.count,
                w.k_lo + part.keys);
+  const int end = min(w.row0 + (part.wide ? kPagedWide : kPagedNarrow), w.rows);
+  if (w.own && a.splits > 1 && unseen(a, w, end)) {
+    const int r = w.row0 + threadIdx.x;
+    if (r < end) {
+      const int64_t p = row_at(a, w, r) * a.splits + a.prefix.runs + w.run;
+      *(float2*)(a.stat + 2 * p) = make_float2(-INFINITY, 0.0f);
+    }
+    return;
+  }
   if (part.wide) {
     wide<C, HD>(a, w, lds);
     return;
