@@ -31,7 +31,7 @@ struct I8RArgs {
 // tokens, its eight waves an eighth of K each, both operands straight from
 // memory into the fragments of v_mfma_i32_16x16x64_i8 (lane l: row l % 16, the
 // 16 bytes at k = 16 (l / 16) of 64), four steps requested at once; the eight
-// sums meet in LDS. 13 x 6144 x 2048: 5.1 us, 2.5 TB/s, of which about 2.0 us
+// sums meet in LDS. 13 x 6144 x 2048: 5.4 us, 2.4 TB/s, of which about 2.0 us
 // are an empty launch's; 16 x 128256 x 4096 128 us, 4.2 TB/s.
 constexpr int kFewWaves = 8, kFewRows = 16, kFewSteps = 4;
 

@@ -24,7 +24,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kCombineRuns = 8;   // more of a row's are added by four waves
 constexpr float kSlack = 8.0f;   // of a running maximum, in units of log2
 
 struct PartArgs {
@@ -1202,8 +1201,10 @@ paged_attention_kernel(PagedArgs a) {
 // A row's partial results added in order by W waves, an equal part of the runs
 // each (at most 64): lane s holds the statistics of the part's run s, lane i
 // sums dims ND i .., eight runs' values requested at once. What runs without a
-// weight hold does not count. 4.7 us for 64 tokens of 32 heads, hd 128, 9 runs;
-// 3.9 for 16 tokens of 16: the launch and two waits for memory.
+// weight hold does not count. Under a trace 5.0 us for 64 tokens of 32 heads,
+// hd 128, 9 runs by one wave a row (5.8 by four); 4.0 for 16 tokens of 16, 18
+// runs, by four (by one 0.6 more): the launch and two
+// waits for memory.
 template <int HD, int W>
 __global__ void __launch_bounds__(kThreads) paged_combine_kernel(PagedArgs a) {
   constexpr int ND = HD / 64, U = 8;
@@ -1368,7 +1369,7 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
   }
   if (a.splits != 1) {
     const int64_t rows = batch->tokens * heads;
-    const bool split = rows < kPagedManyRows && a.splits > kCombineRuns;
+    const bool split = rows < kPagedManyRows && a.splits > (rows < 2048 ? 8 : 16);
     const int64_t blocks = split ? rows : (rows + kWaves - 1) / kWaves;
     auto k = cache->hd == 128 ? (split ? paged_combine_kernel<128, kWaves>
                                        : paged_combine_kernel<128, 1>)

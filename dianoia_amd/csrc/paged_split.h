@@ -31,10 +31,12 @@ struct PagedSplit {
 constexpr int kPagedNarrow = 16, kPagedWide = 64;   // rows of a workgroup
 constexpr int kPagedStep = 64;       // runs are whole steps
 // Runs of the prefix, and of a sequence: up to 32, and more (256 in all) where
-// they hold 256 keys each and the call has few rows (whose partial results are
+// they hold 128 keys each and the call has few rows (whose partial results are
 // then added by four waves each). One token after 131072 keys, 8 heads over
 // one, hd 128, bf16: 45 us with 32 runs, 19 with 128 or 256; f32 147, 46, 34.
-constexpr int kPagedRuns = 32, kPagedMaxRuns = 256, kPagedLong = 256;
+// (At least 256 keys each: 8192 keys of one key head, f32, 14.3 us against 11.4,
+// bf16 9.1 against 8.5, but 32768 keys 11.0 against 11.7.)
+constexpr int kPagedRuns = 32, kPagedMaxRuns = 256, kPagedLong = 128;
 constexpr int64_t kPagedManyRows = 1 << 20;
 
 // Wide blocks read the keys for 64 rows at once and take fewer products, but
@@ -60,9 +62,9 @@ inline PagedPart paged_part(int64_t tokens, int64_t group, int64_t units, int64_
   p.blocks = (rows + block - 1) / block;
   p.keys = kPagedStep;
   if (keys <= 0 || units <= 0 || rows <= 0) return p;
-  // Runs that make about 256 workgroups, of `least` to `most` keys (24 calls,
-  // geometric mean: 11.5 us; with 128 or 512 workgroups, or 128 keys at
-  // least, 11.9 to 12.2).
+  // Runs that make about 256 workgroups, of `least` to `most` keys (49 calls,
+  // geometric mean: 13.7 us; with 192 or 384 workgroups 13.9 and 14.0, with 128
+  // keys at least 14.1).
   const int64_t wgs = units * p.blocks;
   int64_t runs = (256 + wgs - 1) / wgs;
   runs = std::min(std::max(runs, (keys + most - 1) / most), std::max<int64_t>(1, keys / least));
