@@ -420,6 +420,20 @@ def test_keys_past_the_bounds_are_not_seen(gpu_ready):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("prefix", [0, 32, 500])
+def test_keys_past_the_table_are_not_seen(gpu_ready, prefix, kind):
+    """A length, and a bound on it, past the pages that a table lists."""
+    b = Batch(16, [1, 1], [48, 48], prefix, 4, 2, 64, kind, 16)
+    tables = b.tables[:, :3].contiguous()
+    b.batch = D.PagedBatch(b.starts, b.lens_d, tables, 2, 1, 1 << 20,
+                           prefix_pages=b.batch.prefix_pages, prefix_len=prefix)
+    b.ws = D.paged_attention_workspace(b.cache, b.batch, 4)
+    b.ws.fill_(0xff)
+    b.lens_d.copy_(ints([1 << 20, 60]))
+    b.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("heads,kv,hd,page", [(4, 2, 64, 16), (64, 2, 64, 64), (64, 1, 128, 16),
                                               (64, 1, 128, 128)])
 def test_infinities_behind_the_mask(gpu_ready, heads, kv, hd, page, kind):
