@@ -86,7 +86,9 @@ DNX_DEV Seen row_sees(const PagedArgs& a, const Item& w, int r) {
     const int place = w.first + token - w.t0;
     const int hi = w.joined + min(w.count, max(place + 1, 0));
     if (a.window == 0) return {0, hi};
-    if (w.joined == 0) return {place - a.window + 1, hi};
+    // (A place before the first own key, down to minus the new tokens, less the
+    // widest window leaves 32 bits.)
+    if (w.joined == 0) return {max(place, 0) - a.window + 1, hi};
     const int lo = max(a.prefix_len + place, 0) - a.window + 1;
     return {lo < a.prefix_len ? lo : lo - a.prefix_len + w.joined, hi};
   }
@@ -1116,7 +1118,7 @@ constexpr int attention_lds() {
 DNX_DEV bool unseen(const PagedArgs& a, const Item& w, int end) {
   int lo = w.k_lo, hi = w.k_hi;
   if (lo < hi && (a.window > 0 || w.rows > a.group)) {
-    if (a.window > 0) lo = max(lo, w.first + w.row0 / a.group - a.window + 1);
+    if (a.window > 0) lo = max(lo, max(w.first + w.row0 / a.group, 0) - a.window + 1);
     hi = min(hi, w.first + (end - 1) / a.group + 1);
   }
   return lo >= hi;

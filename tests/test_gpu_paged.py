@@ -393,6 +393,32 @@ def test_more_tokens_than_own_keys(gpu_ready, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [0, 5000, 0x7ffffffd, 0x7fffffff])
+@pytest.mark.parametrize("count,own,other,prefix,heads", [
+    (8, 4, 2000, 0, 4), (70, 66, 2000, 0, 4), (6, 2, 1, 500, 4), (6, 0, 900, 500, 2), (100, 3, 300, 500, 6)])
+def test_tokens_before_their_own_keys_in_many_runs(gpu_ready, count, own, other, prefix, heads, window,
+                                                   kind):
+    """More new tokens than own keys in calls that add partial results, under
+    windows whose first key lies 2^31 places before the token: the first tokens
+    see the prefix alone (or nothing), the last ones all up to their own key."""
+    b = Batch(count, [count, 1], [own, other], prefix, heads, 2, 64, kind, 16)
+    assert b.ws.numel() > 4 * heads * 64          # partial results
+    out = host(b.run(window))
+    want, room = b.expected()                     # the rows whose place is a key's
+    rest = count - own
+    assert (np.abs(out[rest:] - want[rest:]) <= room[rest:]).all()
+    if prefix == 0:
+        assert (out[:rest] == 0).all()
+        return
+    for i in range(0, rest, 7):                   # a token at the prefix's last key sees all of it
+        alone = Batch(count, [1], [0], prefix, heads, 2, 64, kind, 16)
+        alone.first_kv = b.first_kv
+        alone.q.copy_(b.q[i:i + 1])
+        want, room = alone.expected()
+        assert (np.abs(out[i] - want[0]) <= room[0]).all(), i
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_pages_outside_the_cache_are_not_seen(gpu_ready, kind):
     b = Batch(4, [1, 3], [100, 90], 64, 8, 4, 128, kind, 16)
     b.tables[0, 2], b.tables[1, 0] = -1, b.keys.shape[0]
