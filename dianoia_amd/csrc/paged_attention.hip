@@ -76,6 +76,16 @@ DNX_DEV int64_t row_at(const PagedArgs& a, const Item& w, int r) {
   return (int64_t)(w.t0 + r / a.group) * a.heads + w.kvh * a.group + r % a.group;
 }
 
+// The first key under the window of a token that stands at `place`: a place
+// before the first key (down to minus the new tokens) sees no less than that
+// key's, and one far behind the last (a length past its bound) nothing. In 64
+// bits: a place less the widest window, and a prefix's length and any other,
+// leave 32. kBehind is behind every key (2^30 of a prefix, 2^30 own).
+constexpr int64_t kBehind = 0x7fff0000;
+DNX_DEV int window_begin(int64_t place, int window) {
+  return (int)min(max(place, (int64_t)0) - window + 1, kBehind);
+}
+
 // The keys of an item that its row r sees: lo .. hi - 1.
 struct Seen {
   int lo, hi;
@@ -86,10 +96,8 @@ DNX_DEV Seen row_sees(const PagedArgs& a, const Item& w, int r) {
     const int place = w.first + token - w.t0;
     const int hi = w.joined + min(w.count, max(place + 1, 0));
     if (a.window == 0) return {0, hi};
-    // (A place before the first own key, down to minus the new tokens, less the
-    // widest window leaves 32 bits.)
-    if (w.joined == 0) return {max(place, 0) - a.window + 1, hi};
-    const int lo = max(a.prefix_len + place, 0) - a.window + 1;
+    if (w.joined == 0) return {window_begin(place, a.window), hi};
+    const int lo = window_begin((int64_t)a.prefix_len + place, a.window);
     return {lo < a.prefix_len ? lo : lo - a.prefix_len + w.joined, hi};
   }
   if (a.window == 0) return {0, w.count};
@@ -98,8 +106,8 @@ DNX_DEV Seen row_sees(const PagedArgs& a, const Item& w, int r) {
     const int mid = (lo + hi) / 2;
     if (a.starts[mid] <= token) lo = mid; else hi = mid;
   }
-  const int place = a.prefix_len + a.lens[lo] - a.starts[lo + 1] + token;
-  return {max(place, 0) - a.window + 1, w.count};
+  const int64_t place = (int64_t)a.prefix_len + a.lens[lo] - a.starts[lo + 1] + token;
+  return {window_begin(place, a.window), w.count};
 }
 
 // 16 keys of an item from kt on (a page holds whole sixteens) as resources
@@ -1118,7 +1126,7 @@ constexpr int attention_lds() {
 DNX_DEV bool unseen(const PagedArgs& a, const Item& w, int end) {
   int lo = w.k_lo, hi = w.k_hi;
   if (lo < hi && (a.window > 0 || w.rows > a.group)) {
-    if (a.window > 0) lo = max(lo, max(w.first + w.row0 / a.group, 0) - a.window + 1);
+    if (a.window > 0) lo = max(lo, window_begin(w.first + w.row0 / a.group, a.window));
     hi = min(hi, w.first + (end - 1) / a.group + 1);
   }
   return lo >= hi;

@@ -419,6 +419,19 @@ def test_tokens_before_their_own_keys_in_many_runs(gpu_ready, count, own, other,
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("prefix", [40, 500])
+@pytest.mark.parametrize("counts", [[1, 1], [1, 5], [70, 2]])
+def test_a_window_far_behind_the_keys(gpu_ready, counts, prefix, kind):
+    """Lengths past the bound, up to the largest: such a token stands behind
+    every key, and under a window sees none of them."""
+    b = Batch(15, counts, [60, 20], prefix, 4, 2, 64, kind, 16)
+    for far in (1 << 20, 0x7fffffff - prefix, 0x7fffffff):
+        b.lens_d.fill_(far)
+        for window in (1, 50, 100000):
+            assert (host(b.run(window)) == 0).all(), (far, window)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_pages_outside_the_cache_are_not_seen(gpu_ready, kind):
     b = Batch(4, [1, 3], [100, 90], 64, 8, 4, 128, kind, 16)
     b.tables[0, 2], b.tables[1, 0] = -1, b.keys.shape[0]
