@@ -42,6 +42,7 @@ struct PagedArgs {
   int window, splits, joined;
   PartArgs prefix, own;
   int64_t prefix_items;
+  int combine_x;   // of the second launch's workgroups, whose y counts the rest
   float scale;
 };
 
@@ -1220,7 +1221,8 @@ __global__ void __launch_bounds__(kThreads) paged_combine_kernel(PagedArgs a) {
   constexpr int ND = HD / 64, U = 8;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t r = (int64_t)blockIdx.x * (kWaves / W) + wave / W;
+  const int64_t r =
+      ((int64_t)blockIdx.y * a.combine_x + blockIdx.x) * (kWaves / W) + wave / W;
   if (r >= (int64_t)a.tokens * a.heads) return;
   const int live = max(0, min(a.starts[a.seqs], a.tokens));
   const int per = (a.splits + W - 1) / W, first = W == 1 ? 0 : wave * per;
@@ -1381,11 +1383,15 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
     const int64_t rows = batch->tokens * heads;
     const bool split = rows < kPagedManyRows && a.splits > (rows < 2048 ? 8 : 16);
     const int64_t blocks = split ? rows : (rows + kWaves - 1) / kWaves;
+    // One dimension holds the workgroups of 2^26 - 4 rows; calls have up to 2^26 - 1.
+    const int64_t x = std::min(blocks, kLaunchThreads / kThreads);
+    a.combine_x = (int)x;
     auto k = cache->hd == 128 ? (split ? paged_combine_kernel<128, kWaves>
                                        : paged_combine_kernel<128, 1>)
                               : (split ? paged_combine_kernel<64, kWaves>
                                        : paged_combine_kernel<64, 1>);
-    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(k, dim3((unsigned)x, (unsigned)((blocks + x - 1) / x)), dim3(kThreads), 0, st,
+                       a);
   }
   return hipGetLastError() == hipSuccess ? DNX_OK : DNX_ELAUNCH;
 }

@@ -544,6 +544,23 @@ def test_offsets_past_32_bits(gpu_ready):
     assert torch.equal(keys[-1, -1], k[0]) and torch.equal(values[-1, -1], k[0])
 
 
+def test_most_rows(gpu_ready):
+    """As many rows as a call may have, nearly all of them padding."""
+    rows, heads, kv = 1082401, 62, 31             # 2^26 - 2 rows of the result
+    b = Batch(14, [3], [40], 500, heads, kv, 64, "bf16", 16)
+    batch = D.PagedBatch(b.starts, b.lens_d, b.tables, rows, 3, 40,
+                         prefix_pages=b.batch.prefix_pages, prefix_len=500)
+    ws = D.paged_attention_workspace(b.cache, batch, heads)
+    assert ws.numel() > 0
+    q, out = (torch.empty(rows, heads, 64, device="cuda") for _ in range(2))
+    q[:3] = b.q
+    out.fill_(3.25)
+    D.paged_attention(b.cache, batch, q, out, ws)
+    want, room = b.expected()
+    assert (np.abs(host(out[:3]) - want) <= room).all()
+    assert not bool((out[3:] != 3.25).any())
+
+
 def test_same_bits_again_on_another_stream(gpu_ready):
     b = Batch(12, [1] * 20, list(range(30, 230, 10)), 1000, 16, 4, 128, "f32", 32)
     first = b.run().clone()
