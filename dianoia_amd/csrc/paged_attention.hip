@@ -42,6 +42,7 @@ struct PagedArgs {
   int window, splits, joined;
   PartArgs prefix, own;
   int64_t prefix_items;
+  uint32_t slots;  // of all sequences' blocks together, or 0
   int combine_x;   // of the second launch's workgroups, whose y counts the rest
   float scale;
 };
@@ -1148,7 +1149,10 @@ DNX_DEV void block_of_16(const PagedArgs& a, const Item& w, int rows, uint8_t* l
 // hd 128, bf16: 93 us, alone 41 and 69; the own ones first 100, with 16384
 // shared and up to 400 own 78 against 105). Workgroups go round the eight XCDs, each with an L2 of its
 // own: the blocks of rows that read the same keys go to one of them.
-template <typename C, int HD>
+// kPacked: the own blocks of all sequences lie in a row (paged_fit). A kernel of
+// its own: the choice in one kernel cost every call 0.1 us (44 calls, geometric
+// mean: 9.11 us against 8.98).
+template <typename C, int HD, bool kPacked>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 paged_attention_kernel(PagedArgs a) {
   __shared__ __align__(16) uint8_t lds[attention_lds<C, HD>()];
@@ -1157,15 +1161,29 @@ paged_attention_kernel(PagedArgs a) {
   w.own = id >= (uint32_t)a.prefix_items;
   if (w.own) id -= (uint32_t)a.prefix_items;
   const PartArgs part = w.own ? a.own : a.prefix;
-  const uint32_t turn = id / 8, unit = turn / (uint32_t)part.blocks * 8 + id % 8;
-  const int block = (int)(turn % (uint32_t)part.blocks);
+  const bool packed = kPacked && w.own;   // its blocks lie among all sequences'
+  uint32_t unit = id, sets = a.slots;
+  int block = 0;
+  if (!packed) {
+    const uint32_t turn = id / 8;
+    unit = turn / (uint32_t)part.blocks * 8 + id % 8;
+    block = (int)(turn % (uint32_t)part.blocks);
+    sets = w.own ? (uint32_t)a.seqs : 1;
+  }
   // The sequences' first runs before their second ones: where the bound on the
   // lengths is far above them, those that have keys start at once.
-  const uint32_t set = unit / (uint32_t)a.kv_heads, sets = w.own ? (uint32_t)a.seqs : 1;
-  const uint32_t b = set % sets;
+  const uint32_t set = unit / (uint32_t)a.kv_heads;
+  uint32_t b = set % sets;
   w.kvh = (int)(unit % (uint32_t)a.kv_heads);
   w.run = (int)(set / sets);
   if (w.run >= part.runs) return;
+  if (packed) {
+    const int rows = part.wide ? kPagedWide : kPagedNarrow, slot = (int)b;
+    const int live = max(0, min(a.starts[a.seqs], a.tokens));
+    b = (uint32_t)paged_sequence(a.starts, a.seqs, live, a.group, rows, slot);
+    block = slot - paged_slot(a.starts, (int)b, live, a.group, rows);
+    if (block < 0) return;   // before the first sequence's rows
+  }
   w.k_lo = w.run * part.keys;
   w.joined = w.own ? a.joined : 0;
   w.table = w.own ? a.tables + b * a.table_stride : a.prefix_pages;
@@ -1317,8 +1335,9 @@ int64_t dnx_paged_attention_workspace_bytes(const dnx_paged_cache* cache,
       heads > 65535 || batch->tokens * heads >= (1 << 26)) {
     return -1;
   }
-  const int64_t splits = split_of(cache, batch, heads).splits();
-  return splits <= 1 ? 0 : batch->tokens * heads * splits * (cache->hd + 2) * 4;
+  const PagedSplit s = split_of(cache, batch, heads);
+  if (s.prefix_items + s.own_items > kPagedItems) return -1;
+  return s.splits() <= 1 ? 0 : batch->tokens * heads * s.splits() * (cache->hd + 2) * 4;
 }
 
 int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* batch,
@@ -1362,21 +1381,21 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
   a.joined = (int)s.joined;
   a.prefix = part_of(s.prefix);
   a.own = part_of(s.own);
-  // Whole rounds of the eight XCDs.
-  auto items = [&](const PagedPart& p, int64_t units) {
-    return (units * p.runs * cache->kv_heads + 7) / 8 * 8 * p.blocks;
-  };
-  a.prefix_items = items(s.prefix, 1);
+  a.slots = (uint32_t)s.slots;
+  a.prefix_items = s.prefix_items;
   a.scale = (float)(1.0 / sqrt((double)cache->hd));
-  const int64_t grid = a.prefix_items + items(s.own, batch->seqs);
-  if (grid > kLaunchThreads / kThreads) return DNX_EINVAL;
+  static_assert(kPagedItems == kLaunchThreads / kThreads, "the launch's limit");
+  const int64_t grid = s.prefix_items + s.own_items;
   const hipStream_t st = (hipStream_t)stream;
   if (grid > 0) {
-    auto k = cache->type == DNX_F32 ? (cache->hd == 128 ? paged_attention_kernel<float, 128>
-                                                        : paged_attention_kernel<float, 64>)
-                                    : (cache->hd == 128 ? paged_attention_kernel<uint16_t, 128>
-                                                        : paged_attention_kernel<uint16_t, 64>);
-    hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(kThreads), 0, st, a);
+    const int kind = (s.slots > 0 ? 4 : 0) + (cache->type == DNX_F32 ? 0 : 2) + (cache->hd == 128);
+    constexpr decltype(&paged_attention_kernel<float, 64, false>) kernels[] = {
+        paged_attention_kernel<float, 64, false>,    paged_attention_kernel<float, 128, false>,
+        paged_attention_kernel<uint16_t, 64, false>, paged_attention_kernel<uint16_t, 128, false>,
+        paged_attention_kernel<float, 64, true>,     paged_attention_kernel<float, 128, true>,
+        paged_attention_kernel<uint16_t, 64, true>,  paged_attention_kernel<uint16_t, 128, true>,
+    };
+    hipLaunchKernelGGL(kernels[kind], dim3((unsigned)grid), dim3(kThreads), 0, st, a);
     if (hipGetLastError() != hipSuccess) return DNX_ELAUNCH;
   }
   if (a.splits != 1) {

@@ -1,5 +1,5 @@
-// How the paged attention deals rows and keys to workgroups. Host code alone,
-// without HIP.
+// How the paged attention deals rows and keys to workgroups. Without HIP: host
+// code, and (constexpr) how a workgroup finds its sequence.
 #pragma once
 
 #include <algorithm>
@@ -22,9 +22,12 @@ struct PagedPart {
 };
 // `joined` (a multiple of kPagedStep): the prefix is walked with each
 // sequence's own keys in one run, in which the own keys begin at that place.
+// `slots`: 0 where each sequence has own.blocks blocks, else the blocks of all
+// sequences together (paged_slot).
 struct PagedSplit {
   PagedPart prefix, own;
-  int64_t joined;
+  int64_t joined, slots;
+  int64_t prefix_items, own_items;   // workgroups of the launch
   int64_t splits() const { return prefix.runs + own.runs; }
 };
 
@@ -38,6 +41,7 @@ constexpr int kPagedStep = 64;       // runs are whole steps
 // bf16 9.1 against 8.5, but 32768 keys 11.0 against 11.7.)
 constexpr int kPagedRuns = 32, kPagedMaxRuns = 256, kPagedLong = 128;
 constexpr int64_t kPagedManyRows = 1 << 20;
+constexpr int64_t kPagedItems = 0xffffffff / 256;   // workgroups that a launch may have
 
 // Wide blocks read the keys for 64 rows at once and take fewer products, but
 // one after another; narrow ones of the same rows run side by side and find
@@ -50,6 +54,18 @@ constexpr int64_t kPagedManyRows = 1 << 20;
 inline bool paged_wide(int64_t rows, int64_t units, int64_t keys, bool f32) {
   if (rows <= 32) return false;
   return rows > 128 || rows * keys * units > (f32 ? 1200000 : 4000000);
+}
+
+// At most that many runs of whole steps.
+inline void paged_deal(PagedPart& p, int64_t keys, int64_t runs) {
+  p.keys = ((keys + runs - 1) / runs + kPagedStep - 1) / kPagedStep * kPagedStep;
+  p.runs = (keys + p.keys - 1) / p.keys;
+}
+
+// The workgroups of a part: for each unit (a key head, of a sequence) its runs
+// and blocks, in whole rounds of the eight XCDs.
+inline int64_t paged_items(const PagedPart& p, int64_t units) {
+  return (units * p.runs + 7) / 8 * 8 * p.blocks;
 }
 
 inline PagedPart paged_part(int64_t tokens, int64_t group, int64_t units, int64_t keys, bool f32,
@@ -70,9 +86,61 @@ inline PagedPart paged_part(int64_t tokens, int64_t group, int64_t units, int64_
   runs = std::min(std::max(runs, (keys + most - 1) / most), std::max<int64_t>(1, keys / least));
   runs = std::min(runs, std::max<int64_t>(kPagedRuns, keys / kPagedLong));
   runs = std::min<int64_t>(std::max<int64_t>(runs, 1), max_runs);
-  p.keys = ((keys + runs - 1) / runs + kPagedStep - 1) / kPagedStep * kPagedStep;
-  p.runs = (keys + p.keys - 1) / p.keys;
+  paged_deal(p, keys, runs);
   return p;
+}
+
+// The blocks of all sequences in a row: sequence b's begin at this place. It
+// has floor((s + n) / block) - floor(s / block) + 1 places for its n rows from
+// s on, at least ceil(n / block), and all sequences together have
+// floor(tokens * group / block) + seqs, however the tokens lie.
+constexpr int paged_slot(const int32_t* starts, int b, int live, int group, int block) {
+  const int64_t s = starts[b] < 0 ? 0 : starts[b] > live ? live : starts[b];
+  return (int)(s * group / block) + b;
+}
+
+// The sequence whose blocks hold place `slot`: the last that begins at or
+// before it.
+constexpr int paged_sequence(const int32_t* starts, int seqs, int live, int group, int block,
+                             int slot) {
+  int lo = 0, hi = seqs;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (paged_slot(starts, mid, live, group, block) <= slot) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// Bounds may lie far above what a batch holds (each of many sequences might
+// have max_tokens new ones, and max_len keys). Where the blocks and runs that
+// they ask for are more workgroups than a launch may have, the blocks of all
+// sequences are bounded by `tokens` together (64 sequences of up to 8192 tokens,
+// 8192 in all, 4 query heads a key head: 576 blocks in place of 32768), and then
+// runs become longer. The other calls keep a place for every block of every
+// sequence, which needs no search. What still does not fit has more than 2^22
+// key heads of sequences.
+inline void paged_fit(PagedSplit& s, int64_t seqs, int64_t tokens, int64_t group,
+                      int64_t kv_heads, int64_t prefix_len, int64_t max_len) {
+  const int64_t units = seqs * kv_heads;
+  s.prefix_items = paged_items(s.prefix, kv_heads);
+  s.own_items = paged_items(s.own, units);
+  if (s.prefix_items + s.own_items <= kPagedItems) return;
+  const auto longer = [](PagedPart& p, int64_t keys, int64_t runs) {
+    if (p.runs > std::max<int64_t>(runs, 1)) paged_deal(p, keys, std::max<int64_t>(runs, 1));
+  };
+  longer(s.prefix, prefix_len, kPagedItems / 2 / s.prefix.blocks / 8 * 8 / kv_heads);
+  s.prefix_items = paged_items(s.prefix, kv_heads);
+  const int64_t left = kPagedItems - s.prefix_items;
+  if (s.own_items <= left) return;
+  const int64_t slots = tokens * group / (s.own.wide ? kPagedWide : kPagedNarrow) + seqs;
+  if (slots * kv_heads < (units + 7) / 8 * 8 * s.own.blocks) {
+    s.slots = slots;
+    longer(s.own, max_len, left / (slots * kv_heads));
+    s.own_items = slots * kv_heads * s.own.runs;
+  } else {
+    longer(s.own, max_len, left / s.own.blocks / 8 * 8 / units);
+    s.own_items = paged_items(s.own, units);
+  }
 }
 
 inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, int64_t group,
@@ -83,7 +151,8 @@ inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, 
   const int64_t max_runs = tokens * group * kv_heads >= kPagedManyRows ? kPagedRuns
                            : prefix_len > 0 ? kPagedMaxRuns / 2 : kPagedMaxRuns;
   PagedSplit s{paged_part(tokens, group, kv_heads, prefix_len, f32, kPagedStep, 1 << 20, max_runs),
-               paged_part(max_tokens, group, seqs * kv_heads, max_len, f32, least, 2048, max_runs), 0};
+               paged_part(max_tokens, group, seqs * kv_heads, max_len, f32, least, 2048, max_runs),
+               0, 0, 0, 0};
   // A short prefix is joined to them where a CU for each workgroup is left: its
   // keys are then read once for each block of rows, but without the second
   // launch. Up to 384 keys, or 256 where the float32 matrix cores take 16 rows
@@ -99,6 +168,7 @@ inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, 
     s.own.keys = keys;
     s.prefix.runs = 0;
   }
+  paged_fit(s, seqs, tokens, group, kv_heads, prefix_len, max_len);
   return s;
 }
 

@@ -611,6 +611,9 @@ typedef struct {
 // last bits of rows that share a step with it. float32 accuracy throughout.
 // workspace: dnx_paged_attention_workspace_bytes of device memory (the partial
 // results of runs of keys), 16-byte aligned; calls that overlap need one each.
+// Batches of up to 2^22 key heads (seqs * kv_heads) are served whatever their
+// bounds; beyond that, those whose workgroups are more than a launch may have are
+// refused, by the workspace's size (-1) and by the call.
 // The two structs are read at the call.
 int64_t dnx_paged_attention_workspace_bytes(const dnx_paged_cache* cache,
                                             const dnx_paged_batch* batch, int64_t heads);

@@ -432,6 +432,40 @@ def test_a_window_far_behind_the_keys(gpu_ready, counts, prefix, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv,seqs,tokens,most,page,width,prefix", [
+    (8, 8, 4096, 4200, 4200, 64, 290, 0), (8, 8, 4096, 4200, 4200, 64, 290, 300),
+    (16, 16, 65536, 2000, 20, 256, 71, 0), (4, 1, 50000, 4200, 4200, 256, 70, 40)])
+def test_bounds_far_above_the_batch(gpu_ready, heads, kv, seqs, tokens, most, page, width, prefix, kind):
+    """Many sequences that might each have many tokens and a long cache, of
+    which a few have any: the bounds' product is more workgroups than a launch
+    may have."""
+    counts, lens = [19, 1, 7, 2, 20], [40, 600, 7, 1, 333]
+    if most > 100:
+        counts[0], lens[0] = 150, 180
+    b = Batch(17, counts, lens, prefix, heads, kv, 64, kind, page, pad=5, gate=True)
+    rng = np.random.default_rng(seqs)
+    at = np.sort(rng.permutation(np.arange(1, seqs - 1))[:3])
+    at = np.concatenate([[0], at, [seqs - 1]])    # the first and the last among them
+    n, own = np.zeros(seqs, np.int64), np.zeros(seqs, np.int64)
+    n[at], own[at] = counts, lens
+    tables = np.full((seqs, width), -7, np.int32)
+    tables[at, :b.tables_h.shape[1]] = b.tables_h
+    rows = b.live + 5
+    q = torch.full((tokens, heads, 64), float("nan"), device="cuda")
+    q[:rows], gate = b.q, torch.zeros(tokens, heads, device="cuda")
+    gate[:rows] = b.gate
+    b.q, b.gate = q, gate
+    b.out = torch.full((tokens, heads, 64), 3.25, device="cuda")
+    b.batch = D.PagedBatch(ints(np.concatenate([[0], np.cumsum(n)])), ints(own), ints(tables), tokens,
+                           most, width * page, prefix_pages=b.batch.prefix_pages if prefix else None,
+                           prefix_len=prefix)
+    b.ws = D.paged_attention_workspace(b.cache, b.batch, heads)
+    b.ws.fill_(0xff)
+    b.check()
+    b.check(100)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_pages_outside_the_cache_are_not_seen(gpu_ready, kind):
     b = Batch(4, [1, 3], [100, 90], 64, 8, 4, 128, kind, 16)
     b.tables[0, 2], b.tables[1, 0] = -1, b.keys.shape[0]

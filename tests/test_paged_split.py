@@ -166,3 +166,109 @@ def test_python_refusals():
                  (i(4), i(3), i(3, 2), 3, 0, 5), (i(4), i(3), i(3, 2), 3, 1, 5)):
         with pytest.raises(ValueError):   # the last: not in HBM
             D.PagedBatch(*args)
+
+
+FIT = """
+#include "paged_split.h"
+extern "C" void fit_of(int64_t seqs, int64_t tokens, int64_t max_tokens, int64_t group,
+                       int64_t kv_heads, int64_t prefix, int64_t len, int64_t f32, int64_t* out) {
+  const dnx::PagedSplit s =
+      dnx::paged_split(seqs, tokens, max_tokens, group, kv_heads, prefix, len, f32 != 0);
+  const int64_t v[] = {s.prefix_items, s.own_items, s.slots, s.prefix.runs, s.prefix.keys, s.own.runs,
+                       s.own.keys, s.splits(), s.own.wide, s.own.blocks};
+  for (int i = 0; i < 10; i++) out[i] = v[i];
+}
+extern "C" int place_of(const int32_t* starts, int b, int live, int group, int block) {
+  return dnx::paged_slot(starts, b, live, group, block);
+}
+extern "C" int sequence_of(const int32_t* starts, int seqs, int live, int group, int block, int slot) {
+  return dnx::paged_sequence(starts, seqs, live, group, block, slot);
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def fit(tmp_path_factory):
+    d = tmp_path_factory.mktemp("fit")
+    (d / "f.cpp").write_text(FIT)
+    so = str(d / "f.so")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-o", so, str(d / "f.cpp"),
+                    "-I", os.path.join(ROOT, "dianoia_amd", "csrc")], check=True)
+    lib = ctypes.CDLL(so)
+    lib.fit_of.argtypes, lib.fit_of.restype = [ctypes.c_int64] * 8 + [ctypes.c_void_p], None
+    lib.place_of.argtypes = [ctypes.c_void_p] + [ctypes.c_int] * 4
+    lib.sequence_of.argtypes = [ctypes.c_void_p] + [ctypes.c_int] * 5
+    return lib
+
+
+def test_every_call_fits_a_launch(fit):
+    """Whatever the bounds, up to 2^22 key heads of sequences and 2^26 rows: no
+    more workgroups than a launch may have, every key in one run, at most 256
+    runs, and where a launch holds a place for every block, that place."""
+    limit = 0xffffffff // 256
+    out = (ctypes.c_int64 * 10)()
+    for seqs, kv, group, tokens, most, prefix, length, f32 in itertools.product(
+            (1, 64, 4096, 1 << 20), (1, 8, 31, 1024), (1, 4, 64), (1, 2000, 16384, 1 << 22),
+            (1, 20, 8192, 1 << 22), (0, 300, 1 << 25, 1 << 30), (0, 200, 131072, 1 << 30), (0, 1)):
+        if tokens * kv * group >= 1 << 26 or seqs * kv > 1 << 22 or prefix + length >= 1 << 31:
+            continue
+        args = seqs, tokens, min(most, tokens), group, kv, prefix, length, f32
+        fit.fit_of(*args, out)
+        prefix_items, own_items, slots, pr, pk, orun, ok, total, wide, blocks = out
+        assert 0 <= prefix_items + own_items <= limit, args
+        assert total == pr + orun <= 256
+        if pr:
+            assert pk % 64 == 0 and (pr - 1) * pk < prefix <= pr * pk < 1 << 31, args
+        if orun:
+            begin = -(-prefix // 64) * 64 if prefix and not pr else 0
+            assert ok % 64 == 0 and (orun - 1) * ok < begin + length <= orun * ok < 1 << 31, args
+            if slots:
+                assert slots >= tokens * group // (64 if wide else 16) + seqs
+                assert own_items == slots * kv * orun
+            else:
+                assert own_items == -(-seqs * kv * orun // 8) * 8 * blocks
+
+
+@pytest.mark.parametrize("group,block", [(1, 16), (3, 16), (4, 64), (7, 64), (64, 16)])
+def test_every_block_has_a_place(fit, group, block):
+    """Blocks of all sequences in a row: each finds its sequence, whatever the
+    tokens of each are, and no place lies outside."""
+    import random
+    rng = random.Random(group * block)
+    for seqs in (1, 2, 5, 100):
+        for most in (0, 1, 17, 300):
+            counts = [rng.choice([0, 0, 1, rng.randint(0, most)]) if most else 0 for _ in range(seqs)]
+            starts = [0]
+            for c in counts:
+                starts.append(starts[-1] + c)
+            live = starts[-1]
+            a = (ctypes.c_int32 * len(starts))(*starts)
+            places = live * group // block + seqs
+            found = set()
+            for slot in range(places):
+                b = fit.sequence_of(a, seqs, live, group, block, slot)
+                at = slot - fit.place_of(a, b, live, group, block)
+                assert 0 <= b < seqs and at >= 0
+                if at * block < counts[b] * group:
+                    assert (b, at) not in found
+                    found.add((b, at))
+            assert found == {(b, i) for b, c in enumerate(counts)
+                             for i in range(-(-c * group // block))}
+
+
+def test_bounds_beyond_a_launch_are_refused_by_both():
+    """More key heads of sequences than a launch has workgroups: no size is given
+    for what the call would refuse."""
+    from dianoia_amd import _lib
+    lib = _lib.load()
+    a = 4096
+    c = _lib.PagedCacheStruct(keys=a, values=a, pages=64, page=16, kv_heads=32, hd=64, type=0)
+    for seqs, ok in ((1 << 17, True), (1 << 20, False)):
+        b = _lib.PagedBatchStruct(starts=a, lens=a, tables=a, prefix_pages=a, table_stride=4,
+                                  prefix_len=1000, seqs=seqs, tokens=8, max_tokens=8, max_len=64)
+        size = lib.dnx_paged_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(b), 32)
+        assert (size > 0) == ok
+        if not ok:
+            assert size == -1
+            assert lib.dnx_paged_attention(ctypes.byref(c), ctypes.byref(b), a, None, a, 32, 0, a,
+                                           1 << 40, None) == -1
