@@ -111,19 +111,28 @@ constexpr int paged_sequence(const int32_t* starts, int seqs, int live, int grou
   return lo;
 }
 
-// Bounds may lie far above what a batch holds (each of many sequences might
-// have max_tokens new ones, and max_len keys). Where the blocks and runs that
-// they ask for are more workgroups than a launch may have, the blocks of all
-// sequences are bounded by `tokens` together (64 sequences of up to 8192 tokens,
-// 8192 in all, 4 query heads a key head: 576 blocks in place of 32768), and then
-// runs become longer. The other calls keep a place for every block of every
-// sequence, which needs no search. What still does not fit has more than 2^22
-// key heads of sequences.
+// Bounds may lie far above what a batch holds: each of many sequences might
+// have max_tokens new ones, of which there are `tokens` in all. Where a place for
+// every block of every sequence, in rounds of the XCDs, makes kPagedEmpty more
+// workgroups than all sequences' blocks in a row, they lie in a row: to find its
+// sequence takes a workgroup up to 0.7 us, but full workgroups wait behind empty
+// ones (us, a place for every block against a row; bf16, 32 / 8 heads, hd 128:
+// 24 sequences of up to 48 tokens, one each, 250 keys, 360 more, 13.5 / 14.1;
+// 24 of up to 16, 240 keys, 528 more, 16.8 / 9.4; 64 of up to 512, one of 512
+// among them, 1000 keys, 15592 more, 132 / 60; one prompt of 2048 tokens on
+// 8 heads over one, whose blocks a place each puts on one XCD, 213 / 69).
+// Runs become longer where a launch may not have as many workgroups. What still
+// does not fit has more than 2^22 key heads of sequences.
+constexpr int64_t kPagedEmpty = 512;
+
 inline void paged_fit(PagedSplit& s, int64_t seqs, int64_t tokens, int64_t group,
                       int64_t kv_heads, int64_t prefix_len, int64_t max_len) {
   const int64_t units = seqs * kv_heads;
+  const int64_t row = kv_heads * (tokens * group / (s.own.wide ? kPagedWide : kPagedNarrow) + seqs);
+  const auto own_items = [&] { return s.slots > 0 ? row * s.own.runs : paged_items(s.own, units); };
+  if (paged_items(s.own, units) - row * s.own.runs >= kPagedEmpty) s.slots = row / kv_heads;
   s.prefix_items = paged_items(s.prefix, kv_heads);
-  s.own_items = paged_items(s.own, units);
+  s.own_items = own_items();
   if (s.prefix_items + s.own_items <= kPagedItems) return;
   const auto longer = [](PagedPart& p, int64_t keys, int64_t runs) {
     if (p.runs > std::max<int64_t>(runs, 1)) paged_deal(p, keys, std::max<int64_t>(runs, 1));
@@ -131,15 +140,10 @@ inline void paged_fit(PagedSplit& s, int64_t seqs, int64_t tokens, int64_t group
   longer(s.prefix, prefix_len, kPagedItems / 2 / s.prefix.blocks / 8 * 8 / kv_heads);
   s.prefix_items = paged_items(s.prefix, kv_heads);
   const int64_t left = kPagedItems - s.prefix_items;
-  if (s.own_items <= left) return;
-  const int64_t slots = tokens * group / (s.own.wide ? kPagedWide : kPagedNarrow) + seqs;
-  if (slots * kv_heads < (units + 7) / 8 * 8 * s.own.blocks) {
-    s.slots = slots;
-    longer(s.own, max_len, left / (slots * kv_heads));
-    s.own_items = slots * kv_heads * s.own.runs;
-  } else {
-    longer(s.own, max_len, left / s.own.blocks / 8 * 8 / units);
-    s.own_items = paged_items(s.own, units);
+  if (s.own_items > left) {
+    if (row < (units + 7) / 8 * 8 * s.own.blocks) s.slots = row / kv_heads;
+    longer(s.own, max_len, s.slots > 0 ? left / row : left / s.own.blocks / 8 * 8 / units);
+    s.own_items = own_items();
   }
 }
 

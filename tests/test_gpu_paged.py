@@ -466,6 +466,21 @@ def test_bounds_far_above_the_batch(gpu_ready, heads, kv, seqs, tokens, most, pa
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [0, 90])
+def test_a_prompt_among_single_tokens(gpu_ready, window, kind):
+    """One long prompt beside decoding sequences, and others without a token or
+    of a few: most sequences have few of the blocks that the longest has. And
+    prompts alone, on few key heads."""
+    counts = [1] * 40 + [210] + [1, 0, 3, 17] * 8
+    lens = [max(c, 5 * i + 1) for i, c in enumerate(counts)]
+    Batch(31, counts, lens, 0, 8, 4, 64, kind, 16, pad=2, gate=True).check(window)
+    Batch(32, counts, lens, 300, 4, 4, 64, kind, 32, pad=70).check(window)
+    short = [min(c, 17) for c in counts]
+    Batch(33, short, lens, 0, 64, 32, 64, kind, 64).check(window)
+    Batch(34, [900, 300], [900, 400], 0, 6, 1, 64, kind, 64, pad=1).check(window)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_pages_outside_the_cache_are_not_seen(gpu_ready, kind):
     b = Batch(4, [1, 3], [100, 90], 64, 8, 4, 128, kind, 16)
     b.tables[0, 2], b.tables[1, 0] = -1, b.keys.shape[0]

@@ -272,3 +272,18 @@ def test_bounds_beyond_a_launch_are_refused_by_both():
             assert size == -1
             assert lib.dnx_paged_attention(ctypes.byref(c), ctypes.byref(b), a, None, a, 32, 0, a,
                                            1 << 40, None) == -1
+
+
+def test_blocks_in_a_row_where_many_would_be_empty(fit):
+    """A step of single tokens and a batch of equal prompts have a place for every
+    block; one prompt among single tokens, and bounds above the batch, do not."""
+    out = (ctypes.c_int64 * 10)()
+
+    def slots(seqs, tokens, most, length=1000, kv=8, group=4):
+        fit.fit_of(seqs, tokens, most, group, kv, 0, length, 0, out)
+        return out[2]
+
+    assert slots(64, 64, 1) == 0 and slots(1, 1, 1) == 0 and slots(16, 16 * 512, 512) == 0
+    assert slots(64, 575, 512) == 575 * 4 // 64 + 64
+    assert slots(64, 64, 64) == 64 * 4 // 64 + 64
+    assert slots(2, 40, 39) == 0 and slots(64, 64, 64, length=0) == 0
