@@ -808,7 +808,8 @@ def paged_append(cache: PagedCache, k, v, positions, slots, rope=None, q=None, q
     ks, k1, k2 = k.stride()
     vs, v1, v2 = v.stride()
     if (kv_heads != cache.kv_heads or hd != cache.hd or v.shape != shape or k.dtype is not _F32
-            or v.dtype is not _F32 or k2 != 1 or k1 != hd or v2 != 1 or v1 != hd):
+            or v.dtype is not _F32 or k2 != 1 or v2 != 1
+            or (kv_heads != 1 and (k1 != hd or v1 != hd))):   # a lone head's stride is anything
         raise ValueError("paged_append: k and v are float32 [n][kv_heads][hd] with dense heads")
     if k.get_device() != d or v.get_device() != d:
         raise ValueError("paged_append: k and v are not on the cache's device")
@@ -817,8 +818,8 @@ def paged_append(cache: PagedCache, k, v, positions, slots, rope=None, q=None, q
     if q is not None:
         tokens, heads, dims = q.shape
         qs, q1, q2 = q.stride()
-        if (tokens != n or dims != hd or q.dtype is not _F32 or q2 != 1 or q1 != hd
-                or q.get_device() != d):
+        if (tokens != n or dims != hd or q.dtype is not _F32 or q2 != 1
+                or (heads != 1 and q1 != hd) or q.get_device() != d):
             raise ValueError("paged_append: q is float32 [n][heads][hd] with dense heads")
         if q_out is None:
             raise ValueError("paged_append: q needs a float32 q_out [n][heads][hd]")

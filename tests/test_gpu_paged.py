@@ -130,6 +130,23 @@ def test_append_q_in_place(gpu_ready):
     assert torch.equal(q, out)
 
 
+def test_append_single_heads_of_any_stride(gpu_ready):
+    """A dimension of one has no stride: a tensor [1][n][hd] turned to [n][1][hd]."""
+    n, hd = 7, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = (torch.randn(1, n, hd, device="cuda", generator=g) for _ in range(3))
+    rope = torch.from_numpy(rope_table(64, hd)).cuda()
+    got = []
+    for turn in (lambda t: t.transpose(0, 1), lambda t: t.view(n, 1, hd)):
+        keys, values = (torch.zeros(1, 16, 1, hd, device="cuda") for _ in range(2))
+        q_out = torch.zeros(n, 1, hd, device="cuda")
+        D.paged_append(D.PagedCache(keys, values), turn(k), turn(v), ints(range(n)), ints(range(n)),
+                       rope=rope, q=turn(q), q_out=q_out)
+        got.append((keys, values, q_out))
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and bool(a.any())
+
+
 # --------------------------------------------------------------- the attention
 
 class Batch:
