@@ -626,6 +626,9 @@ def matmul_q4(qs, scales, x, y, rows: int, cols: int, n: int, int8_inputs: bool,
 # Python: sizes are compared in place, and an operand is named only once one
 # is too small.
 
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _device_of(t: torch.Tensor) -> int:
     """The current device, which has to be the tensor's."""
     d = t.get_device()
@@ -659,70 +662,96 @@ def _refuse(*tensors) -> None:
     raise ValueError("device launchers take tensors of one CUDA (HIP) device")
 
 
-def _quantize_i8r(name: str, size: int, x, qs, scales, rows, cols, cols_pad, stream) -> None:
+_F32, _I8, _I32 = torch.float32, torch.int8, torch.int32
+_BF16 = (torch.bfloat16, torch.uint16, torch.int16)    # values, or their bits
+
+
+def _types(name: str, **operands) -> None:
+    """Names the operand that is not of its type, which a caller has seen."""
+    for what, (t, kinds) in operands.items():
+        kinds = kinds if isinstance(kinds, tuple) else (kinds,)
+        if t is not None and t.dtype not in kinds:
+            raise ValueError(f"{name}: {what} is {t.dtype}, not {' or '.join(map(str, kinds))}")
+
+
+def _quantize_i8r(name: str, size: int, kinds, x, qs, scales, rows, cols, cols_pad, stream) -> None:
+    if x.dtype not in kinds or qs.dtype is not _I8 or scales.dtype is not _F32:
+        _types(name, x=(x, kinds), qs=(qs, _I8), scales=(scales, _F32))
     if x.nbytes < rows * cols * size or qs.nbytes < rows * cols_pad or scales.nbytes < rows * 4:
         _need(name, x=(x, rows * cols * size), qs=(qs, rows * cols_pad), scales=(scales, rows * 4))
-    d = torch._C._cuda_getDevice() if x.is_cuda else -2
-    if (x.get_device() != d or qs.get_device() != d or scales.get_device() != d
+    d = x.get_device()
+    if (d < 0 or d != _current_device() or qs.get_device() != d or scales.get_device() != d
             or not (x.is_contiguous() and qs.is_contiguous() and scales.is_contiguous())):
         _refuse(x, qs, scales)
-    rc = getattr(_lib.load(), name)(x.data_ptr(), qs.data_ptr(), scales.data_ptr(), rows, cols,
-                                    cols_pad, _on(d, stream))
+    rc = getattr(_lib._lib or _lib.load(), name)(
+        x.data_ptr(), qs.data_ptr(), scales.data_ptr(), rows, cols, cols_pad,
+        _raw_stream(d) if stream is None else stream.cuda_stream)
     if rc:
         _check(rc, name)
 
 
 def quantize_i8r(x, qs, scales, rows: int, cols: int, cols_pad: int, stream=None) -> None:
     """fp32 rows -> int8 [rows][cols_pad] with one scale a row (value = code * scale)."""
-    _quantize_i8r("dnx_quantize_i8r", 4, x, qs, scales, rows, cols, cols_pad, stream)
+    _quantize_i8r("dnx_quantize_i8r", 4, (_F32,), x, qs, scales, rows, cols, cols_pad, stream)
 
 
 def quantize_i8r_bf16(x, qs, scales, rows: int, cols: int, cols_pad: int, stream=None) -> None:
-    """bf16 rows (weights as they lie in a file) -> int8 with one scale a row."""
-    _quantize_i8r("dnx_quantize_i8r_bf16", 2, x, qs, scales, rows, cols, cols_pad, stream)
+    """bf16 rows (weights as they lie in a file: bfloat16, or its bits as 16-bit
+    integers) -> int8 with one scale a row."""
+    _quantize_i8r("dnx_quantize_i8r_bf16", 2, _BF16, x, qs, scales, rows, cols, cols_pad, stream)
 
 
 def rms_norm_i8r(x, w, qs, scales, rows: int, cols: int, cols_pad: int, eps: float, m=None,
                  x_out=None, stream=None) -> None:
     """RMSNorm(s) * w as int8 with one scale a row; s = x, or x + m, which goes
     to x_out (x itself, m or another tensor)."""
+    if (x.dtype is not _F32 or w.dtype is not _F32 or qs.dtype is not _I8
+            or scales.dtype is not _F32 or (m is not None and m.dtype is not _F32)
+            or (x_out is not None and x_out.dtype is not _F32)):
+        _types("rms_norm_i8r", x=(x, _F32), w=(w, _F32), qs=(qs, _I8), scales=(scales, _F32),
+               m=(m, _F32), x_out=(x_out, _F32))
     size = rows * cols * 4
     if (x.nbytes < size or w.nbytes < cols * 4 or qs.nbytes < rows * cols_pad
             or scales.nbytes < rows * 4 or (m is not None and m.nbytes < size)
             or (x_out is not None and x_out.nbytes < size)):
         _need("rms_norm_i8r", x=(x, size), w=(w, cols * 4), qs=(qs, rows * cols_pad),
               scales=(scales, rows * 4), m=(m, size), x_out=(x_out, size))
-    d = torch._C._cuda_getDevice() if x.is_cuda else -2
-    if (x.get_device() != d or w.get_device() != d or qs.get_device() != d
+    d = x.get_device()
+    if (d < 0 or d != _current_device() or w.get_device() != d or qs.get_device() != d
             or scales.get_device() != d or not (x.is_contiguous() and w.is_contiguous()
                                                 and qs.is_contiguous() and scales.is_contiguous())):
         _refuse(x, w, qs, scales)
-    rc = _lib.load().dnx_rms_norm_i8r(
+    rc = (_lib._lib or _lib.load()).dnx_rms_norm_i8r(
         x.data_ptr(), None if m is None else _at(m, d), None if x_out is None else _at(x_out, d),
-        w.data_ptr(), qs.data_ptr(), scales.data_ptr(), rows, cols, cols_pad, eps, _on(d, stream))
+        w.data_ptr(), qs.data_ptr(), scales.data_ptr(), rows, cols, cols_pad, eps,
+        _raw_stream(d) if stream is None else stream.cuda_stream)
     if rc:
         _check(rc, "dnx_rms_norm_i8r")
 
 
 def gemm_i8r(w, w_scale, x, x_scale, y, rows: int, cols: int, n: int, stream=None) -> None:
     """y [n][rows] = the int8 rows x times the int8 rows w, each with its scale."""
+    if (w.dtype is not _I8 or x.dtype is not _I8 or w_scale.dtype is not _F32
+            or x_scale.dtype is not _F32 or y.dtype is not _F32):
+        _types("gemm_i8r", w=(w, _I8), w_scale=(w_scale, _F32), x=(x, _I8), x_scale=(x_scale, _F32),
+               y=(y, _F32))
     if (w.nbytes < rows * cols or w_scale.nbytes < rows * 4 or x.nbytes < n * cols
             or x_scale.nbytes < n * 4 or y.nbytes < n * rows * 4):
         _need("gemm_i8r", w=(w, rows * cols), w_scale=(w_scale, rows * 4), x=(x, n * cols),
               x_scale=(x_scale, n * 4), y=(y, n * rows * 4))
-    d = torch._C._cuda_getDevice() if w.is_cuda else -2
-    if (w.get_device() != d or w_scale.get_device() != d or x.get_device() != d
+    d = w.get_device()
+    if (d < 0 or d != _current_device() or w_scale.get_device() != d or x.get_device() != d
             or x_scale.get_device() != d or y.get_device() != d
             or not (w.is_contiguous() and w_scale.is_contiguous() and x.is_contiguous()
                     and x_scale.is_contiguous() and y.is_contiguous())):
         _refuse(w, w_scale, x, x_scale, y)
-    rc = _lib.load().dnx_gemm_i8r(w.data_ptr(), w_scale.data_ptr(), x.data_ptr(), x_scale.data_ptr(),
-                                  y.data_ptr(), rows, cols, n, _on(d, stream))
+    rc = (_lib._lib or _lib.load()).dnx_gemm_i8r(
+        w.data_ptr(), w_scale.data_ptr(), x.data_ptr(), x_scale.data_ptr(), y.data_ptr(), rows, cols,
+        n, _raw_stream(d) if stream is None else stream.cuda_stream)
     if rc:
         _check(rc, "dnx_gemm_i8r")
 
 
-_F32, _I32 = torch.float32, torch.int32
 _CACHE_TYPES = {torch.float32: 0, torch.bfloat16: 1}   # DNX_F32, DNX_BF16
 
 

@@ -346,3 +346,30 @@ def test_refusals():
         D.gemm_i8r(t, t, t, t, t, 8, 64, 2)
     with pytest.raises(ValueError):   # not in HBM
         D.quantize_i8r(t, t, t, 1, 64, 64)
+
+
+def test_types_are_refused():
+    """A tensor large enough, but of another type than the kernel reads or
+    writes: refused before anything is launched, by its name."""
+    h, d = torch.zeros(64, 64).half(), torch.zeros(64, 64).double()
+    b, q, u = h.bfloat16(), torch.zeros(64, 64, dtype=torch.int8), torch.zeros(64, 64, dtype=torch.uint8)
+    s, s64 = torch.zeros(64), torch.zeros(64).double()
+    for f in (D.quantize_i8r, D.quantize_i8r_bf16):
+        x = torch.zeros(64, 64, dtype=torch.float32 if f is D.quantize_i8r else torch.bfloat16)
+        for args, what in (((h if f is D.quantize_i8r_bf16 else d, q, s), "x is"), ((x, u, s), "qs is"),
+                           ((x, q, s64), "scales is"), ((d, q, s), "x is")):
+            with pytest.raises(ValueError, match=what):
+                f(*args, 64, 64, 64)
+        with pytest.raises(ValueError, match="CUDA"):      # of its types, but not in HBM
+            f(x, q, s, 64, 64, 64)
+    with pytest.raises(ValueError, match="CUDA"):          # bf16 bits
+        D.quantize_i8r_bf16(b.view(torch.int16), q, s, 64, 64, 64)
+    x = torch.zeros(64, 64)
+    norm = dict(x=x, w=s, qs=q, scales=s, m=x, x_out=x)
+    for name, bad in (("x", d), ("w", s64), ("qs", u), ("scales", s64), ("m", d), ("x_out", d)):
+        with pytest.raises(ValueError, match=f"{name} is"):
+            D.rms_norm_i8r(**{**norm, name: bad}, rows=64, cols=64, cols_pad=64, eps=EPS)
+    product = dict(w=q, w_scale=s, x=q, x_scale=s, y=x)
+    for name, bad in (("w", u), ("w_scale", s64), ("x", x), ("x_scale", s64), ("y", d)):
+        with pytest.raises(ValueError, match=f"{name} is"):
+            D.gemm_i8r(**{**product, name: bad}, rows=64, cols=64, n=64)
