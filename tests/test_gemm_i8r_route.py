@@ -48,3 +48,28 @@ def test_every_size_has_one(route):
         for rows in (1, 33, 5000, 1 << 30):
             for cols in (32, 1120, 131040):
                 assert 0 <= route(n, rows, cols) < 7
+
+
+FEW = """
+#include "gemm_i8r_route.h"
+extern "C" int few(int64_t n, int64_t rows) { return dnx::i8r_few_tiles(n, rows); }
+"""
+
+
+def test_few_tokens_tiles_of_a_workgroup(tmp_path):
+    """Two tiles of rows a workgroup from five tokens on, where they leave no CU
+    more rows than one would, or where there are very many rows."""
+    (tmp_path / "f.cpp").write_text(FEW)
+    so = str(tmp_path / "f.so")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-o", so, str(tmp_path / "f.cpp"),
+                    "-I", os.path.join(ROOT, "dianoia_amd", "csrc")], check=True)
+    few = ctypes.CDLL(so).few
+    few.argtypes, few.restype = [ctypes.c_int64] * 2, ctypes.c_int
+    for n in (1, 4):
+        assert all(few(n, rows) == 1 for rows in (1, 6144, 8192, 32769, 1 << 21))
+    for n in (5, 16):
+        # 256 CUs: one round of 16 or 32 rows a workgroup up to 4096 and 8192 rows.
+        for rows, tiles in ((1, 1), (4096, 1), (4097, 2), (6144, 2), (8192, 2), (8193, 1), (12288, 1),
+                            (12289, 2), (16384, 2), (20480, 1), (32768, 2), (32769, 2), (36864, 2),
+                            (128256, 2)):
+            assert few(n, rows) == tiles, (n, rows)

@@ -498,6 +498,19 @@ def test_a_prompt_among_single_tokens(gpu_ready, window, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("prefix", [0, 32, 500])
+def test_lengths_past_the_bound(gpu_ready, prefix, kind):
+    """lens far past max_len: the keys up to max_len count, those in listed
+    pages of the cache, and a table's other entries none."""
+    b = Batch(18, [1, 2], [100, 48], prefix, 4, 2, 64, kind, 16)   # 7 and 3 pages; the others -7
+    b.lens = [1 << 30, 1 << 30]
+    b.lens_d.copy_(ints(b.lens))
+    out = b.check().copy()
+    b.lens_d.copy_(ints([100, 1000]))
+    assert np.array_equal(out, host(b.run()))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_pages_outside_the_cache_are_not_seen(gpu_ready, kind):
     b = Batch(4, [1, 3], [100, 90], 64, 8, 4, 128, kind, 16)
     b.tables[0, 2], b.tables[1, 0] = -1, b.keys.shape[0]
