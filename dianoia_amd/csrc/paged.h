@@ -21,6 +21,8 @@ inline bool batch_ok(const dnx_paged_batch* b) {
          b->max_len >= 0 && b->max_len <= (1 << 30) && b->prefix_len >= 0 &&
          b->prefix_len <= (1 << 30) && b->prefix_len + b->max_len <= 0x7fffffff && b->table_stride >= 0 && b->table_stride <= (1 << 26) &&
          b->starts != nullptr && b->lens != nullptr &&
+         (((uintptr_t)b->starts | (uintptr_t)b->lens | (uintptr_t)b->tables |
+           (uintptr_t)b->prefix_pages) & 3) == 0 &&
          (b->tables != nullptr || b->max_len == 0 || b->table_stride == 0) &&
          (b->prefix_pages != nullptr || b->prefix_len == 0);
 }

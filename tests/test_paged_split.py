@@ -287,3 +287,20 @@ def test_blocks_in_a_row_where_many_would_be_empty(fit):
     assert slots(64, 575, 512) == 575 * 4 // 64 + 64
     assert slots(64, 64, 64) == 64 * 4 // 64 + 64
     assert slots(2, 40, 39) == 0 and slots(64, 64, 64, length=0) == 0
+
+
+def test_arrays_off_their_alignment_are_refused():
+    """A scalar load drops the last bits of an address: it would read other numbers."""
+    from dianoia_amd import _lib
+    lib = _lib.load()
+    a = 4096
+    c = _lib.PagedCacheStruct(keys=a, values=a, pages=64, page=16, kv_heads=2, hd=64, type=0)
+    good = dict(starts=a, lens=a, tables=a, prefix_pages=a, table_stride=4, prefix_len=1000, seqs=3,
+                tokens=8, max_tokens=1, max_len=64)
+    size = lambda **k: lib.dnx_paged_attention_workspace_bytes(
+        ctypes.byref(c), ctypes.byref(_lib.PagedBatchStruct(**{**good, **k})), 4)
+    assert size() > 0
+    for name in ("starts", "lens", "tables", "prefix_pages"):
+        for off in (1, 2, 3):
+            assert size(**{name: a + off}) == -1, (name, off)
+        assert size(**{name: a + 4}) > 0
