@@ -511,6 +511,41 @@ def test_lengths_past_the_bound(gpu_ready, prefix, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("prefix", [0, 200])
+def test_another_prompt_at_each_replay(gpu_ready, prefix, kind):
+    """One captured call whose rows are another sequence's at each replay: the
+    prompt of 150 tokens moves, the others have one token or none."""
+    seqs, heads, kv, lens = 48, 8, 8, [200 + i for i in range(48)]
+    ones = Batch(41, [1] * seqs, lens, prefix, heads, kv, 64, kind, 32, gate=True)
+    rows = 150 + seqs
+    g = torch.Generator(device="cuda").manual_seed(6)
+    ones.q = 2 * torch.randn(rows, heads, 64, device="cuda", generator=g)
+    ones.gate = torch.randn(rows, heads, device="cuda", generator=g)
+    ones.out = torch.full((rows, heads, 64), 3.25, device="cuda")
+    ones.batch = D.PagedBatch(ones.starts, ones.lens_d, ones.tables, rows, 150, max(lens),
+                              prefix_pages=ones.batch.prefix_pages, prefix_len=prefix)
+    ones.ws = D.paged_attention_workspace(ones.cache, ones.batch, heads)
+    ones.ws.fill_(0xff)
+    ones.run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ones.run()
+    for at in (0, 17, seqs - 1, 5):
+        counts = [1 if (i + at) % 3 else 0 for i in range(seqs)]
+        counts[at] = 150
+        ones.counts, ones.live = counts, sum(counts)
+        ones.starts.copy_(ints(np.concatenate([[0], np.cumsum(counts)])))
+        ones.out.fill_(3.25)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = ones.out.clone()
+        ones.out.fill_(3.25)
+        ones.check()
+        assert torch.equal(got, ones.out)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_pages_outside_the_cache_are_not_seen(gpu_ready, kind):
     b = Batch(4, [1, 3], [100, 90], 64, 8, 4, 128, kind, 16)
     b.tables[0, 2], b.tables[1, 0] = -1, b.keys.shape[0]
