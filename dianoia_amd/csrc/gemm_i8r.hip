@@ -31,8 +31,8 @@ struct I8RArgs {
 // tokens, its eight waves an eighth of K each, both operands straight from
 // memory into the fragments of v_mfma_i32_16x16x64_i8 (lane l: row l % 16, the
 // 16 bytes at k = 16 (l / 16) of 64), four steps requested at once; the eight
-// sums meet in LDS. 13 x 6144 x 2048: 5.4 us, 2.4 TB/s, of which about 2.0 us
-// are an empty launch's; 16 x 128256 x 4096 128 us, 4.2 TB/s.
+// sums meet in LDS. 13 x 6144 x 2048: 5.1 us (5.8 on another card), 2.5 TB/s, of
+// which about 2.0 us are an empty launch's; 16 x 128256 x 4096 128 us, 4.2 TB/s.
 constexpr int kFewWaves = 8, kFewRows = 16, kFewSteps = 4;
 
 template <int NR>
@@ -98,10 +98,10 @@ __global__ void __launch_bounds__(kFewWaves * 64) gemm_i8r_few_kernel(I8RArgs p)
 // tiles alone are too few to keep the chip busy; their sums are added in LDS.
 //
 // 2047 x 8192 x 4096 on 256 x 256 tiles of 16 waves: 73 to 76 us, 1.8 to 1.9
-// POP/s (a library product of that size with int32 outputs takes 76). The
-// matrix cores are busy half of the cycles (65 k of 131 k a CU) and the clock
-// falls to about 1.8 GHz under them; LDS is busy 25 k cycles, without bank
-// conflicts; the 67 MB of outputs are 5 us. Eight waves of twice the tile took
+// POP/s (a library product of that size with int32 outputs takes 76). By the
+// counters the matrix cores are busy 66 k of 106 k cycles, and the clock falls to
+// about 1.5 GHz under them; LDS is busy 37 k cycles, without bank conflicts; the
+// 67 MB of outputs are 5 us. Eight waves of twice the tile took
 // 80 us (fewer waves to cover a barrier), four 85. 1024 x 4304 x 1152: 14 us.
 constexpr int kStageK = 64;
 

@@ -799,9 +799,9 @@ attention_combine_kernel(const float* __restrict__ ws, const float* __restrict__
 // out. A float32 operand of 2^-110 or more is the exact sum of three bf16
 // pieces (8 significant bits each; below that the last piece is a bf16
 // subnormal or lost: 2e-7 of the operand at 2^-112, 2e-3 at 2^-125); of the
-// nine piece products of a q.k or p.v term the six with i + j <= 2 are formed,
-// the others lie below 2^-26 of the term, and the sums are float32. Six bf16 MFMAs cost less than half of the float32
-// ones they replace (v_mfma_f32_16x16x4f32: 32 multiply-adds a clock and
+// nine piece products of a q.k or p.v term the six with i + j <= 2 are formed
+// (of the others two reach 2^-25 of the term, all together 2^-24), and the sums
+// are float32. Six bf16 MFMAs cost less than half of the float32 ones they replace (v_mfma_f32_16x16x4f32: 32 multiply-adds a clock and
 // SIMD, 16x16x32_bf16: 512).
 //
 // A wave takes 16 queries of one head, a workgroup 4 waves sharing one KV

@@ -766,8 +766,9 @@ DNX_DEV void few(const PagedArgs& a, const Item& w, uint8_t* lds) {
 // values as [8 keys][dim] in the order in which a lane's weights stand (k slot
 // j of quarter g: key 4 g + j, or 16 + 4 g + j - 4), 16 bytes each. float32
 // caches are split into three pieces on the way (PC = 3), each product formed
-// from the six largest products of pieces (below 2^-26 of it are left out). The
-// next tile is in registers meanwhile.
+// from the six largest products of pieces; of the three left out two reach 2^-25
+// of it, all together 2^-24 (a float's half step). The pieces of an operand below
+// 2^-110 are not all of it. The next tile is in registers meanwhile.
 //
 // A prefix of 8192 keys, bf16, for 64 tokens of 32 / 8 heads, hd 128: 40 us
 // for 16 tiles of 64 keys a wave, 0.6 PFLOP/s of bf16 products, three for each

@@ -530,8 +530,9 @@ int dnx_quantize_i8r(const float* x, int8_t* qs, float* scales, int64_t rows, in
 int dnx_quantize_i8r_bf16(const uint16_t* x, int8_t* qs, float* scales, int64_t rows, int64_t cols,
                           int64_t cols_pad, dnx_stream_t stream);
 // The same of RMSNorm(s) * w, s = x + m (float32, written to x_out, which may
-// be x or m) or, with m and x_out both null, s = x. Sums and codes are formed
-// in 64 bits: they do not depend on an order of summation.
+// be x or m) or, with m and x_out both null, s = x. In 64 bits: the codes do not
+// depend on the sum of squares, and a scale is that of the formula, rounded once
+// (but for the last bits of a sum of doubles).
 int dnx_rms_norm_i8r(const float* x, const float* m, float* x_out, const float* w, int8_t* qs,
                      float* scales, int64_t rows, int64_t cols, int64_t cols_pad, float eps,
                      dnx_stream_t stream);
@@ -568,7 +569,9 @@ typedef struct {
 // lies outside the cache (-1: padding) or whose position lies outside the
 // table is left out: nothing is written for it. Two tokens of one call must
 // not have the same slot (which of them is kept, and whether whole, is open).
-// Strides in floats, multiples of 4; pointers 16-byte aligned.
+// Strides in floats, multiples of 4; pointers 16-byte aligned (positions and
+// slots 4). n up to 2^22, heads up to 65535, n * (heads + 2 kv_heads) * hd below
+// 2^35 - 2048.
 int dnx_paged_append(const dnx_paged_cache* cache, const float* q, int64_t q_stride, float* q_out,
                      const float* k, int64_t k_stride, const float* v, int64_t v_stride,
                      const float* q_norm, const float* k_norm, const float* rope,
@@ -586,7 +589,9 @@ int dnx_paged_append(const dnx_paged_cache* cache, const float* q, int64_t q_str
 // read nor written. The arrays lie in device
 // memory and may change from call to call under one captured graph; the
 // numbers here bound them: no sequence has more than max_tokens new tokens,
-// and own keys past max_len or past the table are not seen.
+// and own keys past max_len or past the table are not seen. tokens and max_tokens
+// up to 2^22, seqs to 2^20, prefix_len and max_len to 2^30 (below 2^31 together),
+// table_stride to 2^26, heads to 65535; the arrays 4-byte aligned.
 typedef struct {
   const int32_t* starts;
   const int32_t* lens;
@@ -608,7 +613,11 @@ typedef struct {
 // prefix's keys are read once for all sequences. Keys in a page outside the
 // cache are not seen, a row without any weight (no key seen) is zeros, and
 // what lies in masked places (infinities, NaN) does not matter, but for the
-// last bits of rows that share a step with it. float32 accuracy throughout.
+// last bits of rows that share a step with it. float32 accuracy: sums are
+// float32, of values times weights of up to 2^8. Where the bf16 matrix cores are
+// used (bf16 caches, and float32 ones where more than 32 rows share keys), each
+// float32 operand is taken as three pieces, whose sum it is down to 2^-110: of
+// values of 2^-118 5e-6 is lost, of 2^-125 6e-4.
 // workspace: dnx_paged_attention_workspace_bytes of device memory (the partial
 // results of runs of keys), 16-byte aligned; calls that overlap need one each.
 // Batches of up to 2^22 key heads (seqs * kv_heads) are served whatever their
