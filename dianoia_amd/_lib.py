@@ -152,8 +152,11 @@ SIGNATURES = {
     "dnx_gemm_i8r": ([_p] * 5 + [_i64] * 3 + [_p], _i32),
     "dnx_paged_append": ([_p, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _p, _i64,
                           _i64, _f32, _p], _i32),
+    "dnx_paged_read": ([_p, _p, _p, _i64, _p, _i64, _i64, _p], _i32),
     "dnx_paged_attention_workspace_bytes": ([_p, _p, _i64], _i64),
     "dnx_paged_attention": ([_p] * 5 + [_i64, _i64, _p, _i64, _p], _i32),
+    "dnx_sample_workspace_bytes": ([_i64, _i64], _i64),
+    "dnx_sample": ([_p, _i64] + [_p] * 6 + [_i64, _i64, _p, _i64, _p], _i32),
     "dnx_add": ([_p, _p, _i64, _p], _i32),
     "dnx_copy": ([_p, _p, _i64, _p], _i32),
     "dnx_steer": ([_p, _p, _i64, _i64, _i64, _f32, _p], _i32),
@@ -163,7 +166,8 @@ SIGNATURES = {
 class PagedCacheStruct(ctypes.Structure):
     """dnx_paged_cache."""
     _fields_ = [("keys", _p), ("values", _p), ("pages", _i64), ("page", ctypes.c_int32),
-                ("kv_heads", ctypes.c_int32), ("hd", ctypes.c_int32), ("type", ctypes.c_int32)]
+                ("kv_heads", ctypes.c_int32), ("hd", ctypes.c_int32), ("type", ctypes.c_int32),
+                ("key_scales", _p), ("value_scales", _p)]
 
 
 class PagedBatchStruct(ctypes.Structure):

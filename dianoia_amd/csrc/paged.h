@@ -12,7 +12,10 @@ inline bool cache_ok(const dnx_paged_cache* c) {
          (((uintptr_t)c->keys | (uintptr_t)c->values) & 15) == 0 && c->pages > 0 &&
          c->page >= 16 && c->page <= 4096 && (c->page & (c->page - 1)) == 0 &&
          c->pages <= 0x7fffffff / c->page && (c->hd == 64 || c->hd == 128) && c->kv_heads > 0 &&
-         c->kv_heads <= 1024 && (c->type == DNX_F32 || c->type == DNX_BF16);
+         c->kv_heads <= 1024 &&
+         (c->type == DNX_F32 || c->type == DNX_BF16 ||
+          (c->type == DNX_I8 && c->key_scales != nullptr && c->value_scales != nullptr &&
+           (((uintptr_t)c->key_scales | (uintptr_t)c->value_scales) & 15) == 0));
 }
 
 inline bool batch_ok(const dnx_paged_batch* b) {

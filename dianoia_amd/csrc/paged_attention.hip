@@ -14,6 +14,7 @@
 #include "bf16_pieces.h"
 #include "common.h"
 #include "paged.h"
+#include "paged_i8.h"
 #include "paged_split.h"
 
 #include <math.h>
@@ -1336,6 +1337,7 @@ int64_t dnx_paged_attention_workspace_bytes(const dnx_paged_cache* cache,
       heads > 65535 || batch->tokens * heads >= (1 << 26)) {
     return -1;
   }
+  if (cache->type == DNX_I8) return 0;
   const PagedSplit s = split_of(cache, batch, heads);
   if (s.prefix_items + s.own_items > kPagedItems) return -1;
   return s.splits() <= 1 ? 0 : batch->tokens * heads * s.splits() * (cache->hd + 2) * 4;
@@ -1353,6 +1355,9 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
       (need > 0 && (workspace == nullptr || ((uintptr_t)workspace & 15) != 0))) {
     return DNX_EINVAL;
   }
+  if (cache->type == DNX_I8)
+    return paged_attention_i8(cache, batch, q, gate, out, heads, window, most_own(cache, batch),
+                              (hipStream_t)stream);
   const PagedSplit s = split_of(cache, batch, heads);
   PagedArgs a{};
   a.keys = cache->keys;

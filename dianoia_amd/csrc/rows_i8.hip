@@ -17,6 +17,7 @@
 // 64-bit multiply-adds run at the rate of 32-bit ones on this chip, so the
 // rows stay bound by their bytes.
 
+#include "codes_i8.h"
 #include "common.h"
 #include "dnx_kernels.h"
 
@@ -34,12 +35,6 @@ constexpr int64_t kMaxCols = (int64_t)kMaxThreads * kMaxV * 4;
 
 // A wave's sum and maximum in 64 bits, and the maximum of unsigned words, on
 // DPP (as wave_sum_dpp): every lane gets the same bits. All lanes active.
-template <int Ctrl>
-DNX_DEV double dpp64(double v) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint64_t lo = (uint32_t)dpp<Ctrl>((int)(uint32_t)b), hi = (uint32_t)dpp<Ctrl>((int)(b >> 32));
-  return __builtin_bit_cast(double, hi << 32 | lo);
-}
 DNX_DEV double lane_value64(double v, int lane) {
   const uint64_t b = __builtin_bit_cast(uint64_t, v);
   const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane);
@@ -77,16 +72,6 @@ DNX_DEV float4 load4(const uint16_t* p) {
                      __uint_as_float(b.y << 16), __uint_as_float(b.y & 0xffff0000u));
 }
 
-// One code: the nearest whole number to y * inv, halves away from zero.
-DNX_DEV int code1(double y, double inv) {
-  const double t = y * inv;
-  return (int)(t + __builtin_copysign(0.5, t));
-}
-
-DNX_DEV int pack4(int a, int b, int c, int d) {
-  return (a & 0xff) | ((b & 0xff) << 8) | ((c & 0xff) << 16) | (int)((uint32_t)d << 24);
-}
-
 // Four normed values' part of a row's sum of squares and top = max |y| without
 // r. The sum also tells of an infinity or NaN: it is finite in 64 bits for
 // finite floats, and nothing times a product is added to it, for one in w.
@@ -120,11 +105,6 @@ DNX_DEV void norm_reduce(double& sum, double& top) {
 
 DNX_DEV float norm_scale(double sum, double top, int cols, float eps) {
   return (float)(top / 127.0 * (1.0 / sqrt(sum / (double)cols + (double)eps)));
-}
-
-// 127 / top, rounded up by 2^-50.
-DNX_DEV double code_factor(double top, bool fine) {
-  return fine && top > 0.0 ? 127.0 / top * (1.0 + 0x1p-50) : 0.0;
 }
 
 // A normed row of more values than registers hold: read again for the codes.

@@ -752,28 +752,42 @@ def gemm_i8r(w, w_scale, x, x_scale, y, rows: int, cols: int, n: int, stream=Non
         _check(rc, "dnx_gemm_i8r")
 
 
-_CACHE_TYPES = {torch.float32: 0, torch.bfloat16: 1}   # DNX_F32, DNX_BF16
+_CACHE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.int8: 2}   # DNX_F32, DNX_BF16, DNX_I8
 
 
 class PagedCache:
     """Keys and values in pages: two tensors [pages][page][kv_heads][hd],
-    float32 or bfloat16 (dnx_paged_cache). Keeps the tensors, not copies."""
+    float32, bfloat16 or int8 (dnx_paged_cache); with int8 also the codes'
+    scales, two float32 tensors [pages][kv_heads][page]. Keeps the tensors, not
+    copies."""
 
-    def __init__(self, keys: torch.Tensor, values: torch.Tensor):
+    def __init__(self, keys: torch.Tensor, values: torch.Tensor,
+                 key_scales: torch.Tensor | None = None, value_scales: torch.Tensor | None = None):
         if keys.dim() != 4 or keys.shape != values.shape or keys.dtype != values.dtype:
             raise ValueError("PagedCache: two tensors [pages][page][kv_heads][hd] of one type")
         if keys.dtype not in _CACHE_TYPES:
-            raise ValueError("PagedCache: float32 or bfloat16")
+            raise ValueError("PagedCache: float32, bfloat16 or int8")
         pages, page, kv_heads, hd = keys.shape
         if page < 16 or page > 4096 or page & (page - 1):
             raise ValueError("PagedCache: the page is a power of two from 16 to 4096")
         if hd not in (64, 128) or not 0 < kv_heads <= 1024 or not 0 < pages * page <= 0x7fffffff:
             raise ValueError("PagedCache: hd 64 or 128, up to 1024 heads, below 2^31 places")
+        scales = (key_scales, value_scales)
+        if keys.dtype is _I8:
+            if any(s is None or s.dtype is not _F32 or s.shape != (pages, kv_heads, page)
+                   for s in scales):
+                raise ValueError("PagedCache: int8 takes two float32 tensors of scales "
+                                 "[pages][kv_heads][page]")
+        elif any(s is not None for s in scales):
+            raise ValueError("PagedCache: scales belong to int8 keys and values")
         self.keys, self.values = keys, values
+        self.key_scales, self.value_scales = scales
         self.page, self.kv_heads, self.hd = page, kv_heads, hd
         self.device = keys.get_device()
         self.struct = _lib.PagedCacheStruct(_ptr(keys), _at(values, self.device), pages, page,
-                                            kv_heads, hd, _CACHE_TYPES[keys.dtype])
+                                            kv_heads, hd, _CACHE_TYPES[keys.dtype],
+                                            _at(key_scales, self.device),
+                                            _at(value_scales, self.device))
         self.ref = ctypes.addressof(self.struct)
 
     def check_device(self) -> int:
@@ -873,6 +887,29 @@ def paged_append(cache: PagedCache, k, v, positions, slots, rope=None, q=None, q
         _check(rc, "dnx_paged_append")
 
 
+def paged_read(cache: PagedCache, slots, k=None, v=None, stream=None) -> None:
+    """Places `slots` of the cache as float32 into k and v [n][kv_heads][hd]
+    (dnx_paged_read); either may be left out, and both may be views of one
+    tensor's rows. A row whose slot lies outside the cache is left as it is."""
+    d = cache.check_device()
+    n, kv_heads, hd = slots.numel(), cache.kv_heads, cache.hd
+    at = []
+    for t in (k, v):
+        if t is None:
+            at += [None, 0]
+            continue
+        s0, s1, s2 = t.stride() if t.dim() == 3 else (0, 0, 0)
+        if (t.shape != (n, kv_heads, hd) or t.dtype is not _F32 or s2 != 1
+                or (kv_heads != 1 and s1 != hd) or t.get_device() != d):
+            raise ValueError("paged_read: k and v are float32 [n][kv_heads][hd] with dense heads, "
+                             "on the cache's device")
+        at += [t.data_ptr(), s0 if n > 1 else kv_heads * hd]
+    rc = _lib.load().dnx_paged_read(cache.ref, _numbers("slots", slots, d, n, _I32), *at, n,
+                                    _on(d, stream))
+    if rc:
+        _check(rc, "dnx_paged_read")
+
+
 def paged_attention_workspace(cache: PagedCache, batch: PagedBatch, heads: int,
                               device="cuda") -> torch.Tensor:
     """Device workspace of paged_attention for a batch of these bounds."""
@@ -901,3 +938,39 @@ def paged_attention(cache: PagedCache, batch: PagedBatch, q, out, workspace, win
                                          _stream(stream))
     if rc:
         _check(rc, "dnx_paged_attention")
+
+
+def sample_workspace(rows: int, vocab: int, device="cuda") -> torch.Tensor:
+    """Device workspace of sample for that many rows of logits."""
+    nbytes = int(_lib.load().dnx_sample_workspace_bytes(rows, vocab))
+    if nbytes < 0:
+        raise RuntimeError(f"dnx_sample_workspace_bytes({rows}, {vocab}) refused the shape")
+    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+
+
+def sample(logits, u, out, workspace, temperature=None, top_k=None, top_p=None, min_p=None,
+           stream=None) -> None:
+    """A token for each row of logits [rows][vocab], from random numbers u
+    [rows] in [0, 1), into out [rows] int32 (dnx_sample). The parameters are
+    tensors [rows], float32 and (top_k) int32: left out, or 1, 0, 1 and 0, they
+    change nothing; a temperature of 0 is the greedy answer. A row whose logits
+    are all -infinity gives -1."""
+    if logits.dim() != 2 or logits.dtype is not _F32:
+        raise ValueError("sample: logits are float32 [rows][vocab]")
+    d = _device_of(logits)
+    rows, vocab = logits.shape
+    stride, inner = logits.stride()
+    if inner != 1 and vocab != 1:
+        raise ValueError("sample: the logits of a row lie side by side")
+
+    def given(what, t, dtype):
+        return None if t is None else _numbers(what, t, d, rows, dtype)
+
+    rc = _lib.load().dnx_sample(
+        logits.data_ptr(), stride if rows > 1 else vocab, _numbers("u", u, d, rows, _F32),
+        given("temperature", temperature, _F32), given("top_k", top_k, _I32),
+        given("top_p", top_p, _F32), given("min_p", min_p, _F32),
+        _numbers("out", out, d, rows, _I32), rows, vocab, _at(workspace, d), workspace.nbytes,
+        _on(d, stream))
+    if rc:
+        _check(rc, "dnx_sample")

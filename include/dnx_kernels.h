@@ -545,8 +545,12 @@ int dnx_gemm_i8r(const int8_t* w, const float* w_scale, const int8_t* x, const f
 
 // Keys and values in pages: each [pages][page][kv_heads][hd], of `type`, page
 // a power of two from 16 to 4096, hd 64 or 128, pages * page below 2^31,
-// kv_heads up to 1024, 16-byte aligned.
-enum { DNX_F32 = 0, DNX_BF16 = 1 };
+// kv_heads up to 1024, 16-byte aligned. An int8 cache holds codes from -127 to
+// 127 and a float32 scale for each place and key head: value = code * scale,
+// the scales [pages][kv_heads][page], 16-byte aligned (a page's scales of one
+// head lie side by side, as attention reads them). The scales' pointers are
+// read for such a cache only.
+enum { DNX_F32 = 0, DNX_BF16 = 1, DNX_I8 = 2 };
 typedef struct {
   void* keys;
   void* values;
@@ -555,6 +559,8 @@ typedef struct {
   int32_t kv_heads;
   int32_t hd;
   int32_t type;
+  float* key_scales;
+  float* value_scales;
 } dnx_paged_cache;
 
 // New tokens' keys and values into their places of the cache. Token t's key
@@ -563,7 +569,11 @@ typedef struct {
 // rope[positions[t]], a row of a table [rope_rows][cos(hd / 2), sin(hd / 2)];
 // null: not) as dnx_head_norm_rope does, its values taken as they are, and
 // both rounded to the cache's type (to nearest, ties to even) at place
-// slots[t] = page * c.page + row of the page. With q (heads per token, null:
+// slots[t] = page * c.page + row of the page. For an int8 cache the keys are
+// normed and rotated in 64 bits: scale = the head's largest |value| / 127,
+// each code the nearest whole number to value / scale, halves away from zero; a
+// head that holds an infinity or NaN, or whose scale is no float, gets a NaN
+// scale and zero codes (a scale below 2^-126 has a subnormal's few bits). With q (heads per token, null:
 // none) the token's queries are normed with q_norm and rotated into q_out
 // [n][heads][hd], which may be q where that is contiguous. A token whose slot
 // lies outside the cache (-1: padding) or whose position lies outside the
@@ -577,6 +587,15 @@ int dnx_paged_append(const dnx_paged_cache* cache, const float* q, int64_t q_str
                      const float* q_norm, const float* k_norm, const float* rope,
                      int64_t rope_rows, const int32_t* positions, const int32_t* slots,
                      int64_t heads, int64_t n, float eps, dnx_stream_t stream);
+
+// Places of the cache as float32: row i of k and v (kv_heads * hd floats at k +
+// i * k_stride) are the key and value heads at place slots[i], exactly what
+// attention takes them for (an int8 cache: code * scale, rounded once). k or v
+// may be null. A row whose slot lies outside the cache is left as it is; the
+// same slot may be read twice. Strides in floats, multiples of 4; k and v
+// 16-byte aligned, slots 4. n up to 2^22, n * kv_heads * hd up to 2^34 - 1024.
+int dnx_paged_read(const dnx_paged_cache* cache, const int32_t* slots, float* k, int64_t k_stride,
+                   float* v, int64_t v_stride, int64_t n, dnx_stream_t stream);
 
 // A batch over such a cache. Its first prefix_len keys, in the pages listed in
 // prefix_pages, are shared: every sequence begins with them. Sequence b's own
@@ -630,6 +649,31 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
                         const float* q, const float* gate, float* out, int64_t heads,
                         int64_t window, void* workspace, int64_t workspace_bytes,
                         dnx_stream_t stream);
+
+// Rows of logits to tokens, from given random numbers u [rows] in [0, 1). With
+// the row's largest logit M, token j weighs w_j = e^((l_j - M) / temperature).
+// In the order of falling logits, of equal ones the lowest index first: the
+// first top_k tokens; of these the shortest beginning that holds top_p of their
+// weight (the token that reaches it among them); of these the tokens with w_j >=
+// min_p. The answer out[row] is the first kept token, in the order of indices,
+// up to which the kept weights' sum exceeds u times that of all. The four
+// parameters are arrays [rows] in device memory, or null: temperature 1 and no
+// filters. A temperature that is not above zero (NaN too) takes the largest
+// logit's first token, whatever the filters; top_k outside 1 .. vocab - 1,
+// top_p from 1 on and NaN, min_p from 0 down and NaN keep everything, top_p from
+// 0 down and min_p from 1 on only the largest; u below 0 and NaN is 0, from 1 on
+// the last kept token's. A logit of NaN is as one of -infinity: never taken, and
+// a row of nothing else gives -1; of logits of +infinity each weighs 1, all else
+// 0. Weights are multiples of 2^-43 of the largest, rounded to nearest, their
+// sums exact: the same logits give the same token, however they are dealt to
+// threads. Row i at logits + i * stride floats, vocab up to 2^20, rows to 2^16;
+// pointers 4-byte aligned. workspace: dnx_sample_workspace_bytes of device
+// memory, 16-byte aligned; calls that overlap need one each.
+int64_t dnx_sample_workspace_bytes(int64_t rows, int64_t vocab);
+int dnx_sample(const float* logits, int64_t stride, const float* u, const float* temperature,
+               const int32_t* top_k, const float* top_p, const float* min_p, int32_t* out,
+               int64_t rows, int64_t vocab, void* workspace, int64_t workspace_bytes,
+               dnx_stream_t stream);
 
 #ifdef __cplusplus
 }

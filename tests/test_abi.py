@@ -69,3 +69,46 @@ def test_sizes_refuse_floats_also_after_integers(size):
     assert size(64, 96) > 0
     with pytest.raises(ctypes.ArgumentError):
         size(64.0, 96)
+
+
+def test_int8_cache_and_sampling_refusals():
+    """What the entry points of the int8 paged cache and of the sampling refuse,
+    none of which launches."""
+    lib = _lib.load()
+    a = 4096   # a pointer that no refused call reads
+
+    def cache(**k):
+        return ctypes.byref(_lib.PagedCacheStruct(**{**dict(
+            keys=a, values=a, pages=64, page=16, kv_heads=2, hd=64, type=2, key_scales=a,
+            value_scales=a), **k}))
+
+    def read(c=None, **k):
+        v = {**dict(slots=a, k=a, ks=128, v=a, vs=128, n=2, st=None), **k}
+        return lib.dnx_paged_read(c or cache(), *v.values())
+
+    bad_caches = [dict(keys=None), dict(key_scales=None), dict(value_scales=None), dict(key_scales=a + 4),
+                  dict(value_scales=a + 8), dict(type=3), dict(hd=32), dict(page=24), dict(kv_heads=0)]
+    for bad in bad_caches:
+        assert read(cache(**bad)) == -1, bad
+        assert lib.dnx_paged_append(cache(**bad), None, 0, None, a, 128, a, 128, None, None, None, 0, None,
+                                    a, 0, 2, 1e-6, None) == -1, bad
+    for bad in (dict(slots=None), dict(slots=a + 2), dict(k=None, v=None), dict(k=a + 4), dict(v=a + 8),
+                dict(ks=127), dict(ks=130), dict(vs=64), dict(n=-1), dict(n=(1 << 22) + 1)):
+        assert read(**bad) == -1, bad
+    assert read(cache(kv_heads=1024, hd=128), ks=1 << 17, vs=1 << 17, n=(1 << 17) + 1) == -1
+    assert read(n=0) == 0
+
+    def sample(**k):
+        v = {**dict(logits=a, stride=100, u=a, t=a, k=a, p=a, low=a, out=a, rows=3, vocab=100, ws=a,
+                    nbytes=1 << 30, st=None), **k}
+        return lib.dnx_sample(*v.values())
+
+    size = lib.dnx_sample_workspace_bytes
+    assert size(3, 100) >= 0 and size(0, 1) == 0 and size(1 << 16, 1 << 20) >= 0
+    for rows, vocab in ((-1, 100), (3, 0), (3, -1), ((1 << 16) + 1, 100), (3, (1 << 20) + 1)):
+        assert size(rows, vocab) == -1 and sample(rows=rows, vocab=vocab, stride=1 << 21) == -1
+    for bad in (dict(logits=None), dict(u=None), dict(out=None), dict(logits=a + 2), dict(u=a + 1),
+                dict(t=a + 2), dict(k=a + 1), dict(p=a + 3), dict(low=a + 1), dict(out=a + 2),
+                dict(stride=99), dict(stride=-1), dict(stride=1 << 41), dict(nbytes=-1)):
+        assert sample(**bad) == -1, bad
+    assert sample(rows=0) == 0
