@@ -14,8 +14,7 @@
 #include "bf16_pieces.h"
 #include "common.h"
 #include "paged.h"
-#include "paged_i8.h"
-#include "paged_split.h"
+#include "paged_attention.h"
 
 #include <math.h>
 
@@ -23,116 +22,13 @@ using namespace dnx;
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
-constexpr float kSlack = 8.0f;   // of a running maximum, in units of log2
-
-struct PartArgs {
-  int wide, few, blocks, runs, keys;
-};
-
-struct PagedArgs {
-  const void *keys, *values;
-  int pages, page_bits, row_bytes;   // row_bytes: of all heads of one place
-  int kv_heads, heads, group;
-  const int32_t *starts, *lens, *tables, *prefix_pages;
-  int64_t table_stride;
-  int prefix_len, seqs, tokens, max_len;   // max_len: within the tables too
-  const float *q, *gate;
-  float *out, *stat, *part;   // partials: stat [rows][splits][2], part [rows][splits][hd]
-  int window, splits, joined;
-  PartArgs prefix, own;
-  int64_t prefix_items;
-  uint32_t slots;  // of all sequences' blocks together, or 0
-  int combine_x;   // of the second launch's workgroups, whose y counts the rest
-  float scale;
-};
-
-// The factor that takes a partial sum (m, l) to the maximum `top`. A partial
-// without a weight (l = 0: no key seen, or every score -inf) counts for
-// nothing; its m is -inf, which a partial whose scores are all NaN has too.
-DNX_DEV float partial_factor(float m, float l, float top) {
-  return l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-}
-
-// A row's output: o / l times its gate, zeros where no key had a weight.
-DNX_DEV float row_scale(float l, const float* gate, int64_t row) {
-  const float s = l == 0.0f ? 0.0f : 1.0f / l;
-  return gate != nullptr ? s / (1.0f + expf(-gate[row])) : s;
-}
-
-// What a workgroup takes: rows row0 .. of the `rows` of tokens t0 .. that
-// share key head kvh, and keys k_lo .. k_hi - 1 of a list of pages. Where the
-// prefix is joined to a sequence's own keys, these begin at key `joined`; the
-// keys from prefix_len to there do not exist.
-struct Item {
-  bool own;
-  int kvh, run, row0, rows, t0, first;   // first: the place of token t0 among the keys
-  int k_lo, k_hi, count, joined;
-  int most;                 // of the list's keys, whatever lens says
-  int page[2];              // of a wave's first keys in a narrow block, and 16 further
-  const int32_t* table;
-};
-
-// The output row of row r of an item.
-DNX_DEV int64_t row_at(const PagedArgs& a, const Item& w, int r) {
-  return (int64_t)(w.t0 + r / a.group) * a.heads + w.kvh * a.group + r % a.group;
-}
-
-// The first key under the window of a token that stands at `place`: a place
-// before the first key (down to minus the new tokens) sees no less than that
-// key's, and one far behind the last (a length past its bound) nothing. In 64
-// bits: a place less the widest window, and a prefix's length and any other,
-// leave 32. kBehind is behind every key (2^30 of a prefix, 2^30 own).
-constexpr int64_t kBehind = 0x7fff0000;
-DNX_DEV int window_begin(int64_t place, int window) {
-  return (int)min(max(place, (int64_t)0) - window + 1, kBehind);
-}
-
-// The keys of an item that its row r sees: lo .. hi - 1.
-struct Seen {
-  int lo, hi;
-};
-DNX_DEV Seen row_sees(const PagedArgs& a, const Item& w, int r) {
-  const int token = w.t0 + r / a.group;
-  if (w.own) {
-    const int place = w.first + token - w.t0;
-    const int hi = w.joined + min(w.count, max(place + 1, 0));
-    if (a.window == 0) return {0, hi};
-    if (w.joined == 0) return {window_begin(place, a.window), hi};
-    const int lo = window_begin((int64_t)a.prefix_len + place, a.window);
-    return {lo < a.prefix_len ? lo : lo - a.prefix_len + w.joined, hi};
-  }
-  if (a.window == 0) return {0, w.count};
-  int lo = 0, hi = a.seqs;              // the token's sequence: starts[lo] <= token < starts[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (a.starts[mid] <= token) lo = mid; else hi = mid;
-  }
-  const int64_t place = (int64_t)a.prefix_len + a.lens[lo] - a.starts[lo + 1] + token;
-  return {window_begin(place, a.window), w.count};
-}
-
 // 16 keys of an item from kt on (a page holds whole sixteens) as resources
 // over one head's rows of the cache: what lies behind the last key, or in a
-// page outside the cache, reads as zeros without touching memory. The page is
-// looked up ahead of its use (page_at; past the list's end its last one) and
-// without a branch or the sequence's length, so that no load waits for another.
+// page outside the cache, reads as zeros without touching memory.
 struct Block {
   i32x4 keys, values;
   int end;      // its keys lie before this key (none: not after the first)
 };
-template <bool kJoined>
-DNX_DEV int page_at(const PagedArgs& a, const Item& w, int kt) {
-  const bool own = !kJoined || kt >= w.joined;
-  const int32_t* table = own ? w.table : a.prefix_pages;
-  const int place = own ? min(kJoined ? kt - w.joined : kt, w.most - 1)
-                        : min(kt, a.prefix_len - 1);
-  // Constant memory to the kernel: a scalar load wherever it stands (behind a
-  // store or a barrier the compiler would wait for a vector load instead).
-  typedef const __attribute__((address_space(4))) int32_t* Constant;
-  return __builtin_amdgcn_readfirstlane(((Constant)(uintptr_t)table)[place >> a.page_bits]);
-}
 // Blocks as seen from `behind` keys before them: the offset of key i of the
 // block is that of row behind + i.
 template <typename C, int HD, bool kJoined>
@@ -350,59 +246,6 @@ DNX_DEV void exact_walk(const PagedArgs& a, const Item& w, const float* qp, Seen
       load_values<C, HD>(b, a.row_bytes, l16, g4, x);
       exact_step<C, HD>(x, q, kt, b.end, see, sl, g4, sums, [] {});
     }
-}
-
-// A row's partial result (or, with one run, its output), EV values from dim
-// `dim` on at a time; `stats`: this lane also writes m and l.
-DNX_DEV void write_row4(const PagedArgs& a, const Item& w, int64_t row, int hd, int dim, float4 o,
-                        float m, float l, bool stats) {
-  if (a.splits == 1) {
-    const float f = row_scale(l, a.gate, row);
-    *(float4*)(a.out + row * hd + dim) = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
-  } else {
-    const int64_t p = row * a.splits + (w.own ? a.prefix.runs : 0) + w.run;
-    *(float4*)(a.part + p * hd + dim) = o;
-    if (stats) *(float2*)(a.stat + 2 * p) = make_float2(m, l);
-  }
-}
-
-// Rows of four waves' sums in LDS: [wave][16][kSumRow] and, behind them, each
-// wave's maxima and sums of weights [wave][2][16].
-template <int HD>
-constexpr int kSumRow = HD + 4;
-template <int HD>
-DNX_DEV float* wave_stats(uint8_t* lds, int wave) {
-  return (float*)lds + kWaves * 16 * kSumRow<HD> + wave * 32;
-}
-
-template <int HD>
-constexpr int kMergeBytes = kWaves * (16 * kSumRow<HD> + 32) * 4;
-
-// The four waves' sums of the first N rows, added in wave order.
-template <int HD, int N>
-DNX_DEV void merge_waves(const PagedArgs& a, const Item& w, uint8_t* lds) {
-  const float* all = (const float*)lds;
-  const float* ml = wave_stats<HD>(lds, 0);
-  __syncthreads();
-  for (int i = threadIdx.x; i < N * HD / 4; i += kThreads) {
-    const int r = i / (HD / 4), c = i % (HD / 4);
-    if (w.row0 + r >= w.rows) break;
-    float top = -INFINITY, total = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kWaves; k++) top = fmaxf(top, ml[2 * k * 16 + r]);
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int k = 0; k < kWaves; k++) {
-      const float l = ml[(2 * k + 1) * 16 + r];
-      if (l == 0.0f) continue;
-      const float f = partial_factor(ml[2 * k * 16 + r], l, top);
-      const float4 y = *(const float4*)&all[(k * 16 + r) * kSumRow<HD> + 4 * c];
-      total = fmaf(l, f, total);
-      acc = make_float4(fmaf(y.x, f, acc.x), fmaf(y.y, f, acc.y), fmaf(y.z, f, acc.z),
-                        fmaf(y.w, f, acc.w));
-    }
-    write_row4(a, w, row_at(a, w, w.row0 + r), HD, 4 * c, acc, top, total, c == 0);
-  }
 }
 
 // ---- 16 rows a workgroup, each wave other keys (decode: few rows read many
@@ -1121,112 +964,27 @@ constexpr int attention_lds() {
   return w > n ? w : n;
 }
 
-// Whether none of an own block's rows, up to `end`, sees a key of its run: the
-// run lies behind the sequence's keys (where the bound on the lengths is far
-// above them), or the window or the rows' own places end before it. Such a run
-// only says so; its sums are not written. 64 sequences of 200 keys, bound 32768,
-// 32 / 8 heads, hd 128, bf16: 65 us without this and with a sequence's runs side
-// by side in the launch, 33 with both (13 with the bound at 200).
-DNX_DEV bool unseen(const PagedArgs& a, const Item& w, int end) {
-  int lo = w.k_lo, hi = w.k_hi;
-  if (lo < hi && (a.window > 0 || w.rows > a.group)) {
-    if (a.window > 0) lo = max(lo, window_begin(w.first + w.row0 / a.group, a.window));
-    hi = min(hi, w.first + (end - 1) / a.group + 1);
+template <typename C, int HD>
+struct FloatBody {
+  static constexpr int kKeys = sizeof(C) == 4 ? 16 : 32;
+  static __device__ __forceinline__ void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
+    ::wide<C, HD>(a, w, lds);
   }
-  return lo >= hi;
-}
-
-template <typename C, int HD, bool kJoined>
-DNX_DEV void block_of_16(const PagedArgs& a, const Item& w, int rows, uint8_t* lds) {
-  if constexpr (sizeof(C) == 4) {
-    if (rows == 2) return few<HD, 2, kJoined>(a, w, lds);
-    if (rows == 4) return few<HD, 4, kJoined>(a, w, lds);
+  template <bool kJoined>
+  static __device__ __forceinline__ void block_of_16(const PagedArgs& a, const Item& w, int rows, uint8_t* lds) {
+    if constexpr (sizeof(C) == 4) {
+      if (rows == 2) return few<HD, 2, kJoined>(a, w, lds);
+      if (rows == 4) return few<HD, 4, kJoined>(a, w, lds);
+    }
+    narrow<C, HD, kJoined>(a, w, lds);
   }
-  narrow<C, HD, kJoined>(a, w, lds);
-}
+};
 
-// The prefix's workgroups, then the sequences' own: both kinds in one launch,
-// so that the matrix cores' work on the prefix runs beside the reading of the
-// sequences' keys (64 tokens, 8192 shared keys, 128 to 2048 own, 32 / 8 heads,
-// hd 128, bf16: 93 us, alone 41 and 69; the own ones first 100, with 16384
-// shared and up to 400 own 78 against 105). Workgroups go round the eight XCDs, each with an L2 of its
-// own: the blocks of rows that read the same keys go to one of them.
-// kPacked: the own blocks of all sequences lie in a row (paged_fit). A kernel of
-// its own: the choice in one kernel cost every call 0.1 us (44 calls, geometric
-// mean: 9.11 us against 8.98).
 template <typename C, int HD, bool kPacked>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 paged_attention_kernel(PagedArgs a) {
   __shared__ __align__(16) uint8_t lds[attention_lds<C, HD>()];
-  Item w;
-  uint32_t id = blockIdx.x;
-  w.own = id >= (uint32_t)a.prefix_items;
-  if (w.own) id -= (uint32_t)a.prefix_items;
-  const PartArgs part = w.own ? a.own : a.prefix;
-  const bool packed = kPacked && w.own;   // its blocks lie among all sequences'
-  uint32_t unit = id, sets = a.slots;
-  int block = 0;
-  if (!packed) {
-    const uint32_t turn = id / 8;
-    unit = turn / (uint32_t)part.blocks * 8 + id % 8;
-    block = (int)(turn % (uint32_t)part.blocks);
-    sets = w.own ? (uint32_t)a.seqs : 1;
-  }
-  // The sequences' first runs before their second ones: where the bound on the
-  // lengths is far above them, those that have keys start at once.
-  const uint32_t set = unit / (uint32_t)a.kv_heads;
-  uint32_t b = set % sets;
-  w.kvh = (int)(unit % (uint32_t)a.kv_heads);
-  w.run = (int)(set / sets);
-  if (w.run >= part.runs) return;
-  if (packed) {
-    const int rows = part.wide ? kPagedWide : kPagedNarrow, slot = (int)b;
-    const int live = max(0, min(a.starts[a.seqs], a.tokens));
-    b = (uint32_t)paged_sequence(a.starts, a.seqs, live, a.group, rows, slot);
-    block = slot - paged_slot(a.starts, (int)b, live, a.group, rows);
-    if (block < 0) return;   // before the first sequence's rows
-  }
-  w.k_lo = w.run * part.keys;
-  w.joined = w.own ? a.joined : 0;
-  w.table = w.own ? a.tables + b * a.table_stride : a.prefix_pages;
-  w.most = w.own ? a.max_len : a.prefix_len;
-  // One wait for everything that the first keys' addresses and rows need.
-  int all = a.starts[a.seqs], s0 = a.starts[b], s1 = a.starts[b + 1], len = a.lens[b];
-  {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int first = w.k_lo + (sizeof(C) == 4 ? 16 : 32) * wave;
-    w.page[0] = page_at<true>(a, w, first);
-    w.page[1] = page_at<true>(a, w, first + 16);
-    asm("" : "+s"(all), "+s"(s0), "+s"(s1), "+s"(len), "+s"(w.page[0]), "+s"(w.page[1]));
-  }
-  const int live = max(0, min(all, a.tokens));
-  w.t0 = w.own ? max(0, min(s0, live)) : 0;
-  const int t1 = w.own ? max(w.t0, min(s1, live)) : live;
-  w.first = w.own ? len - (t1 - w.t0) : 0;
-  w.count = w.own ? max(min(len, a.max_len), 0) : a.prefix_len;
-  w.row0 = block * (part.wide ? kPagedWide : kPagedNarrow);
-  w.rows = (t1 - w.t0) * a.group;
-  if (w.row0 >= w.rows) return;
-  w.k_hi = min(w.joined > 0 && w.count == 0 ? a.prefix_len : w.joined + w.count,
-               w.k_lo + part.keys);
-  const int end = min(w.row0 + (part.wide ? kPagedWide : kPagedNarrow), w.rows);
-  if (w.own && a.splits > 1 && unseen(a, w, end)) {
-    const int r = w.row0 + threadIdx.x;
-    if (r < end) {
-      const int64_t p = row_at(a, w, r) * a.splits + a.prefix.runs + w.run;
-      *(float2*)(a.stat + 2 * p) = make_float2(-INFINITY, 0.0f);
-    }
-    return;
-  }
-  if (part.wide) {
-    wide<C, HD>(a, w, lds);
-    return;
-  }
-  if (w.joined > 0) {
-    block_of_16<C, HD, true>(a, w, part.few, lds);
-  } else {
-    block_of_16<C, HD, false>(a, w, part.few, lds);
-  }
+  paged_workgroup<FloatBody<C, HD>, kPacked>(a, lds);
 }
 
 // A row's partial results added in order by W waves, an equal part of the runs
@@ -1337,7 +1095,6 @@ int64_t dnx_paged_attention_workspace_bytes(const dnx_paged_cache* cache,
       heads > 65535 || batch->tokens * heads >= (1 << 26)) {
     return -1;
   }
-  if (cache->type == DNX_I8) return 0;
   const PagedSplit s = split_of(cache, batch, heads);
   if (s.prefix_items + s.own_items > kPagedItems) return -1;
   return s.splits() <= 1 ? 0 : batch->tokens * heads * s.splits() * (cache->hd + 2) * 4;
@@ -1355,16 +1112,15 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
       (need > 0 && (workspace == nullptr || ((uintptr_t)workspace & 15) != 0))) {
     return DNX_EINVAL;
   }
-  if (cache->type == DNX_I8)
-    return paged_attention_i8(cache, batch, q, gate, out, heads, window, most_own(cache, batch),
-                              (hipStream_t)stream);
   const PagedSplit s = split_of(cache, batch, heads);
   PagedArgs a{};
   a.keys = cache->keys;
   a.values = cache->values;
   a.pages = (int)cache->pages;
   a.page_bits = __builtin_ctz((unsigned)cache->page);
-  a.row_bytes = cache->kv_heads * cache->hd * (cache->type == DNX_F32 ? 4 : 2);
+  a.row_bytes = cache->kv_heads * cache->hd * (cache->type == DNX_F32 ? 4 : cache->type == DNX_BF16 ? 2 : 1);
+  a.key_scales = cache->key_scales;
+  a.value_scales = cache->value_scales;
   a.kv_heads = cache->kv_heads;
   a.heads = (int)heads;
   a.group = (int)(heads / cache->kv_heads);
@@ -1394,14 +1150,16 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
   const int64_t grid = s.prefix_items + s.own_items;
   const hipStream_t st = (hipStream_t)stream;
   if (grid > 0) {
-    const int kind = (s.slots > 0 ? 4 : 0) + (cache->type == DNX_F32 ? 0 : 2) + (cache->hd == 128);
+    const int kind = (s.slots > 0 ? 4 : 0) + (cache->type == DNX_BF16 ? 2 : 0) + (cache->hd == 128);
     constexpr decltype(&paged_attention_kernel<float, 64, false>) kernels[] = {
         paged_attention_kernel<float, 64, false>,    paged_attention_kernel<float, 128, false>,
         paged_attention_kernel<uint16_t, 64, false>, paged_attention_kernel<uint16_t, 128, false>,
         paged_attention_kernel<float, 64, true>,     paged_attention_kernel<float, 128, true>,
         paged_attention_kernel<uint16_t, 64, true>,  paged_attention_kernel<uint16_t, 128, true>,
     };
-    hipLaunchKernelGGL(kernels[kind], dim3((unsigned)grid), dim3(kThreads), 0, st, a);
+    const PagedKernel k = cache->type == DNX_I8 ? paged_attention_i8(cache->hd, s.slots > 0)
+                                                : kernels[kind];
+    hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(kThreads), 0, st, a);
     if (hipGetLastError() != hipSuccess) return DNX_ELAUNCH;
   }
   if (a.splits != 1) {
