@@ -21,25 +21,37 @@ using namespace dnx;
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int64_t kMaxVocab = 1 << 20;   // the sum of a row's weights is below 2^64
 constexpr int64_t kMaxRows = 1 << 16;
+constexpr int kBins = 256, kBinsPerUnit = 8;   // of l / T: 32 in all
+constexpr int kMaxChunks = 128;
+constexpr int kChunkFound = 1024;        // tokens of the bins in question, of a chunk
+constexpr int kFound = 4096;             // of a row, that are sorted at once
+constexpr int kParts = 2048;             // of a span of order keys that holds more
 
 struct SampleArgs {
   const float *logits, *u, *temperature, *top_p, *min_p;
   const int32_t* top_k;
   int32_t* out;
   int64_t stride;
-  int vocab;
+  int vocab, chunks;
+  // Of each row and chunk:
+  uint64_t* hist;      // [kBins]: counts (the upper 16 bits) and weights
+  uint64_t* sums;      // [3]: of weights
+  uint64_t* found;     // [kChunkFound] order keys
+  float* tops;         // the largest logit
+  uint32_t* founds;    // how many tokens were found
+  int32_t* cuts;       // [4] of each row: the bins in question
 };
 
-// A row's request. T = 0: greedy.
+// A row's request. Greedy: of a steep T, the first token.
 struct Request {
   double inv_t, top_p, min_p;
-  float u;
+  float u, inv;        // inv: of the bins, finite
   int top_k;
-  bool greedy;
+  bool cut;            // by rank or weight
 };
 DNX_DEV Request request(const SampleArgs& a, int row) {
   Request r;
@@ -48,12 +60,14 @@ DNX_DEV Request request(const SampleArgs& a, int row) {
   const float low = a.min_p != nullptr ? a.min_p[row] : 0.0f;
   const int k = a.top_k != nullptr ? a.top_k[row] : 0;
   const float u = a.u[row];
-  r.greedy = !(t > 0.0f);
-  r.inv_t = r.greedy ? 0.0 : 1.0 / (double)t;
-  r.top_p = p < 1.0f ? fmax((double)p, 0.0) : 1.0;
-  r.min_p = low > 0.0f ? fmin((double)low, 1.0) : 0.0;
-  r.top_k = k > 0 && k < a.vocab ? k : 0;
+  const bool greedy = !(t > 0.0f);
+  r.inv_t = greedy ? 0x1p40 : 1.0 / (double)t;
+  r.inv = (float)fmax(fmin(r.inv_t, 1e37), 1e-41);   // an infinity times it is one
+  r.top_p = !greedy && p < 1.0f ? fmax((double)p, 0.0) : 1.0;
+  r.min_p = !greedy && low > 0.0f ? fmin((double)low, 1.0) : 0.0;
+  r.top_k = greedy ? 1 : k > 0 && k < a.vocab ? k : 0;
   r.u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
+  r.cut = r.top_k > 0 || r.top_p < 1.0;
   return r;
 }
 
@@ -65,21 +79,49 @@ DNX_DEV uint32_t falling_key(float v) {
   if (v != v) b = 0xff800000u;
   return (b & 0x80000000u) ? b : ~b & 0x7fffffffu;
 }
+DNX_DEV float of_key(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k : ~k & 0x7fffffffu);
+}
+DNX_DEV uint64_t order_key(float v, int j) { return (uint64_t)falling_key(v) << 32 | (uint32_t)j; }
 
-// A token's weight in multiples of 2^-43.
-DNX_DEV uint64_t weight(float l, float top, const Request& r) {
+// A token's weight in multiples of 2^-43, and whether that is enough.
+DNX_DEV uint64_t weight(float l, float top, double inv_t) {
   if (!(l > -INFINITY)) return 0;
   if (l == top) return 1ull << 43;
-  const double d = ((double)l - (double)top) * r.inv_t;
-  if (!(d > -31.0)) return 0;
-  const double w = exp(d);
-  if (w < r.min_p) return 0;
-  return (uint64_t)(w * 0x1p43 + 0.5);
+  const double d = ((double)l - (double)top) * inv_t;
+  return d > -31.0 ? (uint64_t)(exp(d) * 0x1p43 + 0.5) : 0;
+}
+DNX_DEV uint64_t at_least(uint64_t w, const Request& r) {
+  return (double)w >= r.min_p * 0x1p43 ? w : 0;
+}
+
+// Bins of l / T, an eighth wide: whole numbers that do not fall as logits rise,
+// the same for every chunk of a row. Far-off values are as the last ones (no
+// difference of two is then an infinity).
+DNX_DEV float scaled(float l, float inv) {
+  return __builtin_amdgcn_fmed3f(l * inv, -1e37f, 1e37f) * (float)kBinsPerUnit;
+}
+// The bin below the one that the row's (or the chunk's) largest logit lies in;
+// kBins and more: no weight.
+DNX_DEV int bin_of(float l, float top, float place, float inv) {
+  if (l == top) return 0;
+  const float d = place - floorf(scaled(l, inv));    // NaN: of a logit NaN
+  return l > -INFINITY && d < (float)kBins ? (int)fmaxf(d, 0.0f) : kBins;
 }
 
 DNX_DEV uint64_t wave_sum_u64(uint64_t v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+template <typename V>
+DNX_DEV V wave_scan(V v) {   // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const V y = __shfl_up(v, o);
+    if (lane >= o) v += y;
+  }
   return v;
 }
 
@@ -94,129 +136,597 @@ DNX_DEV uint64_t block_sum(uint64_t v, uint64_t* part) {
   return v;
 }
 
-// One workgroup a row: cuts are found by their order keys, eight bits at a
-// time, each step counting and weighing the tokens that share the bits found.
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
-  __shared__ uint64_t part[kWaves];
-  __shared__ uint64_t mass[256];
-  __shared__ uint32_t count[256];
-  __shared__ uint64_t found[3];
-  const int row = blockIdx.x, tid = threadIdx.x;
-  const float* x = a.logits + row * a.stride;
-  const Request r = request(a, row);
-
-  uint64_t best = 0;
-  for (int j = tid; j < a.vocab; j += kThreads) {
-    const uint64_t k = (uint64_t)~falling_key(x[j]) << 32 | (uint32_t)~j;
-    best = k > best ? k : best;
-  }
-  best = wave_max_u64(best);
-  if ((tid & 63) == 0) part[tid >> 6] = best;
+// The sum of the threads' values before this one's; the workgroup's in `all`.
+DNX_DEV uint64_t block_before(uint64_t v, uint64_t* part, uint64_t& all) {
+  const uint64_t upto = wave_scan(v);
   __syncthreads();
-  for (int i = 0; i < kWaves; i++) best = part[i] > best ? part[i] : best;
-  const int first = (int)~(uint32_t)best;
-  if (~(uint32_t)(best >> 32) == kNothing) {
+  if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = upto;
+  __syncthreads();
+  uint64_t before = upto - v;
+  all = 0;
+  for (int i = 0; i < kWaves; i++) {
+    if (i < (int)threadIdx.x >> 6) before += part[i];
+    all += part[i];
+  }
+  return before;
+}
+
+// The row's largest logit, of its chunks'.
+DNX_DEV float row_top(const SampleArgs& a, int row) {
+  const int lane = threadIdx.x & 63;
+  float top = -INFINITY;
+  for (int c = lane; c < a.chunks; c += 64) top = fmaxf(top, a.tops[(int64_t)row * a.chunks + c]);
+  return wave_max_dpp(top);
+}
+
+// ---- Step 1, a workgroup a chunk of a row: its largest logit, and (for a row
+// that is cut) how many tokens and how much weight each bin holds, the weights
+// relative to the bin's lower end.
+template <int E>
+DNX_DEV void count_chunk(const SampleArgs& a, int row, int chunk) {
+  __shared__ unsigned long long hist[kBins];
+  __shared__ float part[kWaves];
+  const int tid = threadIdx.x;
+  const float* x = a.logits + row * a.stride;
+  const int j0 = chunk * (kThreads * E) + tid;
+  float l[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int j = j0 + e * kThreads;
+    l[e] = j < a.vocab ? x[j] : -INFINITY;
+  }
+  const Request r = request(a, row);
+  if (tid < kBins) hist[tid] = 0;
+  float top = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < E; e++) top = fmaxf(top, l[e]);
+  top = wave_max_dpp(top);
+  if ((tid & 63) == 0) part[tid >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; i++) top = fmaxf(top, part[i]);
+  const int64_t at = (int64_t)row * a.chunks + chunk;
+  if (tid == 0) a.tops[at] = top;
+  if (!r.cut) return;
+  const float place = floorf(scaled(top, r.inv));
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int b = bin_of(l[e], top, place, r.inv);
+    if (b < kBins) {
+      const float y = scaled(l[e], r.inv);
+      const float w = __builtin_amdgcn_exp2f((y - floorf(y)) * (1.44269504088896341f / kBinsPerUnit));
+      atomicAdd(&hist[b], (1ull << 48) | (unsigned long long)(uint32_t)(w * 0x1p26f + 0.5f));
+    }
+  }
+  __syncthreads();
+  if (tid < kBins) a.hist[at * kBins + tid] = hist[tid];
+}
+
+// The bins in question: cuts lie in bins lo .. hi (by weight) and k (by rank),
+// lo <= hi <= k; before: tokens before bin k. Without a cut lo = kBins.
+struct Cuts {
+  int lo, hi, k, before;
+};
+
+// Step 2 begins with them, in each of a row's workgroups: its chunks' bins added,
+// and their running sums. The weights of bins are off by 2^-22 or, for large l /
+// T, by the rounding of that; where a cut by weight may lie takes this in.
+DNX_DEV Cuts find_cuts(const SampleArgs& a, int row, float top, const Request& r) {
+  __shared__ uint64_t mass[kThreads];
+  __shared__ uint32_t count[kThreads];
+  __shared__ int32_t found[3][kBins / 64];
+  const int tid = threadIdx.x, b = tid % kBins;
+  const float place = floorf(scaled(top, r.inv));
+  uint64_t w = 0;
+  uint32_t n = 0;
+  for (int c = tid / kBins; c < a.chunks; c += kThreads / kBins) {
+    const int64_t at = (int64_t)row * a.chunks + c;
+    const float mine = a.tops[at];
+    const float d = mine == top ? 0.0f : place - floorf(scaled(mine, r.inv));
+    const int i = mine > -INFINITY && d < (float)kBins ? b - (int)fmaxf(d, 0.0f) : -1;
+    if (i < 0) continue;
+    const uint64_t h = a.hist[at * kBins + i];
+    w += h & ((1ull << 48) - 1);
+    n += (uint32_t)(h >> 48);
+  }
+  mass[tid] = w;
+  count[tid] = n;
+  __syncthreads();
+  if (tid < kBins) {
+    for (int k = tid + kBins; k < kThreads; k += kBins) w += mass[k], n += count[k];
+    // Below 2^(26 + 20 + 1): in whole multiples, whose running sums rise.
+    mass[tid] = (uint64_t)((double)w * exp((double)tid * (-1.0 / kBinsPerUnit)) * 0x1p15);
+    count[tid] = n;
+  }
+  __syncthreads();
+  if (tid < 64) {     // running sums: four bins a lane
+    uint64_t m[4], before = 0;
+    uint32_t c[4], c_before = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      m[i] = before += mass[4 * tid + i];
+      c[i] = c_before += count[4 * tid + i];
+    }
+    before = wave_scan(before) - before;
+    c_before = wave_scan(c_before) - c_before;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      mass[4 * tid + i] = before + m[i];
+      count[4 * tid + i] = c_before + c[i];
+    }
+  }
+  __syncthreads();
+  // The first bin of which `holds` is true, of every thread's below kBins.
+  auto first = [&](int which, bool holds) {
+    const uint64_t with = __ballot(holds);
+    if (tid < kBins && (tid & 63) == 0)
+      found[which][tid / 64] = with != 0 ? tid + __builtin_ctzll(with) : kBins;
+    __syncthreads();
+    int i = kBins;
+#pragma unroll
+    for (int k = kBins / 64 - 1; k >= 0; k--) i = found[which][k] < kBins ? found[which][k] : i;
+    return i;
+  };
+  Cuts cuts{kBins, kBins, kBins, 0};
+  const uint64_t all = mass[kBins - 1];
+  if (r.top_k > 0) {
+    cuts.k = first(2, tid < kBins && count[tid & (kBins - 1)] >= (uint32_t)r.top_k);
+    if (cuts.k > 0 && cuts.k < kBins) cuts.before = (int)count[cuts.k - 1];
+  }
+  if (r.top_p < 1.0) {
+    const double slack = 0x1p-17 + fabs((double)place) * 0x1p-22;
+    const double least = (double)(cuts.k == kBins ? all : cuts.k == 0 ? 0 : mass[cuts.k - 1]);
+    const double most = (double)(cuts.k == kBins ? all : mass[cuts.k]);
+    const double upto = (double)mass[tid & (kBins - 1)];
+    const int last = min(cuts.k, kBins - 1);
+    cuts.lo = min(first(0, tid < kBins && upto >= r.top_p * least * (1.0 - slack)), last);
+    cuts.hi = min(first(1, tid < kBins && upto >= r.top_p * most * (1.0 + slack)), last);
+  } else if (cuts.k < kBins) {
+    cuts.lo = cuts.hi = cuts.k;
+  }
+  return cuts;
+}
+
+// Step 2, a workgroup a chunk: the weights of the tokens before the bins in
+// question (before lo; before k; before lo and of min_p), and the keys of the
+// tokens in them.
+template <int E>
+DNX_DEV void weigh_chunk(const SampleArgs& a, int row, int chunk) {
+  __shared__ uint64_t part[kWaves];
+  __shared__ uint32_t found;
+  const int tid = threadIdx.x;
+  const float* x = a.logits + row * a.stride;
+  const int j0 = chunk * (kThreads * E) + tid;
+  float l[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int j = j0 + e * kThreads;
+    l[e] = j < a.vocab ? x[j] : -INFINITY;
+  }
+  const Request r = request(a, row);
+  const float top = row_top(a, row);
+  const int64_t at = (int64_t)row * a.chunks + chunk;
+  Cuts cuts{kBins, kBins, kBins, 0};
+  if (top > -INFINITY && r.cut) cuts = find_cuts(a, row, top, r);
+  if (tid == 0) found = 0;
+  __syncthreads();
+  if (chunk == 0 && tid == 0) {
+    int32_t* to = a.cuts + 4 * (int64_t)row;
+    to[0] = cuts.lo, to[1] = cuts.hi, to[2] = cuts.k, to[3] = cuts.before;
+  }
+  const float place = floorf(scaled(top, r.inv));
+  uint64_t before_lo = 0, before_k = 0, kept = 0;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int b = r.cut ? bin_of(l[e], top, place, r.inv) : l[e] > -INFINITY ? 0 : kBins;
+    if (b < cuts.k && b < kBins) {
+      const uint64_t w = weight(l[e], top, r.inv_t);
+      before_k += w;
+      if (b < cuts.lo) {
+        before_lo += w;
+        kept += at_least(w, r);
+      }
+    }
+    if (b < kBins && ((b >= cuts.lo && b <= cuts.hi) || b == cuts.k)) {
+      const uint32_t i = atomicAdd(&found, 1u);
+      if (i < kChunkFound) a.found[at * kChunkFound + i] = order_key(l[e], j0 + e * kThreads);
+    }
+  }
+  before_lo = block_sum(before_lo, part);
+  before_k = block_sum(before_k, part);
+  kept = block_sum(kept, part);
+  if (tid == 0) {
+    a.sums[3 * at] = before_lo;
+    a.sums[3 * at + 1] = before_k;
+    a.sums[3 * at + 2] = kept;
+    a.founds[at] = found;
+  }
+}
+
+// Keys in rising order: N a power of two, those past n above all.
+DNX_DEV void sort_keys(uint64_t* keys, int n) {
+  const int tid = threadIdx.x;
+  if (n <= 128) {           // each to its rank
+    __syncthreads();
+    const uint64_t mine = tid < n ? keys[tid] : 0;
+    int rank = 0;
+    if (tid < n)
+      for (int i = 0; i < n; i++) rank += keys[i] < mine;
+    __syncthreads();
+    if (tid < n) keys[rank] = mine;
+    __syncthreads();
+    return;
+  }
+  int size = 256;
+  while (size < n) size *= 2;
+  for (int i = n + tid; i < size; i += kThreads) keys[i] = ~0ull;
+  for (int k = 2; k <= size; k *= 2)
+    for (int j = k / 2; j > 0; j /= 2) {
+      __syncthreads();
+      for (int t = tid; t < size / 2; t += kThreads) {
+        const int i = 2 * t - (t & (j - 1)), p = i + j;
+        const uint64_t x = keys[i], y = keys[p];
+        if ((x > y) == ((i & k) == 0)) keys[i] = y, keys[p] = x;
+      }
+    }
+  __syncthreads();
+}
+
+// What step 3 keeps in LDS: order keys and the running sums of their weights, or
+// the counts and weights of a span's parts.
+struct PickShared {
+  uint64_t keys[kFound], upto[kFound];
+  uint64_t part[kWaves], ends[2];
+  unsigned long long sums[kMaxChunks];
+  int begin[kMaxChunks + 1], at[2], n;
+};
+
+// n keys of sh.keys in order, and the running sums of their weights.
+DNX_DEV void order_keys(PickShared& sh, int n, float top, const Request& r) {
+  const int tid = threadIdx.x;
+  sort_keys(sh.keys, n);
+  const int per = (n + kThreads - 1) / kThreads;    // in a row a thread
+  uint64_t sum = 0, all;
+  for (int i = tid * per; i < min(n, (tid + 1) * per); i++) {
+    sh.upto[i] = weight(of_key((uint32_t)(sh.keys[i] >> 32)), top, r.inv_t);
+    sum += sh.upto[i];
+  }
+  uint64_t before = block_before(sum, sh.part, all);
+  for (int i = tid * per; i < min(n, (tid + 1) * per); i++) sh.upto[i] = before += sh.upto[i];
+  __syncthreads();
+}
+
+// Of the tokens that `each` gives in bins lo .. hi, the order key of the one of
+// that rank (from 1), or with rank 0 of the first up to which the weights,
+// `before` among them, reach the target. upto: the weights up to it, `before`
+// among them. Where they are too many to be sorted, the span of their keys is
+// cut into parts until the one in question holds few enough: equal logits have
+// different keys. false: the weights do not reach the target here.
+template <typename Each>
+DNX_DEV bool find_key(PickShared& sh, Each each, float top, const Request& r, int lo, int hi,
+                      uint64_t rank, uint64_t target, uint64_t before, uint64_t& key,
+                      uint64_t& upto) {
+  const int tid = threadIdx.x;
+  const float place = floorf(scaled(top, r.inv));
+  uint64_t first = ~0ull, last = 0, n = 0;
+  each([&](uint64_t k) {
+    const int b = bin_of(of_key((uint32_t)(k >> 32)), top, place, r.inv);
+    if (b < lo || b > hi) return;
+    first = k < first ? k : first;
+    last = k > last ? k : last;
+    n++;
+  });
+  n = block_sum(n, sh.part);
+  first = ~wave_max_u64(~first);
+  last = wave_max_u64(last);
+  __syncthreads();
+  if (tid < 2) sh.ends[tid] = tid == 0 ? ~0ull : 0;
+  __syncthreads();
+  if ((tid & 63) == 0) {
+    atomicMin((unsigned long long*)&sh.ends[0], (unsigned long long)first);
+    atomicMax((unsigned long long*)&sh.ends[1], (unsigned long long)last);
+  }
+  __syncthreads();
+  first = sh.ends[0];
+  last = sh.ends[1];
+  if (n == 0) return false;
+  uint32_t* count = (uint32_t*)sh.keys;
+  uint64_t rank_before = 0;
+  while (n > kFound) {
+    const int shift = max(0, 64 - 11 - __builtin_clzll(last - first));
+    __syncthreads();
+    for (int i = tid; i < kParts; i += kThreads) count[i] = 0, sh.upto[i] = 0;
+    __syncthreads();
+    each([&](uint64_t k) {
+      if (k < first || k > last) return;
+      const int i = (int)((k - first) >> shift);
+      atomicAdd(&count[i], 1u);
+      atomicAdd((unsigned long long*)&sh.upto[i],
+                (unsigned long long)weight(of_key((uint32_t)(k >> 32)), top, r.inv_t));
+    });
+    __syncthreads();
+    constexpr int P = kParts / kThreads;
+    uint64_t c[P], w[P], cs = 0, ws = 0, all;
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+      cs += c[i] = count[P * tid + i];
+      ws += w[i] = sh.upto[P * tid + i];
+    }
+    uint64_t cb = block_before(cs, sh.part, all) + rank_before;
+    uint64_t wb = block_before(ws, sh.part, all) + before;
+    if (tid == 0) sh.n = -1;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+      const bool here = rank > 0 ? cb < rank && cb + c[i] >= rank : wb < target && wb + w[i] >= target;
+      if (here) {
+        sh.n = P * tid + i;
+        sh.ends[0] = cb;
+        sh.ends[1] = wb;
+        sh.part[0] = c[i];
+      }
+      cb += c[i];
+      wb += w[i];
+    }
+    __syncthreads();
+    if (sh.n < 0) return false;
+    rank_before = sh.ends[0];
+    before = sh.ends[1];
+    n = sh.part[0];
+    first += (uint64_t)sh.n << shift;
+    const uint64_t width = (1ull << shift) - 1;
+    last = last - first > width ? first + width : last;
+  }
+  __syncthreads();
+  if (tid == 0) sh.n = 0;
+  __syncthreads();
+  each([&](uint64_t k) {
+    const int b = bin_of(of_key((uint32_t)(k >> 32)), top, place, r.inv);
+    if (k < first || k > last || b < lo || b > hi) return;
+    sh.keys[atomicAdd(&sh.n, 1)] = k;
+  });
+  __syncthreads();
+  const int found = sh.n;
+  order_keys(sh, found, top, r);
+  if (tid == 0) sh.at[0] = rank > 0 ? (int)(rank - rank_before) - 1 : kFound;
+  __syncthreads();
+  if (rank == 0)
+    for (int i = tid; i < found; i += kThreads)
+      if (before + sh.upto[i] >= target && (i == 0 || before + sh.upto[i - 1] < target)) sh.at[0] = i;
+  __syncthreads();
+  const int i = sh.at[0];
+  if (i >= found || (rank == 0 && before >= target)) return false;
+  key = sh.keys[i];
+  upto = before + sh.upto[i];
+  __syncthreads();
+  return true;
+}
+
+// Step 3, a workgroup a row: the tokens of the bins in question in order, where
+// among them the cuts lie, the kept weights of each chunk, and the token in its
+// chunk.
+template <int E>
+DNX_DEV void pick(const SampleArgs& a, int row) {
+  constexpr int kChunk = kThreads * E;
+  __shared__ PickShared sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float* x = a.logits + row * a.stride;
+  const int64_t base = (int64_t)row * a.chunks;
+  const float top = row_top(a, row);
+  if (!(top > -INFINITY)) {
     if (tid == 0) a.out[row] = -1;
     return;
   }
-  if (r.greedy) {
-    if (tid == 0) a.out[row] = first;
-    return;
-  }
-  const float top = x[first];
-  Request all = r;
-  all.min_p = 0.0;
-
-  // The last key of the first `tokens` tokens, or of the shortest beginning of
-  // that weight; `within`: among keys up to that one. Its weight too.
-  auto cut = [&](uint64_t within, uint32_t tokens, uint64_t target, uint64_t& weighs) {
-    uint64_t prefix = 0, before = 0;
-    uint32_t n_before = 0;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kThreads) mass[i] = 0, count[i] = 0;
-      __syncthreads();
-      for (int j = tid; j < a.vocab; j += kThreads) {
-        const uint64_t k = (uint64_t)falling_key(x[j]) << 32 | (uint32_t)j;
-        if (k > within || (shift < 56 && (k ^ prefix) >> (shift + 8) != 0)) continue;
-        atomicAdd(&count[k >> shift & 255], 1u);
-        atomicAdd((unsigned long long*)&mass[k >> shift & 255],
-                  (unsigned long long)weight(x[j], top, all));
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int b = 0;
-        uint64_t m = before;
-        uint32_t n = n_before;
-        int last = 0;
-        for (; b < 256; b++) {
-          if (count[b] == 0) continue;
-          last = b;
-          if (tokens > 0 ? n + count[b] >= tokens : m + mass[b] >= target) break;
-          m += mass[b];
-          n += count[b];
-        }
-        if (b == 256) {   // all of them
-          b = last;
-          m -= mass[b];
-          n -= count[b];
-        }
-        found[0] = prefix | (uint64_t)b << shift;
-        found[1] = m;
-        found[2] = n;
-        mass[0] = mass[b];
-      }
-      __syncthreads();
-      prefix = found[0];
-      before = found[1];
-      n_before = (uint32_t)found[2];
-      weighs = before + mass[0];
-      __syncthreads();
+  const Request r = request(a, row);
+  uint64_t before_lo = 0, before_k = 0;
+  for (int c = tid; c < kMaxChunks; c += kThreads) {
+    sh.sums[c] = c < a.chunks ? a.sums[3 * (base + c) + 2] : 0;
+    if (r.cut && c < a.chunks) {
+      before_lo += a.sums[3 * (base + c)];
+      before_k += a.sums[3 * (base + c) + 1];
     }
-    return prefix;
-  };
-
-  uint64_t within = ~0ull, total = 0;
-  if (r.top_k > 0) within = cut(within, (uint32_t)r.top_k, 0, total);
-  if (r.top_p < 1.0) {
-    if (r.top_k == 0) {
-      for (int j = tid; j < a.vocab; j += kThreads) total += weight(x[j], top, all);
-      total = block_sum(total, part);
-    }
-    const double target = ceil(r.top_p * (double)total);
-    within = cut(within, 0, (uint64_t)target, total);
   }
-
-  auto kept = [&](int j) -> uint64_t {
-    if (j >= a.vocab || ((uint64_t)falling_key(x[j]) << 32 | (uint32_t)j) > within) return 0;
-    return weight(x[j], top, r);
-  };
-  total = 0;
-  for (int j = tid; j < a.vocab; j += kThreads) total += kept(j);
-  total = block_sum(total, part);
-  uint64_t target = (uint64_t)((double)r.u * (double)total);
-  target = target < total ? target : total - 1;
-  uint64_t before = 0;
-  for (int j0 = 0; j0 < a.vocab; j0 += kThreads) {
-    const uint64_t w = kept(j0 + tid);
-    uint64_t upto = w;
+  uint64_t within = ~0ull;
+  bool whole = false;       // the chunks' sums have to be formed again
+  const int32_t* cut = a.cuts + 4 * (int64_t)row;
+  const int lo = cut[0], hi = cut[1], bin_k = cut[2], rank_k = r.top_k - cut[3];
+  const float place = floorf(scaled(top, r.inv));
+  if (lo < kBins) {
+    before_lo = block_sum(before_lo, sh.part);
+    before_k = block_sum(before_k, sh.part);
+    if (wave == 0) {        // where each chunk's tokens begin
+      int n[kMaxChunks / 64], sum = 0;
+      bool over = false;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t y = __shfl_up(upto, o);
-      if ((tid & 63) >= o) upto += y;
+      for (int i = 0; i < kMaxChunks / 64; i++) {
+        const int c = kMaxChunks / 64 * lane + i;
+        n[i] = c < a.chunks ? (int)a.founds[base + c] : 0;
+        over |= n[i] > kChunkFound;
+        sum += n[i];
+      }
+      int b = wave_scan(sum) - sum;
+#pragma unroll
+      for (int i = 0; i < kMaxChunks / 64; i++) {
+        sh.begin[kMaxChunks / 64 * lane + i] = b;
+        b += n[i];
+      }
+      over = __any(over);
+      if (lane == 63) sh.begin[kMaxChunks] = over ? -1 : b;
+    }
+    if (tid < 2) sh.at[tid] = kFound;
+    __syncthreads();
+    const int n = sh.begin[kMaxChunks];     // -1: more than a chunk's list holds
+    uint64_t total = before_k;
+    bool done = n > 0 && n <= kFound;
+    if (done) {
+      for (int c = wave; c < a.chunks; c += kWaves) {
+        const int b = sh.begin[c];
+        for (int i = b + lane; i < sh.begin[c + 1]; i += 64)
+          sh.keys[i] = a.found[(base + c) * kChunkFound + i - b];
+      }
+      order_keys(sh, n, top, r);
+      // The first token of bin k, and the last one by rank.
+      auto bin_at = [&](int i) {
+        return bin_of(of_key((uint32_t)(sh.keys[i] >> 32)), top, place, r.inv);
+      };
+      int last = n - 1, end = n;          // end: of the tokens up to bin hi
+      if (bin_k < kBins) {
+        for (int i = tid; i < n; i += kThreads)
+          if (bin_at(i) == bin_k && (i == 0 || bin_at(i - 1) < bin_k)) sh.at[0] = i;
+        __syncthreads();
+        const int first = sh.at[0];
+        last = min(first + rank_k - 1, n - 1);
+        total += sh.upto[last] - (first > 0 ? sh.upto[first - 1] : 0);
+        if (hi < bin_k) end = first;
+      }
+      if (r.top_p < 1.0) {
+        const uint64_t target = max((uint64_t)ceil(r.top_p * (double)total), (uint64_t)1);
+        for (int i = tid; i < end; i += kThreads)
+          if (before_lo + sh.upto[i] >= target && (i == 0 || before_lo + sh.upto[i - 1] < target))
+            sh.at[1] = i;
+        __syncthreads();
+        done = before_lo < target && sh.at[1] < kFound;    // or the bins' weights misled
+        last = min(last, sh.at[1]);
+        total = before_k;
+      }
+      if (done) {
+        within = sh.keys[last];
+        for (int i = tid; i <= last; i += kThreads) {
+          const uint64_t w = at_least(sh.upto[i] - (i > 0 ? sh.upto[i - 1] : 0), r);
+          if (w > 0) atomicAdd(&sh.sums[(uint32_t)sh.keys[i] / kChunk], (unsigned long long)w);
+        }
+      }
+    }
+    if (!done) {
+      whole = n < 0;
+      const auto listed = [&](auto f) {
+        if (n < 0) {
+          for (int j = tid; j < a.vocab; j += kThreads)
+            if (x[j] > -INFINITY) f(order_key(x[j], j));
+        } else {
+          for (int c = wave; c < a.chunks; c += kWaves)
+            for (int i = lane; i < (int)a.founds[base + c]; i += 64)
+              f(a.found[(base + c) * kChunkFound + i]);
+        }
+      };
+      const auto any = [&](auto f) {
+        for (int j = tid; j < a.vocab; j += kThreads)
+          if (x[j] > -INFINITY) f(order_key(x[j], j));
+      };
+      uint64_t key = ~0ull, upto;
+      if (bin_k < kBins &&
+          find_key(sh, listed, top, r, bin_k, bin_k, rank_k, 0, before_k, key, upto)) {
+        within = key;
+        total = upto;
+      }
+      if (r.top_p < 1.0) {
+        const uint64_t target = max((uint64_t)ceil(r.top_p * (double)total), (uint64_t)1);
+        if (!find_key(sh, listed, top, r, lo, hi, 0, target, before_lo, key, upto)) {
+          whole = true;           // the bins' weights misled
+          find_key(sh, any, top, r, 0, kBins - 1, 0, target, 0, key, upto);
+        }
+        within = key < within ? key : within;
+      }
+      for (int c = wave; c < a.chunks && !whole; c += kWaves) {
+        uint64_t s = 0;
+        for (int i = lane; i < (int)a.founds[base + c]; i += 64) {
+          const uint64_t k = a.found[(base + c) * kChunkFound + i];
+          if (k <= within) s += at_least(weight(of_key((uint32_t)(k >> 32)), top, r.inv_t), r);
+        }
+        s = wave_sum_u64(s);
+        if (lane == 0) sh.sums[c] += s;
+      }
+    }
+  }
+  auto kept = [&](int j) -> uint64_t {
+    if (j >= a.vocab) return 0;
+    const float l = x[j];
+    return order_key(l, j) <= within ? at_least(weight(l, top, r.inv_t), r) : 0;
+  };
+  __syncthreads();
+  if (whole) {
+    for (int c = wave; c < a.chunks; c += kWaves) {
+      uint64_t s = 0;
+#pragma unroll 4
+      for (int e = 0; e < kChunk / 64; e++) s += kept(c * kChunk + e * 64 + lane);
+      s = wave_sum_u64(s);
+      if (lane == 0) sh.sums[c] = s;
     }
     __syncthreads();
-    if ((tid & 63) == 63) part[tid >> 6] = upto;
-    __syncthreads();
-    uint64_t at = before;
-    for (int i = 0; i < kWaves; i++) {
-      if (i < tid >> 6) at += part[i];
-      before += part[i];
+  }
+  // The chunk, by every wave alike.
+  uint64_t s[kMaxChunks / 64], mine = 0;
+#pragma unroll
+  for (int i = 0; i < kMaxChunks / 64; i++) mine += s[i] = sh.sums[kMaxChunks / 64 * lane + i];
+  const uint64_t all = wave_scan(mine), total = __shfl(all, 63);
+  uint64_t target = (uint64_t)((double)r.u * (double)total), before = all - mine;
+  target = target < total ? target : total - 1;
+  int chunk = 0;
+  uint64_t chunk_before = 0;
+  bool here = false;
+#pragma unroll
+  for (int i = 0; i < kMaxChunks / 64; i++) {
+    if (before <= target && target < before + s[i]) {
+      here = true;
+      chunk = kMaxChunks / 64 * lane + i;
+      chunk_before = before;
     }
-    upto += at;
-    if (w > 0 && upto > target && upto - w <= target) a.out[row] = j0 + tid;
-    if (before > target) return;
+    before += s[i];
+  }
+  const int from = __builtin_ctzll(__ballot(here));
+  chunk = __shfl(chunk, from);
+  before = __shfl(chunk_before, from);
+  // Its tokens in order: a wave 64 E of them.
+  const int j0 = chunk * kChunk + wave * (64 * E) + lane;
+  uint64_t w[E], of_wave = 0;
+#pragma unroll
+  for (int e = 0; e < E; e++) of_wave += w[e] = kept(j0 + 64 * e);
+  of_wave = wave_sum_u64(of_wave);
+  if (lane == 0) sh.part[wave] = of_wave;
+  __syncthreads();
+  for (int i = 0; i < wave; i++) before += sh.part[i];
+  if (target < before || target >= before + of_wave) return;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const uint64_t to = before + wave_scan(w[e]);
+    if (to > target && to - w[e] <= target) a.out[row] = j0 + 64 * e;
+    before = __shfl(to, 63);
   }
 }
+
+template <int E>
+__global__ void __launch_bounds__(kThreads) count_kernel(SampleArgs a) {
+  count_chunk<E>(a, blockIdx.x, blockIdx.y);
+}
+template <int E>
+__global__ void __launch_bounds__(kThreads) weigh_kernel(SampleArgs a) {
+  weigh_chunk<E>(a, blockIdx.x, blockIdx.y);
+}
+template <int E>
+__global__ void __launch_bounds__(kThreads) pick_kernel(SampleArgs a) {
+  pick<E>(a, blockIdx.x);
+}
+// A row of one chunk: the three steps by one workgroup.
+template <int E>
+__global__ void __launch_bounds__(kThreads) row_kernel(SampleArgs a) {
+  count_chunk<E>(a, blockIdx.x, 0);
+  __syncthreads();
+  weigh_chunk<E>(a, blockIdx.x, 0);
+  __syncthreads();
+  pick<E>(a, blockIdx.x);
+}
+
+// Tokens of a thread in a chunk: 16, or 4 where that leaves CUs without a
+// workgroup.
+int per_thread(int64_t rows, int64_t vocab) {
+  const int64_t chunks = (vocab + 16 * kThreads - 1) / (16 * kThreads);
+  return chunks > 1 && rows * chunks < 256 && vocab <= kMaxChunks * 4 * kThreads ? 4 : 16;
+}
+int64_t chunks_of(int64_t rows, int64_t vocab) {
+  const int64_t chunk = kThreads * per_thread(rows, vocab);
+  return (vocab + chunk - 1) / chunk;
+}
+constexpr int64_t kChunkBytes = 8 * (kBins + 3 + kChunkFound) + 8;
 
 }  // namespace
 
@@ -224,7 +734,7 @@ extern "C" {
 
 int64_t dnx_sample_workspace_bytes(int64_t rows, int64_t vocab) {
   if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab) return -1;
-  return 0;
+  return rows * (chunks_of(rows, vocab) * kChunkBytes + 16);
 }
 
 int dnx_sample(const float* logits, int64_t stride, const float* u, const float* temperature,
@@ -237,13 +747,29 @@ int dnx_sample(const float* logits, int64_t stride, const float* u, const float*
   const uintptr_t all = (uintptr_t)logits | (uintptr_t)u | (uintptr_t)temperature |
                         (uintptr_t)top_k | (uintptr_t)top_p | (uintptr_t)min_p | (uintptr_t)out;
   if (logits == nullptr || u == nullptr || out == nullptr || (all & 3) != 0 || stride < vocab ||
-      stride > (int64_t)1 << 40 || workspace_bytes < need ||
-      (need > 0 && (workspace == nullptr || ((uintptr_t)workspace & 15) != 0))) {
+      stride > (int64_t)1 << 40 || workspace_bytes < need || workspace == nullptr ||
+      ((uintptr_t)workspace & 15) != 0) {
     return DNX_EINVAL;
   }
-  const SampleArgs a{logits, u, temperature, top_p, min_p, top_k, out, stride, (int)vocab};
-  hipLaunchKernelGGL(sample_kernel, dim3((unsigned)rows), dim3(kThreads), 0, (hipStream_t)stream, a);
-  return hipGetLastError() == hipSuccess ? DNX_OK : DNX_ELAUNCH;
+  const int64_t chunks = chunks_of(rows, vocab), n = rows * chunks;
+  SampleArgs a{logits, u, temperature, top_p, min_p, top_k, out, stride, (int)vocab, (int)chunks};
+  a.hist = (uint64_t*)workspace;
+  a.sums = a.hist + n * kBins;
+  a.found = a.sums + 3 * n;
+  a.tops = (float*)(a.found + n * kChunkFound);
+  a.founds = (uint32_t*)(a.tops + n);
+  a.cuts = (int32_t*)(a.founds + n);
+  const bool few = per_thread(rows, vocab) == 4;
+  const hipStream_t st = (hipStream_t)stream;
+  const auto launch = [&](void (*k)(SampleArgs), int64_t y) {
+    hipLaunchKernelGGL(k, dim3((unsigned)rows, (unsigned)y), dim3(kThreads), 0, st, a);
+    return hipGetLastError() == hipSuccess;
+  };
+  if (chunks == 1) return launch(row_kernel<16>, 1) ? DNX_OK : DNX_ELAUNCH;
+  const bool done = launch(few ? count_kernel<4> : count_kernel<16>, chunks) &&
+                    launch(few ? weigh_kernel<4> : weigh_kernel<16>, chunks) &&
+                    launch(few ? pick_kernel<4> : pick_kernel<16>, 1);
+  return done ? DNX_OK : DNX_ELAUNCH;
 }
 
 }  // extern "C"
