@@ -25,10 +25,11 @@ constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int64_t kMaxVocab = 1 << 20;   // the sum of a row's weights is below 2^64
 constexpr int64_t kMaxRows = 1 << 16;
-constexpr int kBins = 256, kBinsPerUnit = 8;   // of l / T: 32 in all
+constexpr int kBins = 1024, kBinsPerUnit = 32;   // of l / T: 32 in all
 constexpr int kMaxChunks = 128;
 constexpr int kChunkFound = 1024;        // tokens of the bins in question, of a chunk
-constexpr int kFound = 4096;             // of a row, that are sorted at once
+constexpr int kListed = 8192;            // of a row, that are held in LDS
+constexpr int kFound = 2048;             // that are sorted at once
 constexpr int kParts = 2048;             // of a span of order keys that holds more
 
 struct SampleArgs {
@@ -36,7 +37,7 @@ struct SampleArgs {
   const int32_t* top_k;
   int32_t* out;
   int64_t stride;
-  int vocab, chunks;
+  int vocab, chunks, wide;   // wide: rows may be read 16 bytes at a time
   // Of each row and chunk:
   uint64_t* hist;      // [kBins]: counts (the upper 16 bits) and weights
   uint64_t* sums;      // [3]: of weights
@@ -48,8 +49,8 @@ struct SampleArgs {
 
 // A row's request. Greedy: of a steep T, the first token.
 struct Request {
-  double inv_t, top_p, min_p;
-  float u, inv;        // inv: of the bins, finite
+  double rate, top_p, min_p;   // rate: log2(e) / T
+  float u, inv;                // inv: 1 / T of the bins, finite
   int top_k;
   bool cut;            // by rank or weight
 };
@@ -61,8 +62,9 @@ DNX_DEV Request request(const SampleArgs& a, int row) {
   const int k = a.top_k != nullptr ? a.top_k[row] : 0;
   const float u = a.u[row];
   const bool greedy = !(t > 0.0f);
-  r.inv_t = greedy ? 0x1p40 : 1.0 / (double)t;
-  r.inv = (float)fmax(fmin(r.inv_t, 1e37), 1e-41);   // an infinity times it is one
+  const double inv = greedy ? 0x1p40 : 1.0 / (double)t;
+  r.rate = inv * 1.4426950408889634;
+  r.inv = (float)fmax(fmin(inv, 1e37), 1e-41);   // an infinity times it is one
   r.top_p = !greedy && p < 1.0f ? fmax((double)p, 0.0) : 1.0;
   r.min_p = !greedy && low > 0.0f ? fmin((double)low, 1.0) : 0.0;
   r.top_k = greedy ? 1 : k > 0 && k < a.vocab ? k : 0;
@@ -84,12 +86,32 @@ DNX_DEV float of_key(uint32_t k) {
 }
 DNX_DEV uint64_t order_key(float v, int j) { return (uint64_t)falling_key(v) << 32 | (uint32_t)j; }
 
-// A token's weight in multiples of 2^-43, and whether that is enough.
-DNX_DEV uint64_t weight(float l, float top, double inv_t) {
-  if (!(l > -INFINITY)) return 0;
-  if (l == top) return 1ull << 43;
-  const double d = ((double)l - (double)top) * inv_t;
-  return d > -31.0 ? (uint64_t)(exp(d) * 0x1p43 + 0.5) : 0;
+// A token's weight in multiples of 2^-43, and whether that is enough. 2^x by the
+// Taylor series about the nearest whole number: |z| <= ln 2 / 2, whose 12th term
+// is below 2^-47. Adding 3 2^51 rounds to a whole number and leaves it in the lower
+// bits, adding 2^52 rounds the result: conversions between 64 bits and whole
+// numbers run at a quarter of the rate.
+DNX_DEV uint64_t weight(float l, float top, double rate) {
+  const double x = ((double)l - (double)top) * rate, m = x + 0x1.8p52;
+  const double z = (x - (m - 0x1.8p52)) * 0.6931471805599453;
+  double p = 1.0 / 39916800.0;
+  p = fma(p, z, 1.0 / 3628800.0);
+  p = fma(p, z, 1.0 / 362880.0);
+  p = fma(p, z, 1.0 / 40320.0);
+  p = fma(p, z, 1.0 / 5040.0);
+  p = fma(p, z, 1.0 / 720.0);
+  p = fma(p, z, 1.0 / 120.0);
+  p = fma(p, z, 1.0 / 24.0);
+  p = fma(p, z, 1.0 / 6.0);
+  p = fma(p, z, 0.5);
+  p = fma(p, z, 1.0);
+  p = fma(p, z, 1.0);
+  const bool some = x > -45.0 && l > -INFINITY;      // no NaN, no exponent out of range
+  const int n = some ? (int)(uint32_t)__builtin_bit_cast(uint64_t, m) : 0;
+  const double w = __builtin_bit_cast(
+      double, __builtin_bit_cast(uint64_t, p) + ((uint64_t)(uint32_t)(n + 43) << 52));
+  const uint64_t whole = __builtin_bit_cast(uint64_t, w + 0x1p52) & ((1ull << 52) - 1);
+  return l == top ? (l > -INFINITY ? 1ull << 43 : 0) : some ? whole : 0;
 }
 DNX_DEV uint64_t at_least(uint64_t w, const Request& r) {
   return (double)w >= r.min_p * 0x1p43 ? w : 0;
@@ -159,6 +181,27 @@ DNX_DEV float row_top(const SampleArgs& a, int row) {
   return wave_max_dpp(top);
 }
 
+// A chunk's logits: a thread has four in a row of each 4 kThreads.
+template <int E>
+DNX_DEV int index_of(int chunk, int e) {
+  return chunk * (kThreads * E) + e / 4 * (4 * kThreads) + 4 * threadIdx.x + e % 4;
+}
+template <int E>
+DNX_DEV void load_chunk(const SampleArgs& a, int row, int chunk, float* l) {
+  const float* x = a.logits + row * a.stride;
+#pragma unroll
+  for (int e = 0; e < E; e += 4) {
+    const int j = index_of<E>(chunk, e);
+    if (a.wide && j + 3 < a.vocab) {
+      const float4 v = *(const float4*)(x + j);
+      l[e] = v.x, l[e + 1] = v.y, l[e + 2] = v.z, l[e + 3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) l[e + i] = j + i < a.vocab ? x[j + i] : -INFINITY;
+    }
+  }
+}
+
 // ---- Step 1, a workgroup a chunk of a row: its largest logit, and (for a row
 // that is cut) how many tokens and how much weight each bin holds, the weights
 // relative to the bin's lower end.
@@ -167,16 +210,10 @@ DNX_DEV void count_chunk(const SampleArgs& a, int row, int chunk) {
   __shared__ unsigned long long hist[kBins];
   __shared__ float part[kWaves];
   const int tid = threadIdx.x;
-  const float* x = a.logits + row * a.stride;
-  const int j0 = chunk * (kThreads * E) + tid;
   float l[E];
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const int j = j0 + e * kThreads;
-    l[e] = j < a.vocab ? x[j] : -INFINITY;
-  }
+  load_chunk<E>(a, row, chunk, l);
   const Request r = request(a, row);
-  if (tid < kBins) hist[tid] = 0;
+  for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
   float top = -INFINITY;
 #pragma unroll
   for (int e = 0; e < E; e++) top = fmaxf(top, l[e]);
@@ -199,95 +236,104 @@ DNX_DEV void count_chunk(const SampleArgs& a, int row, int chunk) {
     }
   }
   __syncthreads();
-  if (tid < kBins) a.hist[at * kBins + tid] = hist[tid];
+  for (int i = tid; i < kBins; i += kThreads) a.hist[at * kBins + i] = hist[i];
 }
 
-// The bins in question: cuts lie in bins lo .. hi (by weight) and k (by rank),
-// lo <= hi <= k; before: tokens before bin k. Without a cut lo = kBins.
-struct Cuts {
-  int lo, hi, k, before;
-};
+// a.cuts: the cut by weight lies in bins lo .. hi, that by rank in bin k, before
+// which there are so many tokens; lo <= hi <= k, which is kBins without one. Without
+// either lo is kBins too.
 
-// Step 2 begins with them, in each of a row's workgroups: its chunks' bins added,
-// and their running sums. The weights of bins are off by 2^-22 or, for large l /
-// T, by the rounding of that; where a cut by weight may lie takes this in.
-DNX_DEV Cuts find_cuts(const SampleArgs& a, int row, float top, const Request& r) {
-  __shared__ uint64_t mass[kThreads];
-  __shared__ uint32_t count[kThreads];
-  __shared__ int32_t found[3][kBins / 64];
-  const int tid = threadIdx.x, b = tid % kBins;
-  const float place = floorf(scaled(top, r.inv));
-  uint64_t w = 0;
-  uint32_t n = 0;
-  for (int c = tid / kBins; c < a.chunks; c += kThreads / kBins) {
-    const int64_t at = (int64_t)row * a.chunks + c;
-    const float mine = a.tops[at];
-    const float d = mine == top ? 0.0f : place - floorf(scaled(mine, r.inv));
-    const int i = mine > -INFINITY && d < (float)kBins ? b - (int)fmaxf(d, 0.0f) : -1;
-    if (i < 0) continue;
-    const uint64_t h = a.hist[at * kBins + i];
-    w += h & ((1ull << 48) - 1);
-    n += (uint32_t)(h >> 48);
-  }
-  mass[tid] = w;
-  count[tid] = n;
-  __syncthreads();
-  if (tid < kBins) {
-    for (int k = tid + kBins; k < kThreads; k += kBins) w += mass[k], n += count[k];
-    // Below 2^(26 + 20 + 1): in whole multiples, whose running sums rise.
-    mass[tid] = (uint64_t)((double)w * exp((double)tid * (-1.0 / kBinsPerUnit)) * 0x1p15);
-    count[tid] = n;
-  }
-  __syncthreads();
-  if (tid < 64) {     // running sums: four bins a lane
-    uint64_t m[4], before = 0;
-    uint32_t c[4], c_before = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      m[i] = before += mass[4 * tid + i];
-      c[i] = c_before += count[4 * tid + i];
-    }
-    before = wave_scan(before) - before;
-    c_before = wave_scan(c_before) - c_before;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      mass[4 * tid + i] = before + m[i];
-      count[4 * tid + i] = c_before + c[i];
-    }
-  }
-  __syncthreads();
-  // The first bin of which `holds` is true, of every thread's below kBins.
-  auto first = [&](int which, bool holds) {
-    const uint64_t with = __ballot(holds);
-    if (tid < kBins && (tid & 63) == 0)
-      found[which][tid / 64] = with != 0 ? tid + __builtin_ctzll(with) : kBins;
+// Step 2, a workgroup a row: its chunks' bins added, their running sums, and where
+// these reach the cuts. The weights of bins are off by 2^-22 or, for large l / T,
+// by the rounding of that; where a cut by weight may lie takes this in.
+DNX_DEV void find_cuts(const SampleArgs& a, int row) {
+  constexpr int P = kBins / kThreads, U = 8;       // bins a thread, chunks at once
+  __shared__ uint64_t mass[kBins];
+  __shared__ uint32_t count[kBins];
+  __shared__ uint64_t part[kWaves];
+  __shared__ int32_t shift[kMaxChunks], found[3];
+  const int tid = threadIdx.x;
+  const int64_t base = (int64_t)row * a.chunks;
+  const float mine = tid < a.chunks ? a.tops[base + tid] : -INFINITY;
+  const Request r = request(a, row);
+  const float top = row_top(a, row);
+  int lo = kBins, hi = kBins, bin_k = kBins, before_k = 0;
+  if (r.cut && top > -INFINITY) {
+    const float place = floorf(scaled(top, r.inv));
+    if (tid < kMaxChunks) shift[tid] = bin_of(mine, top, place, r.inv);   // a chunk's first bin
+    if (tid < 3) found[tid] = kBins;
     __syncthreads();
-    int i = kBins;
+    uint64_t w[P] = {};
+    uint32_t n[P] = {};
+    for (int c0 = 0; c0 < a.chunks; c0 += U) {
+      uint64_t h[U][P];
 #pragma unroll
-    for (int k = kBins / 64 - 1; k >= 0; k--) i = found[which][k] < kBins ? found[which][k] : i;
-    return i;
-  };
-  Cuts cuts{kBins, kBins, kBins, 0};
-  const uint64_t all = mass[kBins - 1];
-  if (r.top_k > 0) {
-    cuts.k = first(2, tid < kBins && count[tid & (kBins - 1)] >= (uint32_t)r.top_k);
-    if (cuts.k > 0 && cuts.k < kBins) cuts.before = (int)count[cuts.k - 1];
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int k = 0; k < P; k++) {
+          const int i = c0 + u < a.chunks ? P * tid + k - shift[c0 + u] : -1;
+          h[u][k] = a.hist[(base + (i < 0 ? 0 : c0 + u)) * kBins + (i < 0 ? 0 : i)];
+          h[u][k] = i < 0 ? 0 : h[u][k];
+        }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int k = 0; k < P; k++) {
+          w[k] += h[u][k] & ((1ull << 48) - 1);
+          n[k] += (uint32_t)(h[u][k] >> 48);
+        }
+    }
+    // Below 2^(26 + 20 + 1): in whole multiples, whose running sums rise.
+    uint64_t ws = 0, ns = 0, all, tokens;
+#pragma unroll
+    for (int k = 0; k < P; k++) {
+      w[k] = (uint64_t)((double)w[k] * exp((double)(P * tid + k) * (-1.0 / kBinsPerUnit)) * 0x1p15);
+      ws += w[k];
+      ns += n[k];
+    }
+    uint64_t wb = block_before(ws, part, all), nb = block_before(ns, part, tokens);
+#pragma unroll
+    for (int k = 0; k < P; k++) {
+      mass[P * tid + k] = wb += w[k];
+      count[P * tid + k] = (uint32_t)(nb += n[k]);
+    }
+    __syncthreads();
+    if (r.top_k > 0) {
+#pragma unroll
+      for (int k = P - 1; k >= 0; k--) {
+        const int b = P * tid + k;
+        if (count[b] >= (uint32_t)r.top_k && (b == 0 || count[b - 1] < (uint32_t)r.top_k)) found[2] = b;
+      }
+      __syncthreads();
+      bin_k = found[2];
+      if (bin_k > 0 && bin_k < kBins) before_k = (int)count[bin_k - 1];
+      lo = hi = bin_k;
+    }
+    if (r.top_p < 1.0) {
+      const double slack = 0x1p-17 + fabs((double)place) * 0x1p-27;
+      const double least = (double)(bin_k == kBins ? all : bin_k == 0 ? 0 : mass[bin_k - 1]);
+      const double most = (double)(bin_k == kBins ? all : mass[bin_k]);
+      const double from = r.top_p * least * (1.0 - slack), to = r.top_p * most * (1.0 + slack);
+#pragma unroll
+      for (int k = 0; k < P; k++) {
+        const int b = P * tid + k;
+        const double upto = (double)mass[b], before = b == 0 ? -1.0 : (double)mass[b - 1];
+        if (upto >= from && before < from) found[0] = b;
+        if (upto >= to && before < to) found[1] = b;
+      }
+      __syncthreads();
+      const int last = min(bin_k, kBins - 1);
+      lo = min(found[0], last);
+      hi = min(found[1], last);
+    }
   }
-  if (r.top_p < 1.0) {
-    const double slack = 0x1p-17 + fabs((double)place) * 0x1p-22;
-    const double least = (double)(cuts.k == kBins ? all : cuts.k == 0 ? 0 : mass[cuts.k - 1]);
-    const double most = (double)(cuts.k == kBins ? all : mass[cuts.k]);
-    const double upto = (double)mass[tid & (kBins - 1)];
-    const int last = min(cuts.k, kBins - 1);
-    cuts.lo = min(first(0, tid < kBins && upto >= r.top_p * least * (1.0 - slack)), last);
-    cuts.hi = min(first(1, tid < kBins && upto >= r.top_p * most * (1.0 + slack)), last);
-  } else if (cuts.k < kBins) {
-    cuts.lo = cuts.hi = cuts.k;
+  if (tid == 0) {
+    int32_t* to = a.cuts + 4 * (int64_t)row;
+    to[0] = lo, to[1] = hi, to[2] = bin_k, to[3] = before_k;
   }
-  return cuts;
 }
 
-// Step 2, a workgroup a chunk: the weights of the tokens before the bins in
+// Step 3, a workgroup a chunk: the weights of the tokens before the bins in
 // question (before lo; before k; before lo and of min_p), and the keys of the
 // tokens in them.
 template <int E>
@@ -295,46 +341,38 @@ DNX_DEV void weigh_chunk(const SampleArgs& a, int row, int chunk) {
   __shared__ uint64_t part[kWaves];
   __shared__ uint32_t found;
   const int tid = threadIdx.x;
-  const float* x = a.logits + row * a.stride;
-  const int j0 = chunk * (kThreads * E) + tid;
   float l[E];
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const int j = j0 + e * kThreads;
-    l[e] = j < a.vocab ? x[j] : -INFINITY;
-  }
+  load_chunk<E>(a, row, chunk, l);
+  const int32_t* cut = a.cuts + 4 * (int64_t)row;
+  const int lo = cut[0], hi = cut[1], bin_k = cut[2];
   const Request r = request(a, row);
   const float top = row_top(a, row);
   const int64_t at = (int64_t)row * a.chunks + chunk;
-  Cuts cuts{kBins, kBins, kBins, 0};
-  if (top > -INFINITY && r.cut) cuts = find_cuts(a, row, top, r);
   if (tid == 0) found = 0;
   __syncthreads();
-  if (chunk == 0 && tid == 0) {
-    int32_t* to = a.cuts + 4 * (int64_t)row;
-    to[0] = cuts.lo, to[1] = cuts.hi, to[2] = cuts.k, to[3] = cuts.before;
-  }
   const float place = floorf(scaled(top, r.inv));
   uint64_t before_lo = 0, before_k = 0, kept = 0;
 #pragma unroll
   for (int e = 0; e < E; e++) {
     const int b = r.cut ? bin_of(l[e], top, place, r.inv) : l[e] > -INFINITY ? 0 : kBins;
-    if (b < cuts.k && b < kBins) {
-      const uint64_t w = weight(l[e], top, r.inv_t);
+    if (b < bin_k) {
+      const uint64_t w = weight(l[e], top, r.rate);
       before_k += w;
-      if (b < cuts.lo) {
+      if (b < lo) {
         before_lo += w;
         kept += at_least(w, r);
       }
     }
-    if (b < kBins && ((b >= cuts.lo && b <= cuts.hi) || b == cuts.k)) {
+    if (b < kBins && ((b >= lo && b <= hi) || b == bin_k)) {
       const uint32_t i = atomicAdd(&found, 1u);
-      if (i < kChunkFound) a.found[at * kChunkFound + i] = order_key(l[e], j0 + e * kThreads);
+      if (i < kChunkFound) a.found[at * kChunkFound + i] = order_key(l[e], index_of<E>(chunk, e));
     }
   }
-  before_lo = block_sum(before_lo, part);
-  before_k = block_sum(before_k, part);
   kept = block_sum(kept, part);
+  if (r.cut) {
+    before_lo = block_sum(before_lo, part);
+    before_k = block_sum(before_k, part);
+  }
   if (tid == 0) {
     a.sums[3 * at] = before_lo;
     a.sums[3 * at + 1] = before_k;
@@ -372,10 +410,12 @@ DNX_DEV void sort_keys(uint64_t* keys, int n) {
   __syncthreads();
 }
 
-// What step 3 keeps in LDS: order keys and the running sums of their weights, or
-// the counts and weights of a span's parts.
+// What step 4 keeps in LDS: the order keys of the bins in question, those of them
+// that are sorted, and the running sums of their weights, or the counts and weights
+// of a span's parts.
+static_assert(kFound <= kParts, "upto serves both");
 struct PickShared {
-  uint64_t keys[kFound], upto[kFound];
+  uint64_t list[kListed], keys[kFound], upto[kParts];
   uint64_t part[kWaves], ends[2];
   unsigned long long sums[kMaxChunks];
   int begin[kMaxChunks + 1], at[2], n;
@@ -388,7 +428,7 @@ DNX_DEV void order_keys(PickShared& sh, int n, float top, const Request& r) {
   const int per = (n + kThreads - 1) / kThreads;    // in a row a thread
   uint64_t sum = 0, all;
   for (int i = tid * per; i < min(n, (tid + 1) * per); i++) {
-    sh.upto[i] = weight(of_key((uint32_t)(sh.keys[i] >> 32)), top, r.inv_t);
+    sh.upto[i] = weight(of_key((uint32_t)(sh.keys[i] >> 32)), top, r.rate);
     sum += sh.upto[i];
   }
   uint64_t before = block_before(sum, sh.part, all);
@@ -442,7 +482,7 @@ DNX_DEV bool find_key(PickShared& sh, Each each, float top, const Request& r, in
       const int i = (int)((k - first) >> shift);
       atomicAdd(&count[i], 1u);
       atomicAdd((unsigned long long*)&sh.upto[i],
-                (unsigned long long)weight(of_key((uint32_t)(k >> 32)), top, r.inv_t));
+                (unsigned long long)weight(of_key((uint32_t)(k >> 32)), top, r.rate));
     });
     __syncthreads();
     constexpr int P = kParts / kThreads;
@@ -502,7 +542,7 @@ DNX_DEV bool find_key(PickShared& sh, Each each, float top, const Request& r, in
   return true;
 }
 
-// Step 3, a workgroup a row: the tokens of the bins in question in order, where
+// Step 4, a workgroup a row: the tokens of the bins in question in order, where
 // among them the cuts lie, the kept weights of each chunk, and the token in its
 // chunk.
 template <int E>
@@ -558,12 +598,23 @@ DNX_DEV void pick(const SampleArgs& a, int row) {
     const int n = sh.begin[kMaxChunks];     // -1: more than a chunk's list holds
     uint64_t total = before_k;
     bool done = n > 0 && n <= kFound;
-    if (done) {
+    if (n > 0 && n <= kListed) {
+      uint64_t* to = done ? sh.keys : sh.list;
       for (int c = wave; c < a.chunks; c += kWaves) {
-        const int b = sh.begin[c];
-        for (int i = b + lane; i < sh.begin[c + 1]; i += 64)
-          sh.keys[i] = a.found[(base + c) * kChunkFound + i - b];
+        const int b = sh.begin[c], m = sh.begin[c + 1] - b;
+        const uint64_t* from = a.found + (base + c) * kChunkFound;
+        for (int i0 = 0; i0 < m; i0 += 256) {
+          uint64_t k[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++) k[u] = from[min(i0 + 64 * u + lane, m - 1)];
+#pragma unroll
+          for (int u = 0; u < 4; u++)
+            if (i0 + 64 * u + lane < m) to[b + i0 + 64 * u + lane] = k[u];
+        }
       }
+      __syncthreads();
+    }
+    if (done) {
       order_keys(sh, n, top, r);
       // The first token of bin k, and the last one by rank.
       auto bin_at = [&](int i) {
@@ -598,20 +649,20 @@ DNX_DEV void pick(const SampleArgs& a, int row) {
       }
     }
     if (!done) {
-      whole = n < 0;
-      const auto listed = [&](auto f) {
-        if (n < 0) {
-          for (int j = tid; j < a.vocab; j += kThreads)
-            if (x[j] > -INFINITY) f(order_key(x[j], j));
-        } else {
-          for (int c = wave; c < a.chunks; c += kWaves)
-            for (int i = lane; i < (int)a.founds[base + c]; i += 64)
-              f(a.found[(base + c) * kChunkFound + i]);
+      whole = n <= 0 || n > kListed;
+      const auto any = [&](auto f) {
+        for (int j0 = tid; j0 < a.vocab; j0 += 8 * kThreads) {
+          float l[8];
+#pragma unroll
+          for (int u = 0; u < 8; u++) l[u] = x[min(j0 + u * kThreads, a.vocab - 1)];
+#pragma unroll
+          for (int u = 0; u < 8; u++)
+            if (j0 + u * kThreads < a.vocab && l[u] > -INFINITY) f(order_key(l[u], j0 + u * kThreads));
         }
       };
-      const auto any = [&](auto f) {
-        for (int j = tid; j < a.vocab; j += kThreads)
-          if (x[j] > -INFINITY) f(order_key(x[j], j));
+      const auto listed = [&](auto f) {
+        if (whole) return any(f);
+        for (int i = tid; i < n; i += kThreads) f(sh.list[i]);
       };
       uint64_t key = ~0ull, upto;
       if (bin_k < kBins &&
@@ -629,9 +680,9 @@ DNX_DEV void pick(const SampleArgs& a, int row) {
       }
       for (int c = wave; c < a.chunks && !whole; c += kWaves) {
         uint64_t s = 0;
-        for (int i = lane; i < (int)a.founds[base + c]; i += 64) {
-          const uint64_t k = a.found[(base + c) * kChunkFound + i];
-          if (k <= within) s += at_least(weight(of_key((uint32_t)(k >> 32)), top, r.inv_t), r);
+        for (int i = sh.begin[c] + lane; i < sh.begin[c + 1]; i += 64) {
+          const uint64_t k = sh.list[i];
+          if (k <= within) s += at_least(weight(of_key((uint32_t)(k >> 32)), top, r.rate), r);
         }
         s = wave_sum_u64(s);
         if (lane == 0) sh.sums[c] += s;
@@ -641,7 +692,7 @@ DNX_DEV void pick(const SampleArgs& a, int row) {
   auto kept = [&](int j) -> uint64_t {
     if (j >= a.vocab) return 0;
     const float l = x[j];
-    return order_key(l, j) <= within ? at_least(weight(l, top, r.inv_t), r) : 0;
+    return order_key(l, j) <= within ? at_least(weight(l, top, r.rate), r) : 0;
   };
   __syncthreads();
   if (whole) {
@@ -698,6 +749,9 @@ template <int E>
 __global__ void __launch_bounds__(kThreads) count_kernel(SampleArgs a) {
   count_chunk<E>(a, blockIdx.x, blockIdx.y);
 }
+__global__ void __launch_bounds__(kThreads) cuts_kernel(SampleArgs a) {
+  find_cuts(a, blockIdx.x);
+}
 template <int E>
 __global__ void __launch_bounds__(kThreads) weigh_kernel(SampleArgs a) {
   weigh_chunk<E>(a, blockIdx.x, blockIdx.y);
@@ -706,10 +760,12 @@ template <int E>
 __global__ void __launch_bounds__(kThreads) pick_kernel(SampleArgs a) {
   pick<E>(a, blockIdx.x);
 }
-// A row of one chunk: the three steps by one workgroup.
+// A row of one chunk: the steps by one workgroup.
 template <int E>
 __global__ void __launch_bounds__(kThreads) row_kernel(SampleArgs a) {
   count_chunk<E>(a, blockIdx.x, 0);
+  __syncthreads();
+  find_cuts(a, blockIdx.x);
   __syncthreads();
   weigh_chunk<E>(a, blockIdx.x, 0);
   __syncthreads();
@@ -752,7 +808,8 @@ int dnx_sample(const float* logits, int64_t stride, const float* u, const float*
     return DNX_EINVAL;
   }
   const int64_t chunks = chunks_of(rows, vocab), n = rows * chunks;
-  SampleArgs a{logits, u, temperature, top_p, min_p, top_k, out, stride, (int)vocab, (int)chunks};
+  SampleArgs a{logits, u, temperature, top_p, min_p, top_k, out, stride, (int)vocab, (int)chunks,
+               ((uintptr_t)logits & 15) == 0 && (stride % 4 == 0 || rows == 1)};
   a.hist = (uint64_t*)workspace;
   a.sums = a.hist + n * kBins;
   a.found = a.sums + 3 * n;
@@ -767,6 +824,7 @@ int dnx_sample(const float* logits, int64_t stride, const float* u, const float*
   };
   if (chunks == 1) return launch(row_kernel<16>, 1) ? DNX_OK : DNX_ELAUNCH;
   const bool done = launch(few ? count_kernel<4> : count_kernel<16>, chunks) &&
+                    launch(cuts_kernel, 1) &&
                     launch(few ? weigh_kernel<4> : weigh_kernel<16>, chunks) &&
                     launch(few ? pick_kernel<4> : pick_kernel<16>, 1);
   return done ? DNX_OK : DNX_ELAUNCH;
