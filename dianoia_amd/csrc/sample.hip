@@ -12,6 +12,8 @@
 // Weights are whole multiples of 2^-43, formed in 64 bits: whole numbers' sums
 // do not depend on their order, whatever deals them to threads.
 
+#include <algorithm>
+
 #include "common.h"
 #include "dnx_kernels.h"
 
@@ -27,9 +29,9 @@ constexpr int64_t kMaxVocab = 1 << 20;   // the sum of a row's weights is below 
 constexpr int64_t kMaxRows = 1 << 16;
 constexpr int kBins = 1024, kBinsPerUnit = 32;   // of l / T: 32 in all
 constexpr int kMaxChunks = 128;
-constexpr int kChunkFound = 1024;        // tokens of the bins in question, of a chunk
+constexpr int kMaxUnits = 1024;
 constexpr int kListed = 8192;            // of a row, that are held in LDS
-constexpr int kFound = 2048;             // that are sorted at once
+constexpr int kFound = 256;              // that are sorted at once
 constexpr int kParts = 2048;             // of a span of order keys that holds more
 
 struct SampleArgs {
@@ -37,19 +39,21 @@ struct SampleArgs {
   const int32_t* top_k;
   int32_t* out;
   int64_t stride;
-  int vocab, chunks, wide;   // wide: rows may be read 16 bytes at a time
-  // Of each row and chunk:
+  int vocab, chunks, units, wide;   // wide: rows may be read 16 bytes at a time
+  // Of each row and chunk (a workgroup's tokens in the first step):
   uint64_t* hist;      // [kBins]: counts (the upper 16 bits) and weights
-  uint64_t* sums;      // [3]: of weights
-  uint64_t* found;     // [kChunkFound] order keys
   float* tops;         // the largest logit
-  uint32_t* founds;    // how many tokens were found
   int32_t* cuts;       // [4] of each row: the bins in question
+  // Of each row and unit (a wave's tokens in the third):
+  uint64_t* sums;      // [3]: of weights
+  uint64_t* found;     // [unit_found(E)] order keys
+  uint32_t* founds;    // how many tokens were found
 };
 
 // A row's request. Greedy: of a steep T, the first token.
 struct Request {
-  double rate, top_p, min_p;   // rate: log2(e) / T
+  double rate, top_p;          // rate: log2(e) / T
+  uint64_t least;              // min_p in weights
   float u, inv;                // inv: 1 / T of the bins, finite
   int top_k;
   bool cut;            // by rank or weight
@@ -66,7 +70,7 @@ DNX_DEV Request request(const SampleArgs& a, int row) {
   r.rate = inv * 1.4426950408889634;
   r.inv = (float)fmax(fmin(inv, 1e37), 1e-41);   // an infinity times it is one
   r.top_p = !greedy && p < 1.0f ? fmax((double)p, 0.0) : 1.0;
-  r.min_p = !greedy && low > 0.0f ? fmin((double)low, 1.0) : 0.0;
+  r.least = !greedy && low > 0.0f ? (uint64_t)ceil(fmin((double)low, 1.0) * 0x1p43) : 0;
   r.top_k = greedy ? 1 : k > 0 && k < a.vocab ? k : 0;
   r.u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
   r.cut = r.top_k > 0 || r.top_p < 1.0;
@@ -86,13 +90,13 @@ DNX_DEV float of_key(uint32_t k) {
 }
 DNX_DEV uint64_t order_key(float v, int j) { return (uint64_t)falling_key(v) << 32 | (uint32_t)j; }
 
-// A token's weight in multiples of 2^-43, and whether that is enough. 2^x by the
+// A token's weight in multiples of 2^-43, and if that is enough for min_p. 2^x by the
 // Taylor series about the nearest whole number: |z| <= ln 2 / 2, whose 12th term
 // is below 2^-47. Adding 3 2^51 rounds to a whole number and leaves it in the lower
 // bits, adding 2^52 rounds the result: conversions between 64 bits and whole
 // numbers run at a quarter of the rate.
 DNX_DEV uint64_t weight(float l, float top, double rate) {
-  const double x = ((double)l - (double)top) * rate, m = x + 0x1.8p52;
+  const double d = ((double)l - (double)top) * rate, x = l == top ? 0.0 : d, m = x + 0x1.8p52;
   const double z = (x - (m - 0x1.8p52)) * 0.6931471805599453;
   double p = 1.0 / 39916800.0;
   p = fma(p, z, 1.0 / 3628800.0);
@@ -106,16 +110,14 @@ DNX_DEV uint64_t weight(float l, float top, double rate) {
   p = fma(p, z, 0.5);
   p = fma(p, z, 1.0);
   p = fma(p, z, 1.0);
-  const bool some = x > -45.0 && l > -INFINITY;      // no NaN, no exponent out of range
-  const int n = some ? (int)(uint32_t)__builtin_bit_cast(uint64_t, m) : 0;
+  const bool some = x > -45.0;      // no NaN (of -inf - -inf too), no exponent out of range
+  const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, m);
   const double w = __builtin_bit_cast(
-      double, __builtin_bit_cast(uint64_t, p) + ((uint64_t)(uint32_t)(n + 43) << 52));
+      double, __builtin_bit_cast(uint64_t, p) + ((uint64_t)(uint32_t)(some ? n + 43 : 0) << 52));
   const uint64_t whole = __builtin_bit_cast(uint64_t, w + 0x1p52) & ((1ull << 52) - 1);
-  return l == top ? (l > -INFINITY ? 1ull << 43 : 0) : some ? whole : 0;
+  return some ? whole : 0;
 }
-DNX_DEV uint64_t at_least(uint64_t w, const Request& r) {
-  return (double)w >= r.min_p * 0x1p43 ? w : 0;
-}
+DNX_DEV uint64_t at_least(uint64_t w, const Request& r) { return w >= r.least ? w : 0; }
 
 // Bins of l / T, an eighth wide: whole numbers that do not fall as logits rise,
 // the same for every chunk of a row. Far-off values are as the last ones (no
@@ -131,21 +133,29 @@ DNX_DEV int bin_of(float l, float top, float place, float inv) {
   return l > -INFINITY && d < (float)kBins ? (int)fmaxf(d, 0.0f) : kBins;
 }
 
-DNX_DEV uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+// Running sums over a wave by DPP: within rows of 16 lanes, then the last lane of
+// a row into the next one's, and of the first half into the second's.
+template <int Ctrl, int Rows>
+DNX_DEV uint64_t dpp_or_0(uint64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, Ctrl, Rows, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), Ctrl, Rows, 0xf, false);
+  return (uint64_t)hi << 32 | lo;
+}
+DNX_DEV uint64_t wave_scan(uint64_t v) {   // inclusive
+  constexpr int kShr = 0x110, kBcast15 = 0x142, kBcast31 = 0x143;
+  v += dpp_or_0<kShr + 1, 0xf>(v);
+  v += dpp_or_0<kShr + 2, 0xf>(v);
+  v += dpp_or_0<kShr + 4, 0xf>(v);
+  v += dpp_or_0<kShr + 8, 0xf>(v);
+  v += dpp_or_0<kBcast15, 0xa>(v);
+  v += dpp_or_0<kBcast31, 0xc>(v);
   return v;
 }
-template <typename V>
-DNX_DEV V wave_scan(V v) {   // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const V y = __shfl_up(v, o);
-    if (lane >= o) v += y;
-  }
-  return v;
+DNX_DEV uint64_t lane_value(uint64_t v, int lane) {
+  const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | lo;
 }
+DNX_DEV uint64_t wave_sum_u64(uint64_t v) { return lane_value(wave_scan(v), 63); }
 
 // The workgroup's sum, in every thread.
 DNX_DEV uint64_t block_sum(uint64_t v, uint64_t* part) {
@@ -181,17 +191,17 @@ DNX_DEV float row_top(const SampleArgs& a, int row) {
   return wave_max_dpp(top);
 }
 
-// A chunk's logits: a thread has four in a row of each 4 kThreads.
-template <int E>
-DNX_DEV int index_of(int chunk, int e) {
-  return chunk * (kThreads * E) + e / 4 * (4 * kThreads) + 4 * threadIdx.x + e % 4;
+// Logits of `threads` threads from token j0 on, E each: of each 4 threads tokens
+// four in a row a thread.
+DNX_DEV int index_of(int j0, int thread, int threads, int e) {
+  return j0 + e / 4 * (4 * threads) + 4 * thread + e % 4;
 }
 template <int E>
-DNX_DEV void load_chunk(const SampleArgs& a, int row, int chunk, float* l) {
+DNX_DEV void load_logits(const SampleArgs& a, int row, int j0, int thread, int threads, float* l) {
   const float* x = a.logits + row * a.stride;
 #pragma unroll
   for (int e = 0; e < E; e += 4) {
-    const int j = index_of<E>(chunk, e);
+    const int j = index_of(j0, thread, threads, e);
     if (a.wide && j + 3 < a.vocab) {
       const float4 v = *(const float4*)(x + j);
       l[e] = v.x, l[e + 1] = v.y, l[e + 2] = v.z, l[e + 3] = v.w;
@@ -211,7 +221,7 @@ DNX_DEV void count_chunk(const SampleArgs& a, int row, int chunk) {
   __shared__ float part[kWaves];
   const int tid = threadIdx.x;
   float l[E];
-  load_chunk<E>(a, row, chunk, l);
+  load_logits<E>(a, row, chunk * kThreads * E, tid, kThreads, l);
   const Request r = request(a, row);
   for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
   float top = -INFINITY;
@@ -247,7 +257,7 @@ DNX_DEV void count_chunk(const SampleArgs& a, int row, int chunk) {
 // these reach the cuts. The weights of bins are off by 2^-22 or, for large l / T,
 // by the rounding of that; where a cut by weight may lie takes this in.
 DNX_DEV void find_cuts(const SampleArgs& a, int row) {
-  constexpr int P = kBins / kThreads, U = 8;       // bins a thread, chunks at once
+  constexpr int P = kBins / kThreads, U = 16;       // bins a thread, chunks at once
   __shared__ uint64_t mass[kBins];
   __shared__ uint32_t count[kBins];
   __shared__ uint64_t part[kWaves];
@@ -333,106 +343,117 @@ DNX_DEV void find_cuts(const SampleArgs& a, int row) {
   }
 }
 
-// Step 3, a workgroup a chunk: the weights of the tokens before the bins in
-// question (before lo; before k; before lo and of min_p), and the keys of the
-// tokens in them.
+// How many tokens of the bins in question a unit of 64 E may list.
+constexpr int unit_found(int E) { return E == 16 ? 128 : 64; }
+
+// Step 3, a wave units of 64 E tokens (`first` and each `step` further): the weights
+// of the tokens before the bins in question (before lo; before k; before lo and of
+// min_p), and the keys of the tokens in them. The next unit is requested before
+// the present one is weighed.
 template <int E>
-DNX_DEV void weigh_chunk(const SampleArgs& a, int row, int chunk) {
-  __shared__ uint64_t part[kWaves];
-  __shared__ uint32_t found;
-  const int tid = threadIdx.x;
-  float l[E];
-  load_chunk<E>(a, row, chunk, l);
+DNX_DEV void weigh_units(const SampleArgs& a, int row, int first, int step) {
+  if (first >= a.units) return;
+  const int lane = threadIdx.x & 63;
+  float l[E], next[E];
+  load_logits<E>(a, row, first * 64 * E, lane, 64, next);
   const int32_t* cut = a.cuts + 4 * (int64_t)row;
   const int lo = cut[0], hi = cut[1], bin_k = cut[2];
   const Request r = request(a, row);
   const float top = row_top(a, row);
-  const int64_t at = (int64_t)row * a.chunks + chunk;
-  if (tid == 0) found = 0;
-  __syncthreads();
   const float place = floorf(scaled(top, r.inv));
-  uint64_t before_lo = 0, before_k = 0, kept = 0;
+#pragma unroll 1
+  for (int unit = first; unit < a.units; unit += step) {
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    const int b = r.cut ? bin_of(l[e], top, place, r.inv) : l[e] > -INFINITY ? 0 : kBins;
-    if (b < bin_k) {
-      const uint64_t w = weight(l[e], top, r.rate);
-      before_k += w;
-      if (b < lo) {
-        before_lo += w;
-        kept += at_least(w, r);
+    for (int e = 0; e < E; e++) l[e] = next[e];
+    load_logits<E>(a, row, (unit + step) * 64 * E, lane, 64, next);   // none past the last
+    const int64_t at = (int64_t)row * a.units + unit;
+    uint64_t before_lo = 0, before_k = 0, kept = 0;
+    uint32_t found = 0;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      int b[4];
+      bool weighs = false, asked = false, here[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        b[i] = r.cut ? bin_of(l[e + i], top, place, r.inv) : l[e + i] > -INFINITY ? 0 : kBins;
+        here[i] = b[i] < kBins && ((b[i] >= lo && b[i] <= hi) || b[i] == bin_k);
+        weighs |= b[i] < bin_k;
+        asked |= here[i];
+      }
+      if (__any(weighs)) {       // four at once: their series are independent
+        uint64_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = weight(l[e + i], top, r.rate);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          before_k += b[i] < bin_k ? w[i] : 0;
+          before_lo += b[i] < lo ? w[i] : 0;
+          kept += b[i] < lo ? at_least(w[i], r) : 0;
+        }
+      }
+      if (!__any(asked)) continue;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint64_t with = __ballot(here[i]);
+        const uint32_t at_i =
+            found + __builtin_amdgcn_mbcnt_hi((uint32_t)(with >> 32),
+                                              __builtin_amdgcn_mbcnt_lo((uint32_t)with, 0));
+        if (here[i] && at_i < unit_found(E))
+          a.found[at * unit_found(E) + at_i] =
+              order_key(l[e + i], index_of(unit * 64 * E, lane, 64, e + i));
+        found += __builtin_popcountll(with);
       }
     }
-    if (b < kBins && ((b >= lo && b <= hi) || b == bin_k)) {
-      const uint32_t i = atomicAdd(&found, 1u);
-      if (i < kChunkFound) a.found[at * kChunkFound + i] = order_key(l[e], index_of<E>(chunk, e));
+    kept = wave_sum_u64(kept);
+    if (r.cut) {
+      before_lo = wave_sum_u64(before_lo);
+      before_k = wave_sum_u64(before_k);
     }
-  }
-  kept = block_sum(kept, part);
-  if (r.cut) {
-    before_lo = block_sum(before_lo, part);
-    before_k = block_sum(before_k, part);
-  }
-  if (tid == 0) {
-    a.sums[3 * at] = before_lo;
-    a.sums[3 * at + 1] = before_k;
-    a.sums[3 * at + 2] = kept;
-    a.founds[at] = found;
+    if (lane == 0) {
+      a.sums[3 * at] = before_lo;
+      a.sums[3 * at + 1] = before_k;
+      a.sums[3 * at + 2] = kept;
+      a.founds[at] = found;
+    }
   }
 }
 
-// Keys in rising order: N a power of two, those past n above all.
+// Up to kFound keys in rising order: each to its rank.
 DNX_DEV void sort_keys(uint64_t* keys, int n) {
   const int tid = threadIdx.x;
-  if (n <= 128) {           // each to its rank
-    __syncthreads();
-    const uint64_t mine = tid < n ? keys[tid] : 0;
-    int rank = 0;
-    if (tid < n)
-      for (int i = 0; i < n; i++) rank += keys[i] < mine;
-    __syncthreads();
-    if (tid < n) keys[rank] = mine;
-    __syncthreads();
-    return;
+  __syncthreads();
+  const uint64_t mine = tid < n ? keys[tid] : 0;
+  int rank = 0;
+  if (tid < n) {
+#pragma unroll 8
+    for (int i = 0; i < n; i++) rank += keys[i] < mine;
   }
-  int size = 256;
-  while (size < n) size *= 2;
-  for (int i = n + tid; i < size; i += kThreads) keys[i] = ~0ull;
-  for (int k = 2; k <= size; k *= 2)
-    for (int j = k / 2; j > 0; j /= 2) {
-      __syncthreads();
-      for (int t = tid; t < size / 2; t += kThreads) {
-        const int i = 2 * t - (t & (j - 1)), p = i + j;
-        const uint64_t x = keys[i], y = keys[p];
-        if ((x > y) == ((i & k) == 0)) keys[i] = y, keys[p] = x;
-      }
-    }
+  __syncthreads();
+  if (tid < n) keys[rank] = mine;
   __syncthreads();
 }
 
 // What step 4 keeps in LDS: the order keys of the bins in question, those of them
 // that are sorted, and the running sums of their weights, or the counts and weights
 // of a span's parts.
-static_assert(kFound <= kParts, "upto serves both");
+static_assert(kFound <= kParts && kFound <= kThreads, "upto serves both, a thread a key");
 struct PickShared {
   uint64_t list[kListed], keys[kFound], upto[kParts];
+  uint32_t count[kParts];
   uint64_t part[kWaves], ends[2];
-  unsigned long long sums[kMaxChunks];
-  int begin[kMaxChunks + 1], at[2], n;
+  unsigned long long sums[kMaxUnits];
+  int begin[kMaxUnits + 1], at[2], n, unit;
+  uint64_t before;
 };
 
 // n keys of sh.keys in order, and the running sums of their weights.
 DNX_DEV void order_keys(PickShared& sh, int n, float top, const Request& r) {
   const int tid = threadIdx.x;
   sort_keys(sh.keys, n);
-  const int per = (n + kThreads - 1) / kThreads;    // in a row a thread
-  uint64_t sum = 0, all;
-  for (int i = tid * per; i < min(n, (tid + 1) * per); i++) {
-    sh.upto[i] = weight(of_key((uint32_t)(sh.keys[i] >> 32)), top, r.rate);
-    sum += sh.upto[i];
-  }
-  uint64_t before = block_before(sum, sh.part, all);
-  for (int i = tid * per; i < min(n, (tid + 1) * per); i++) sh.upto[i] = before += sh.upto[i];
+  uint64_t all;
+  const uint64_t w = tid < n ? weight(of_key((uint32_t)(sh.keys[tid] >> 32)), top, r.rate) : 0;
+  const uint64_t before = block_before(w, sh.part, all);
+  if (tid < n) sh.upto[tid] = before + w;
   __syncthreads();
 }
 
@@ -470,7 +491,7 @@ DNX_DEV bool find_key(PickShared& sh, Each each, float top, const Request& r, in
   first = sh.ends[0];
   last = sh.ends[1];
   if (n == 0) return false;
-  uint32_t* count = (uint32_t*)sh.keys;
+  uint32_t* count = sh.count;
   uint64_t rank_before = 0;
   while (n > kFound) {
     const int shift = max(0, 64 - 11 - __builtin_clzll(last - first));
@@ -543,74 +564,78 @@ DNX_DEV bool find_key(PickShared& sh, Each each, float top, const Request& r, in
 }
 
 // Step 4, a workgroup a row: the tokens of the bins in question in order, where
-// among them the cuts lie, the kept weights of each chunk, and the token in its
-// chunk.
+// among them the cuts lie, the kept weights of each unit, and the token in its
+// unit.
 template <int E>
 DNX_DEV void pick(const SampleArgs& a, int row) {
-  constexpr int kChunk = kThreads * E;
+  constexpr int kUnit = 64 * E, kUnitFound = unit_found(E), U = kMaxUnits / kThreads;
   __shared__ PickShared sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* x = a.logits + row * a.stride;
-  const int64_t base = (int64_t)row * a.chunks;
+  const int64_t base = (int64_t)row * a.units;
+  const int32_t* cut = a.cuts + 4 * (int64_t)row;
+  const int lo = cut[0], hi = cut[1], bin_k = cut[2];
+  // A thread's units: U in a row. All is requested before the first wait.
+  uint64_t before_lo = 0, before_k = 0, mine[U];
+  uint32_t counts[U];
+#pragma unroll
+  for (int i = 0; i < U; i++) {
+    const int c = U * tid + i;
+    const uint64_t* from = a.sums + 3 * (base + min(c, a.units - 1));
+    const uint64_t s0 = from[0], s1 = from[1], s2 = from[2];
+    const uint32_t n = a.founds[base + min(c, a.units - 1)];
+    mine[i] = c < a.units ? s2 : 0;
+    counts[i] = c < a.units ? n : 0;
+    before_lo += c < a.units ? s0 : 0;
+    before_k += c < a.units ? s1 : 0;
+  }
+  const Request r = request(a, row);
+  const int rank_k = r.top_k - cut[3];
   const float top = row_top(a, row);
   if (!(top > -INFINITY)) {
     if (tid == 0) a.out[row] = -1;
     return;
   }
-  const Request r = request(a, row);
-  uint64_t before_lo = 0, before_k = 0;
-  for (int c = tid; c < kMaxChunks; c += kThreads) {
-    sh.sums[c] = c < a.chunks ? a.sums[3 * (base + c) + 2] : 0;
-    if (r.cut && c < a.chunks) {
-      before_lo += a.sums[3 * (base + c)];
-      before_k += a.sums[3 * (base + c) + 1];
-    }
-  }
+#pragma unroll
+  for (int i = 0; i < U; i++) sh.sums[U * tid + i] = mine[i];
   uint64_t within = ~0ull;
-  bool whole = false;       // the chunks' sums have to be formed again
-  const int32_t* cut = a.cuts + 4 * (int64_t)row;
-  const int lo = cut[0], hi = cut[1], bin_k = cut[2], rank_k = r.top_k - cut[3];
+  bool whole = false;       // the units' sums have to be formed again
   const float place = floorf(scaled(top, r.inv));
   if (lo < kBins) {
     before_lo = block_sum(before_lo, sh.part);
     before_k = block_sum(before_k, sh.part);
-    if (wave == 0) {        // where each chunk's tokens begin
-      int n[kMaxChunks / 64], sum = 0;
-      bool over = false;
+    // Where each unit's tokens begin in the list; a unit that found more than it
+    // may list counts so that the list is too long.
+    uint64_t sum = 0, all;
 #pragma unroll
-      for (int i = 0; i < kMaxChunks / 64; i++) {
-        const int c = kMaxChunks / 64 * lane + i;
-        n[i] = c < a.chunks ? (int)a.founds[base + c] : 0;
-        over |= n[i] > kChunkFound;
-        sum += n[i];
-      }
-      int b = wave_scan(sum) - sum;
+    for (int i = 0; i < U; i++) sum += counts[i] > kUnitFound ? kListed + 1 : counts[i];
+    uint64_t b = block_before(sum, sh.part, all);
 #pragma unroll
-      for (int i = 0; i < kMaxChunks / 64; i++) {
-        sh.begin[kMaxChunks / 64 * lane + i] = b;
-        b += n[i];
-      }
-      over = __any(over);
-      if (lane == 63) sh.begin[kMaxChunks] = over ? -1 : b;
+    for (int i = 0; i < U; i++) {
+      sh.begin[U * tid + i] = (int)b;
+      b += counts[i];
     }
+    if (tid == 0) sh.begin[kMaxUnits] = (int)all;
     if (tid < 2) sh.at[tid] = kFound;
     __syncthreads();
-    const int n = sh.begin[kMaxChunks];     // -1: more than a chunk's list holds
+    const int n = sh.begin[kMaxUnits];
     uint64_t total = before_k;
     bool done = n > 0 && n <= kFound;
-    if (n > 0 && n <= kListed) {
+    if (n <= kListed) {
       uint64_t* to = done ? sh.keys : sh.list;
-      for (int c = wave; c < a.chunks; c += kWaves) {
-        const int b = sh.begin[c], m = sh.begin[c + 1] - b;
-        const uint64_t* from = a.found + (base + c) * kChunkFound;
-        for (int i0 = 0; i0 < m; i0 += 256) {
-          uint64_t k[4];
+      for (int i0 = tid; i0 < n; i0 += 4 * kThreads) {
+        uint64_t k[4];
 #pragma unroll
-          for (int u = 0; u < 4; u++) k[u] = from[min(i0 + 64 * u + lane, m - 1)];
+        for (int u = 0; u < 4; u++) {
+          const int i = min(i0 + u * kThreads, n - 1);
+          int c = 0;                        // the last unit that begins at or before i
 #pragma unroll
-          for (int u = 0; u < 4; u++)
-            if (i0 + 64 * u + lane < m) to[b + i0 + 64 * u + lane] = k[u];
+          for (int step = kMaxUnits / 2; step > 0; step /= 2) c += sh.begin[c + step] <= i ? step : 0;
+          k[u] = a.found[(base + c) * kUnitFound + i - sh.begin[c]];
         }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+          if (i0 + u * kThreads < n) to[i0 + u * kThreads] = k[u];
       }
       __syncthreads();
     }
@@ -644,7 +669,7 @@ DNX_DEV void pick(const SampleArgs& a, int row) {
         within = sh.keys[last];
         for (int i = tid; i <= last; i += kThreads) {
           const uint64_t w = at_least(sh.upto[i] - (i > 0 ? sh.upto[i - 1] : 0), r);
-          if (w > 0) atomicAdd(&sh.sums[(uint32_t)sh.keys[i] / kChunk], (unsigned long long)w);
+          if (w > 0) atomicAdd(&sh.sums[(uint32_t)sh.keys[i] / kUnit], (unsigned long long)w);
         }
       }
     }
@@ -678,70 +703,67 @@ DNX_DEV void pick(const SampleArgs& a, int row) {
         }
         within = key < within ? key : within;
       }
-      for (int c = wave; c < a.chunks && !whole; c += kWaves) {
-        uint64_t s = 0;
-        for (int i = sh.begin[c] + lane; i < sh.begin[c + 1]; i += 64) {
-          const uint64_t k = sh.list[i];
-          if (k <= within) s += at_least(weight(of_key((uint32_t)(k >> 32)), top, r.rate), r);
-        }
-        s = wave_sum_u64(s);
-        if (lane == 0) sh.sums[c] += s;
+      __syncthreads();
+      for (int i = tid; i < n && !whole; i += kThreads) {
+        const uint64_t k = sh.list[i];
+        const uint64_t w = k <= within ? at_least(weight(of_key((uint32_t)(k >> 32)), top, r.rate), r) : 0;
+        if (w > 0) atomicAdd(&sh.sums[(uint32_t)k / kUnit], (unsigned long long)w);
       }
     }
   }
-  auto kept = [&](int j) -> uint64_t {
-    if (j >= a.vocab) return 0;
-    const float l = x[j];
-    return order_key(l, j) <= within ? at_least(weight(l, top, r.rate), r) : 0;
+  // The kept weights of a lane's tokens of a unit.
+  auto kept = [&](int unit, uint64_t* w) {
+    float l[E];
+    load_logits<E>(a, row, unit * kUnit, lane, 64, l);
+    uint64_t sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      w[e] = order_key(l[e], index_of(unit * kUnit, lane, 64, e)) <= within
+                 ? at_least(weight(l[e], top, r.rate), r) : 0;
+      sum += w[e];
+    }
+    return sum;
   };
   __syncthreads();
   if (whole) {
-    for (int c = wave; c < a.chunks; c += kWaves) {
-      uint64_t s = 0;
-#pragma unroll 4
-      for (int e = 0; e < kChunk / 64; e++) s += kept(c * kChunk + e * 64 + lane);
-      s = wave_sum_u64(s);
+    for (int c = wave; c < a.units; c += kWaves) {
+      uint64_t w[E];
+      const uint64_t s = wave_sum_u64(kept(c, w));
       if (lane == 0) sh.sums[c] = s;
     }
     __syncthreads();
   }
-  // The chunk, by every wave alike.
-  uint64_t s[kMaxChunks / 64], mine = 0;
+  // The unit.
+  uint64_t s = 0, total;
 #pragma unroll
-  for (int i = 0; i < kMaxChunks / 64; i++) mine += s[i] = sh.sums[kMaxChunks / 64 * lane + i];
-  const uint64_t all = wave_scan(mine), total = __shfl(all, 63);
-  uint64_t target = (uint64_t)((double)r.u * (double)total), before = all - mine;
+  for (int i = 0; i < U; i++) s += mine[i] = sh.sums[U * tid + i];
+  uint64_t before = block_before(s, sh.part, total);
+  uint64_t target = (uint64_t)((double)r.u * (double)total);
   target = target < total ? target : total - 1;
-  int chunk = 0;
-  uint64_t chunk_before = 0;
-  bool here = false;
 #pragma unroll
-  for (int i = 0; i < kMaxChunks / 64; i++) {
-    if (before <= target && target < before + s[i]) {
-      here = true;
-      chunk = kMaxChunks / 64 * lane + i;
-      chunk_before = before;
+  for (int i = 0; i < U; i++) {
+    if (before <= target && target < before + mine[i]) {
+      sh.unit = U * tid + i;
+      sh.before = before;
     }
-    before += s[i];
+    before += mine[i];
   }
-  const int from = __builtin_ctzll(__ballot(here));
-  chunk = __shfl(chunk, from);
-  before = __shfl(chunk_before, from);
-  // Its tokens in order: a wave 64 E of them.
-  const int j0 = chunk * kChunk + wave * (64 * E) + lane;
-  uint64_t w[E], of_wave = 0;
-#pragma unroll
-  for (int e = 0; e < E; e++) of_wave += w[e] = kept(j0 + 64 * e);
-  of_wave = wave_sum_u64(of_wave);
-  if (lane == 0) sh.part[wave] = of_wave;
   __syncthreads();
-  for (int i = 0; i < wave; i++) before += sh.part[i];
-  if (target < before || target >= before + of_wave) return;
+  if (wave > 0) return;
+  const int unit = sh.unit;
+  before = sh.before;
+  uint64_t w[E];
+  kept(unit, w);
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    const uint64_t to = before + wave_scan(w[e]);
-    if (to > target && to - w[e] <= target) a.out[row] = j0 + 64 * e;
-    before = __shfl(to, 63);
+  for (int e = 0; e < E; e += 4) {
+    const uint64_t four = w[e] + w[e + 1] + w[e + 2] + w[e + 3], upto = wave_scan(four);
+    uint64_t at = before + upto - four;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (at <= target && target < at + w[e + i]) a.out[row] = index_of(unit * kUnit, lane, 64, e + i);
+      at += w[e + i];
+    }
+    before += lane_value(upto, 63);
   }
 }
 
@@ -749,40 +771,43 @@ template <int E>
 __global__ void __launch_bounds__(kThreads) count_kernel(SampleArgs a) {
   count_chunk<E>(a, blockIdx.x, blockIdx.y);
 }
-__global__ void __launch_bounds__(kThreads) cuts_kernel(SampleArgs a) {
-  find_cuts(a, blockIdx.x);
-}
+__global__ void __launch_bounds__(kThreads) cuts_kernel(SampleArgs a) { find_cuts(a, blockIdx.x); }
+constexpr int kUnitWaves = 4;
 template <int E>
-__global__ void __launch_bounds__(kThreads) weigh_kernel(SampleArgs a) {
-  weigh_chunk<E>(a, blockIdx.x, blockIdx.y);
+__global__ void __launch_bounds__(64 * kUnitWaves) weigh_kernel(SampleArgs a) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  weigh_units<E>(a, blockIdx.x, blockIdx.y * kUnitWaves + wave, gridDim.y * kUnitWaves);
 }
 template <int E>
 __global__ void __launch_bounds__(kThreads) pick_kernel(SampleArgs a) {
   pick<E>(a, blockIdx.x);
 }
 // A row of one chunk: the steps by one workgroup.
-template <int E>
 __global__ void __launch_bounds__(kThreads) row_kernel(SampleArgs a) {
-  count_chunk<E>(a, blockIdx.x, 0);
+  count_chunk<16>(a, blockIdx.x, 0);
   __syncthreads();
   find_cuts(a, blockIdx.x);
   __syncthreads();
-  weigh_chunk<E>(a, blockIdx.x, 0);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  weigh_units<16>(a, blockIdx.x, wave, kWaves);
   __syncthreads();
-  pick<E>(a, blockIdx.x);
+  pick<16>(a, blockIdx.x);
 }
 
-// Tokens of a thread in a chunk: 16, or 4 where that leaves CUs without a
-// workgroup.
-int per_thread(int64_t rows, int64_t vocab) {
-  const int64_t chunks = (vocab + 16 * kThreads - 1) / (16 * kThreads);
-  return chunks > 1 && rows * chunks < 256 && vocab <= kMaxChunks * 4 * kThreads ? 4 : 16;
+// Tokens of a thread in a chunk: 32 where that many workgroups are on the card at
+// once (64 rows of 151936: COUNT32), else 16. Tokens of a lane in a unit: 4
+// where 16 would leave SIMDs without a wave.
+struct Shape {
+  int64_t chunks, units;
+  int counted, tokens;
+};
+Shape shape_of(int64_t rows, int64_t vocab) {
+  const auto parts = [&](int64_t size) { return (vocab + size - 1) / size; };
+  const int counted = rows * parts(kThreads * 16) > 1024 && vocab > kThreads * 16 ? 32 : 16;
+  const int64_t chunks = parts(kThreads * counted);
+  const bool few = chunks > 1 && rows * parts(64 * 16) < 1024 && parts(64 * 4) <= kMaxUnits;
+  return {chunks, parts(64 * (few ? 4 : 16)), counted, few ? 4 : 16};
 }
-int64_t chunks_of(int64_t rows, int64_t vocab) {
-  const int64_t chunk = kThreads * per_thread(rows, vocab);
-  return (vocab + chunk - 1) / chunk;
-}
-constexpr int64_t kChunkBytes = 8 * (kBins + 3 + kChunkFound) + 8;
 
 }  // namespace
 
@@ -790,7 +815,8 @@ extern "C" {
 
 int64_t dnx_sample_workspace_bytes(int64_t rows, int64_t vocab) {
   if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab) return -1;
-  return rows * (chunks_of(rows, vocab) * kChunkBytes + 16);
+  const Shape s = shape_of(rows, vocab);
+  return rows * (s.chunks * (8 * kBins + 4) + s.units * (8 * (3 + unit_found(s.tokens)) + 4) + 16);
 }
 
 int dnx_sample(const float* logits, int64_t stride, const float* u, const float* temperature,
@@ -807,25 +833,27 @@ int dnx_sample(const float* logits, int64_t stride, const float* u, const float*
       ((uintptr_t)workspace & 15) != 0) {
     return DNX_EINVAL;
   }
-  const int64_t chunks = chunks_of(rows, vocab), n = rows * chunks;
-  SampleArgs a{logits, u, temperature, top_p, min_p, top_k, out, stride, (int)vocab, (int)chunks,
-               ((uintptr_t)logits & 15) == 0 && (stride % 4 == 0 || rows == 1)};
+  const Shape s = shape_of(rows, vocab);
+  SampleArgs a{logits, u, temperature, top_p, min_p, top_k, out, stride, (int)vocab, (int)s.chunks,
+               (int)s.units, ((uintptr_t)logits & 15) == 0 && (stride % 4 == 0 || rows == 1)};
   a.hist = (uint64_t*)workspace;
-  a.sums = a.hist + n * kBins;
-  a.found = a.sums + 3 * n;
-  a.tops = (float*)(a.found + n * kChunkFound);
-  a.founds = (uint32_t*)(a.tops + n);
-  a.cuts = (int32_t*)(a.founds + n);
-  const bool few = per_thread(rows, vocab) == 4;
+  a.sums = a.hist + rows * s.chunks * kBins;
+  a.found = a.sums + 3 * rows * s.units;
+  a.tops = (float*)(a.found + rows * s.units * unit_found(s.tokens));
+  a.founds = (uint32_t*)(a.tops + rows * s.chunks);
+  a.cuts = (int32_t*)(a.founds + rows * s.units);
   const hipStream_t st = (hipStream_t)stream;
-  const auto launch = [&](void (*k)(SampleArgs), int64_t y) {
-    hipLaunchKernelGGL(k, dim3((unsigned)rows, (unsigned)y), dim3(kThreads), 0, st, a);
+  const auto launch = [&](void (*k)(SampleArgs), int64_t y, int threads = kThreads) {
+    hipLaunchKernelGGL(k, dim3((unsigned)rows, (unsigned)y), dim3(threads), 0, st, a);
     return hipGetLastError() == hipSuccess;
   };
-  if (chunks == 1) return launch(row_kernel<16>, 1) ? DNX_OK : DNX_ELAUNCH;
-  const bool done = launch(few ? count_kernel<4> : count_kernel<16>, chunks) &&
-                    launch(cuts_kernel, 1) &&
-                    launch(few ? weigh_kernel<4> : weigh_kernel<16>, chunks) &&
+  if (vocab <= kThreads * 16) return launch(row_kernel, 1) ? DNX_OK : DNX_ELAUNCH;
+  const bool few = s.tokens == 4;
+  // Four waves a SIMD, of at least a unit each.
+  const int64_t weighers = std::min((s.units + kUnitWaves - 1) / kUnitWaves,
+                                    std::max<int64_t>(1, 4096 / kUnitWaves / rows));
+  const bool done = launch(s.counted == 32 ? count_kernel<32> : count_kernel<16>, s.chunks) && launch(cuts_kernel, 1) &&
+                    launch(few ? weigh_kernel<4> : weigh_kernel<16>, weighers, 64 * kUnitWaves) &&
                     launch(few ? pick_kernel<4> : pick_kernel<16>, 1);
   return done ? DNX_OK : DNX_ELAUNCH;
 }
