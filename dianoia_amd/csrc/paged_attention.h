@@ -14,7 +14,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr float kSlack = 8.0f;   // of a running maximum, in units of log2
 
 struct PartArgs {
-  int wide, few, blocks, runs, keys;
+  int wide, few, blocks, runs, keys, together;
 };
 
 struct PagedArgs {
@@ -211,9 +211,13 @@ DNX_DEV void paged_workgroup(const PagedArgs& a, uint8_t* lds) {
   }
   // The sequences' first runs before their second ones: where the bound on the
   // lengths is far above them, those that have keys start at once.
-  const uint32_t set = unit / (uint32_t)a.kv_heads;
-  uint32_t b = set % sets;
+  uint32_t set = unit / (uint32_t)a.kv_heads;
   w.kvh = (int)(unit % (uint32_t)a.kv_heads);
+  if (Body::kTogether && part.together) {   // all heads of a run to one XCD
+    set = unit / 8 / (uint32_t)a.kv_heads * 8 + unit % 8;
+    w.kvh = (int)(unit / 8 % (uint32_t)a.kv_heads);
+  }
+  uint32_t b = set % sets;
   w.run = (int)(set / sets);
   if (w.run >= part.runs) return;
   if (packed) {

@@ -967,6 +967,7 @@ constexpr int attention_lds() {
 template <typename C, int HD>
 struct FloatBody {
   static constexpr int kKeys = sizeof(C) == 4 ? 16 : 32;
+  static constexpr bool kTogether = false;
   static __device__ __forceinline__ void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
     ::wide<C, HD>(a, w, lds);
   }
@@ -1072,7 +1073,7 @@ __global__ void __launch_bounds__(kThreads) paged_combine_kernel(PagedArgs a) {
 }
 
 PartArgs part_of(const PagedPart& p) {
-  return {p.wide, p.few, (int)p.blocks, (int)p.runs, (int)p.keys};
+  return {p.wide, p.few, (int)p.blocks, (int)p.runs, (int)p.keys, p.together};
 }
 
 // The most own keys of a sequence that can be seen.
@@ -1082,7 +1083,8 @@ int64_t most_own(const dnx_paged_cache* c, const dnx_paged_batch* b) {
 
 PagedSplit split_of(const dnx_paged_cache* c, const dnx_paged_batch* b, int64_t heads) {
   return paged_split(b->seqs, b->tokens, std::min(b->max_tokens, b->tokens), heads / c->kv_heads,
-                     c->kv_heads, b->prefix_len, most_own(c, b), c->type == DNX_F32);
+                     c->kv_heads, b->prefix_len, most_own(c, b), c->type == DNX_F32,
+                     c->type == DNX_I8 ? c->hd : 0);
 }
 
 }  // namespace

@@ -49,18 +49,18 @@ DNX_DEV float abs_max(float x, float y) {
   return __builtin_elementwise_maximum(fabsf(x), fabsf(y));
 }
 
-// The digits of a query row at the lane's dims, 16 of each 64, and the factor
-// that takes a sum of products of theirs to a score in units of log2. A row
-// with an infinity or NaN: a factor of NaN.
+// The digits of a query row at the lane's dims, 16 from `dim` on and each `step`
+// further, and the factor that takes a sum of products of theirs to a score in
+// units of log2. A row with an infinity or NaN: a factor of NaN.
 template <int HD>
-DNX_DEV float query_digits(const float* q, int g4, float scale, uint4 (*qd)[3]) {
+DNX_DEV float query_digits(const float* q, int dim, int step, float scale, uint4 (*qd)[3]) {
   constexpr int ND = HD / 64;
   float x[ND][16], top = 0.0f;
 #pragma unroll
   for (int d = 0; d < ND; d++)
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
-      const float4 v = *(const float4*)(q + 64 * d + 16 * g4 + j);
+      const float4 v = *(const float4*)(q + dim + step * d + j);
       x[d][j] = v.x, x[d][j + 1] = v.y, x[d][j + 2] = v.z, x[d][j + 3] = v.w;
     }
 #pragma unroll
@@ -234,17 +234,36 @@ DNX_DEV float step_weights(v4f* s, float c, const float4* vs, bool edge, F sees,
 
 // ---- 16 rows a workgroup, each wave other keys, 64 a step.
 //
-// Lane l (quarter g = l / 16) holds key 16 u + l % 16 at the dims 16 (4 d + g)
-// .. of K, whose products with row l % 16's digits leave it with the scores of
-// keys 16 u + 4 g + v: the sixteen keys whose values it holds at dims EV (l %
-// 16) .., turned in registers into bytes of one dim, and whose weights' digits
-// are then the other operand as they are.
+// Lane l (quarter g = l / 16) takes key 16 u + l % 16 at 16 dims of each 64, whose
+// products with row l % 16's digits leave it with the scores of keys 16 u + 4 g
+// + v: the sixteen keys whose values it takes at HD / 16 dims, turned in
+// registers into bytes of one dim, and whose weights' digits are then the other
+// operand as they are.
+//
+// What bounds it is the reading, and how fast that goes depends on what one load
+// instruction covers (537 MB of keys and values read and dropped, hd 128, 8 key
+// heads: 4.8 TB/s by half lines of 16 keys, 5.1 by whole lines of 8, 5.9 by whole
+// lines marked as read once). So at hd 128 a load covers the 128 bytes of eight
+// keys, half of what a lane gets is for the lane 8 further in its quarter, and
+// the two trade it: K arrives as key l % 8 (+ 8) at dims 32 g + 16 (l / 8 % 2)
+// .., V as dims 16 (l % 8) .. of key 16 u + 4 g + l / 8 % 2 (+ 2). At hd 64 the
+// lines hold two heads: those of a run run on one XCD, through one L2 (64
+// sequences of 1088 keys, 28 -> 19.5 us; at hd 128 3% slower).
 template <int HD>
 struct Raw {
   uint4 k[4][HD / 64];
   uint32_t v[4][4][HD / 64];
   float4 ks[4], vs[4];
 };
+
+// Lanes 0 .. 7 of 16 keep x and take the x of 8 .. 15 into y; those keep their y
+// and take the y of 0 .. 7 into x.
+DNX_DEV void trade8(uint32_t& x, uint32_t& y) {
+  constexpr int kRor8 = 0x128;
+  const uint32_t a = x, b = y;
+  x = (uint32_t)__builtin_amdgcn_update_dpp((int)a, (int)b, kRor8, 0xf, 0xc, false);
+  y = (uint32_t)__builtin_amdgcn_update_dpp((int)b, (int)a, kRor8, 0xf, 0x3, false);
+}
 
 template <int HD, bool kJoined>
 DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
@@ -274,13 +293,18 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
 #pragma unroll
     for (int u = 0; u < 4; u++) block[u] = block_at<HD, kJoined>(a, w, at + 16 * u, page[u]);
   };
+  const int l8 = l16 & 7, b8 = l16 >> 3;
   auto request_keys = [&] {
 #pragma unroll
     for (int u = 0; u < 4; u++) {
       const i32x4 r = codes_of(block[u], a.keys);
+      if constexpr (ND == 2) {
 #pragma unroll
-      for (int d = 0; d < ND; d++)
-        x.k[u][d] = buffer_load16(r, l16 * a.row_bytes + (4 * d + g4) * 16);
+        for (int d = 0; d < 2; d++)
+          x.k[u][d] = buffer_load16_stream(r, (8 * d + l8) * a.row_bytes + 32 * g4 + 16 * b8);
+      } else {
+        x.k[u][0] = buffer_load16(r, l16 * a.row_bytes + 16 * g4);
+      }
       x.ks[u] = buffer_load_f4(scales_of(block[u], a.key_scales), 16 * g4);
     }
   };
@@ -288,15 +312,17 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
 #pragma unroll
     for (int u = 0; u < 4; u++) {
       const i32x4 r = codes_of(block[u], a.values);
+      if constexpr (ND == 2) {
 #pragma unroll
-      for (int v = 0; v < 4; v++) {
-        const int at = (4 * g4 + v) * a.row_bytes + EV * l16;
-        if constexpr (ND == 2) {
-          const i32x2 y = dnx_raw_buffer_load_v2i32(r, at, 0, 0);
-          x.v[u][v][0] = (uint32_t)y.x, x.v[u][v][1] = (uint32_t)y.y;
-        } else {
-          x.v[u][v][0] = (uint32_t)dnx_raw_buffer_load_i32(r, at, 0, 0);
+        for (int j = 0; j < 2; j++) {
+          const uint4 y = buffer_load16_stream(r, (4 * g4 + 2 * j + b8) * a.row_bytes + 16 * l8);
+          x.v[u][2 * j][0] = y.x, x.v[u][2 * j][1] = y.y;
+          x.v[u][2 * j + 1][0] = y.z, x.v[u][2 * j + 1][1] = y.w;
         }
+      } else {
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+          x.v[u][v][0] = (uint32_t)dnx_raw_buffer_load_i32(r, (4 * g4 + v) * a.row_bytes + EV * l16, 0, 0);
       }
       x.vs[u] = buffer_load_f4(scales_of(block[u], a.value_scales), 16 * g4);
     }
@@ -321,7 +347,8 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
     request_values();
     after = next(kt + kStride);
     pages(after);
-    c = query_digits<HD>(qp, g4, a.scale, qd);
+    c = ND == 2 ? query_digits<HD>(qp, 32 * g4, 16, a.scale, qd)
+                : query_digits<HD>(qp, 16 * g4, 64, a.scale, qd);
   }
   while (kt < w.k_hi) {
     int end[4];
@@ -333,6 +360,12 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
     v4f s[4];
 #pragma unroll
     for (int u = 0; u < 4; u++) {
+      if constexpr (ND == 2) {     // (the key of the first eight, dims of b8) for (own key, first dims)
+        trade8(x.k[u][0].x, x.k[u][1].x);
+        trade8(x.k[u][0].y, x.k[u][1].y);
+        trade8(x.k[u][0].z, x.k[u][1].z);
+        trade8(x.k[u][0].w, x.k[u][1].w);
+      }
       v4i t[3];
 #pragma unroll
       for (int k = 0; k < 3; k++) {
@@ -353,6 +386,14 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
     };
     uint32_t pd[3][4];
     const float beta = step_weights<HD>(s, c, x.vs, edge, sees, sums, pd);
+    if constexpr (ND == 2) {       // (key of b8, its first dims) for (first key, own dims)
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int v = 0; v < 4; v += 2)
+#pragma unroll
+          for (int h = 0; h < 2; h++) trade8(x.v[u][v][h], x.v[u][v + 1][h]);
+    }
 #pragma unroll
     for (int h = 0; h < ND; h++) {
       uint32_t f[4][4];
@@ -382,6 +423,8 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
   }
   sums.l = rows4_sum(sums.l);
 
+  // The dims of which row i of the products is: EV from here on.
+  auto dim_of = [](int i) { return ND == 2 ? 16 * (i & 7) + 8 * (i >> 3) : EV * i; };
   float* all = (float*)lds;
   float* ml = wave_stats<HD>(lds, wave);
   if (g4 == 0) {
@@ -392,7 +435,7 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
   for (int v = 0; v < 4; v++)
 #pragma unroll
     for (int e = 0; e < EV; e += 4)
-      *(float4*)&all[(wave * 16 + l16) * kSumRow<HD> + EV * (4 * g4 + v) + e] =
+      *(float4*)&all[(wave * 16 + l16) * kSumRow<HD> + dim_of(4 * g4 + v) + e] =
           make_float4(sums.o[e][v], sums.o[e + 1][v], sums.o[e + 2][v], sums.o[e + 3][v]);
   merge_waves<HD, 16>(a, w, lds);
 }
@@ -538,7 +581,7 @@ DNX_DEV void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
     load_tile(from);
     pages(from + KT);
   }
-  const float c = query_digits<HD>(qp, g4, a.scale, qd);
+  const float c = query_digits<HD>(qp, 16 * g4, 64, a.scale, qd);
   Sums<HD> sums;
   sums.m = -INFINITY;
   sums.l = 0.0f;
@@ -611,6 +654,7 @@ constexpr int attention_lds() {
 template <int HD>
 struct Int8Body {
   static constexpr int kKeys = 64;
+  static constexpr bool kTogether = HD == 64;
   static __device__ __forceinline__ void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
     ::wide<HD>(a, w, lds);
   }

@@ -18,6 +18,7 @@ namespace dnx {
 struct PagedPart {
   bool wide;
   int few;
+  bool together;                // all key heads of a run to one XCD (paged_together)
   int64_t blocks, runs, keys;   // blocks of rows, runs of that many keys
 };
 // `joined` (a multiple of kPagedStep): the prefix is walked with each
@@ -147,8 +148,16 @@ inline void paged_fit(PagedSplit& s, int64_t seqs, int64_t tokens, int64_t group
   }
 }
 
+inline void paged_together(PagedPart& p, int64_t sets, int64_t kv_heads, int64_t blocks,
+                           int64_t& items) {
+  const int64_t rounds = (sets + 7) / 8, all = rounds * 8 * kv_heads * blocks;
+  p.together = (sets % 8 == 0 || sets >= 64) && all <= kPagedItems / 2;
+  if (p.together) items = all;
+}
+
 inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, int64_t group,
-                              int64_t kv_heads, int64_t prefix_len, int64_t max_len, bool f32) {
+                              int64_t kv_heads, int64_t prefix_len, int64_t max_len, bool f32,
+                              int i8 = 0) {
   // Without a prefix, keys that one workgroup walks in about the time of the
   // second launch (3 us) stay in one run: up to 256.
   const int64_t least = prefix_len == 0 && max_len <= 256 ? 256 : kPagedStep;
@@ -173,6 +182,11 @@ inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, 
     s.prefix.runs = 0;
   }
   paged_fit(s, seqs, tokens, group, kv_heads, prefix_len, max_len);
+  if (i8 == 64) {
+    paged_together(s.prefix, s.prefix.runs, kv_heads, s.prefix.blocks, s.prefix_items);
+    paged_together(s.own, (s.slots > 0 ? s.slots : seqs) * s.own.runs, kv_heads,
+                   s.slots > 0 ? 1 : s.own.blocks, s.own_items);
+  }
   return s;
 }
 
