@@ -192,7 +192,9 @@ DNX_DEV bool unseen(const PagedArgs& a, const Item& w, int end) {
 // its own: the choice in one kernel cost every call 0.1 us (44 calls, geometric
 // mean: 9.11 us against 8.98).
 // Body: the blocks of one cache type and head size. kKeys: of a wave's step in a
-// block of 16.
+// block of 16. kTogether: paged_together's order. kLastFirst: a prompt's last rows,
+// which see the most keys, begin first (int8, 4096 tokens, 32 / 8 heads, hd 128: 366
+// -> 328 us; 2047 of 4099, 16 / 8 141 -> 118).
 template <typename Body, bool kPacked>
 DNX_DEV void paged_workgroup(const PagedArgs& a, uint8_t* lds) {
   Item w;
@@ -207,6 +209,7 @@ DNX_DEV void paged_workgroup(const PagedArgs& a, uint8_t* lds) {
     const uint32_t turn = id / 8;
     unit = turn / (uint32_t)part.blocks * 8 + id % 8;
     block = (int)(turn % (uint32_t)part.blocks);
+    if (Body::kLastFirst) block = part.blocks - 1 - block;   // they see the most keys
     sets = w.own ? (uint32_t)a.seqs : 1;
   }
   // The sequences' first runs before their second ones: where the bound on the

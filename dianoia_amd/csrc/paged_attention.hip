@@ -967,7 +967,7 @@ constexpr int attention_lds() {
 template <typename C, int HD>
 struct FloatBody {
   static constexpr int kKeys = sizeof(C) == 4 ? 16 : 32;
-  static constexpr bool kTogether = false;
+  static constexpr bool kTogether = false, kLastFirst = false;
   static __device__ __forceinline__ void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
     ::wide<C, HD>(a, w, lds);
   }

@@ -44,6 +44,17 @@ DNX_DEV float power2(int e) { return __int_as_float((e + 127) << 23); }
 constexpr int kMiddle = 0x8080;
 constexpr uint32_t kSigns = 0x80808080u;
 
+// Word k of the result holds byte k of each of four words; of the lower two bytes
+// the digits.
+DNX_DEV void bytes_of(const uint32_t* y, uint32_t* d) {
+  const uint32_t a = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u);
+  const uint32_t b = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
+  d[0] = __builtin_amdgcn_perm(b, a, 0x05040100u) ^ kSigns;
+  d[1] = __builtin_amdgcn_perm(b, a, 0x07060302u) ^ kSigns;
+  d[2] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(y[3], y[2], 0x0c0c0602u),
+                               __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602u), 0x05040100u);
+}
+
 // The larger of |x| and |y|, NaN if either is.
 DNX_DEV float abs_max(float x, float y) {
   return __builtin_elementwise_maximum(fabsf(x), fabsf(y));
@@ -79,16 +90,16 @@ DNX_DEV float query_digits(const float* q, int dim, int step, float scale, uint4
     uint32_t w[3][4];
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
-      uint32_t y[4];
+      // The float 3 2^22 + 0x8080 + q 2^(22 - e): its third byte is 64 more than
+      // the signed digit.
+      uint32_t y[4], t[3];
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        y[i] = (uint32_t)((int)rintf(__builtin_amdgcn_ldexpf(x[d][j + i], 22 - e)) + kMiddle);
+        y[i] = __float_as_uint(__builtin_amdgcn_ldexpf(x[d][j + i], 22 - e) + (12582912.0f + kMiddle));
+      bytes_of(y, t);
+      t[2] = ((t[2] & 0x7f7f7f7fu) + 0x40404040u) ^ ((t[2] ^ 0xc0c0c0c0u) & kSigns);   // + 192, bytewise
 #pragma unroll
-      for (int k = 0; k < 3; k++) {
-        const uint32_t v = (y[0] >> 8 * k & 255) | (y[1] >> 8 * k & 255) << 8 |
-                           (y[2] >> 8 * k & 255) << 16 | (y[3] >> 8 * k & 255) << 24;
-        w[k][j / 4] = k < 2 ? v ^ kSigns : v;
-      }
+      for (int k = 0; k < 3; k++) w[k][j / 4] = t[k];
     }
 #pragma unroll
     for (int k = 0; k < 3; k++) qd[d][k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
@@ -96,18 +107,13 @@ DNX_DEV float query_digits(const float* q, int dim, int step, float scale, uint4
   return __builtin_amdgcn_ldexpf(scale * 1.44269504088896341f, e - 22) + (top - top);
 }
 
-// The digits of four weights below 2^(e + 1) / 2 each, word k those of place k:
-// the float 2^23 + 0x8080 + w 2^(22 - e) has them as its bytes.
+// The digits of four weights below 2^e, word k those of place k: the float 2^23 +
+// 0x8080 + w 2^(22 - e) has them as its bytes.
 DNX_DEV void weight_digits(const float* w, float unit, uint32_t* d) {
   uint32_t y[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) y[i] = __float_as_uint(fmaf(w[i], unit, 8388608.0f + kMiddle));
-  const uint32_t a = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u);
-  const uint32_t b = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
-  d[0] = __builtin_amdgcn_perm(b, a, 0x05040100u) ^ kSigns;
-  d[1] = __builtin_amdgcn_perm(b, a, 0x07060302u) ^ kSigns;
-  d[2] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(y[3], y[2], 0x0c0c0602u),
-                               __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602u), 0x05040100u);
+  bytes_of(y, d);
 }
 
 // Bytes of four words turned: word c of the result holds byte c of each.
@@ -654,7 +660,7 @@ constexpr int attention_lds() {
 template <int HD>
 struct Int8Body {
   static constexpr int kKeys = 64;
-  static constexpr bool kTogether = HD == 64;
+  static constexpr bool kTogether = HD == 64, kLastFirst = true;
   static __device__ __forceinline__ void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
     ::wide<HD>(a, w, lds);
   }

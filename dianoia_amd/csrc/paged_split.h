@@ -148,6 +148,8 @@ inline void paged_fit(PagedSplit& s, int64_t seqs, int64_t tokens, int64_t group
   }
 }
 
+// int8 at head size 64: a line of the cache holds two heads. Where the runs are
+// whole rounds of the XCDs, or many, all heads of one go to the same XCD.
 inline void paged_together(PagedPart& p, int64_t sets, int64_t kv_heads, int64_t blocks,
                            int64_t& items) {
   const int64_t rounds = (sets + 7) / 8, all = rounds * 8 * kv_heads * blocks;
@@ -155,6 +157,7 @@ inline void paged_together(PagedPart& p, int64_t sets, int64_t kv_heads, int64_t
   if (p.together) items = all;
 }
 
+// i8: the head size of an int8 cache, else 0.
 inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, int64_t group,
                               int64_t kv_heads, int64_t prefix_len, int64_t max_len, bool f32,
                               int i8 = 0) {
@@ -163,7 +166,12 @@ inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, 
   const int64_t least = prefix_len == 0 && max_len <= 256 ? 256 : kPagedStep;
   const int64_t max_runs = tokens * group * kv_heads >= kPagedManyRows ? kPagedRuns
                            : prefix_len > 0 ? kPagedMaxRuns / 2 : kPagedMaxRuns;
-  PagedSplit s{paged_part(tokens, group, kv_heads, prefix_len, f32, kPagedStep, 1 << 20, max_runs),
+  // int8: a wide block's partial results are as many bytes as 256 of its keys and
+  // values (64 sequences of 128 to 4096 keys after 1000 shared ones, 32 / 8 heads,
+  // hd 128: prefix runs of 64 keys at least 92 us, 128 90, 256 84, 512 88).
+  const int64_t prefix_least =
+      i8 > 0 && paged_wide(tokens * group, kv_heads, prefix_len, f32) ? 256 : kPagedStep;
+  PagedSplit s{paged_part(tokens, group, kv_heads, prefix_len, f32, prefix_least, 1 << 20, max_runs),
                paged_part(max_tokens, group, seqs * kv_heads, max_len, f32, least, 2048, max_runs),
                0, 0, 0, 0};
   // A short prefix is joined to them where a CU for each workgroup is left: its
