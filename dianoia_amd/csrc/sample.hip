@@ -52,9 +52,9 @@ struct SampleArgs {
 
 // A row's request. Greedy: of a steep T, the first token.
 struct Request {
-  double rate, top_p;          // rate: log2(e) / T
+  double rate, top_p;          // rate: kPowers log2(e) / T
   uint64_t least;              // min_p in weights
-  float u, inv;                // inv: 1 / T of the bins, finite
+  float u, inv;                // inv: bins per unit / T, finite and not zero
   int top_k;
   bool cut;            // by rank or weight
 };
@@ -67,8 +67,8 @@ DNX_DEV Request request(const SampleArgs& a, int row) {
   const float u = a.u[row];
   const bool greedy = !(t > 0.0f);
   const double inv = greedy ? 0x1p40 : 1.0 / (double)t;
-  r.rate = inv * 1.4426950408889634;
-  r.inv = (float)fmax(fmin(inv, 1e37), 1e-41);   // an infinity times it is one
+  r.rate = inv * (1.4426950408889634 * 128.0);
+  r.inv = (float)fmax(fmin(inv * kBinsPerUnit, 1e38), 1e-41);   // an infinity times it is one
   r.top_p = !greedy && p < 1.0f ? fmax((double)p, 0.0) : 1.0;
   r.least = !greedy && low > 0.0f ? (uint64_t)ceil(fmin((double)low, 1.0) * 0x1p43) : 0;
   r.top_k = greedy ? 1 : k > 0 && k < a.vocab ? k : 0;
@@ -90,30 +90,39 @@ DNX_DEV float of_key(uint32_t k) {
 }
 DNX_DEV uint64_t order_key(float v, int j) { return (uint64_t)falling_key(v) << 32 | (uint32_t)j; }
 
-// A token's weight in multiples of 2^-43, and if that is enough for min_p. 2^x by the
-// Taylor series about the nearest whole number: |z| <= ln 2 / 2, whose 12th term
-// is below 2^-47. Adding 3 2^51 rounds to a whole number and leaves it in the lower
-// bits, adding 2^52 rounds the result: conversions between 64 bits and whole
+// Powers 2^(j / kPowers), by the Taylor series: |z| < ln 2, whose 18th term is below
+// 2^-62.
+constexpr int kPowers = 128;
+DNX_DEV void fill_powers(double* powers) {
+  if (threadIdx.x >= kPowers) return;
+  const double z = (double)threadIdx.x * (0.6931471805599453 / kPowers);
+  double p = 1.0;
+#pragma unroll
+  for (int i = 17; i > 0; i--) p = fma(p * (1.0 / i), z, 1.0);
+  powers[threadIdx.x] = p;
+}
+
+// A token's weight in multiples of 2^-43, and if that is enough for min_p. With
+// x = kPowers log2 of it, its whole part selects a power of two and one from the
+// table, the rest z is at most a half: the series in z ln 2 / kPowers, whose 5th
+// term is below 2^-49. Adding 3 2^51 rounds to a whole number and leaves it in the
+// lower bits, adding 2^52 rounds the result: conversions between 64 bits and whole
 // numbers run at a quarter of the rate.
-DNX_DEV uint64_t weight(float l, float top, double rate) {
+DNX_DEV uint64_t weight(float l, float top, double rate, const double* powers) {
+  constexpr double c = 0.6931471805599453 / kPowers;
   const double d = ((double)l - (double)top) * rate, x = l == top ? 0.0 : d, m = x + 0x1.8p52;
-  const double z = (x - (m - 0x1.8p52)) * 0.6931471805599453;
-  double p = 1.0 / 39916800.0;
-  p = fma(p, z, 1.0 / 3628800.0);
-  p = fma(p, z, 1.0 / 362880.0);
-  p = fma(p, z, 1.0 / 40320.0);
-  p = fma(p, z, 1.0 / 5040.0);
-  p = fma(p, z, 1.0 / 720.0);
-  p = fma(p, z, 1.0 / 120.0);
-  p = fma(p, z, 1.0 / 24.0);
-  p = fma(p, z, 1.0 / 6.0);
-  p = fma(p, z, 0.5);
+  const double z = x - (m - 0x1.8p52);
+  double p = c * c * c * c / 24.0;
+  p = fma(p, z, c * c * c / 6.0);
+  p = fma(p, z, c * c / 2.0);
+  p = fma(p, z, c);
   p = fma(p, z, 1.0);
-  p = fma(p, z, 1.0);
-  const bool some = x > -45.0;      // no NaN (of -inf - -inf too), no exponent out of range
-  const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, m);
+  const bool some = x > -45.0 * kPowers;   // no NaN (of -inf - -inf too), no exponent out of range
+  const int n = some ? (int)(uint32_t)__builtin_bit_cast(uint64_t, m) : 0;
+  p *= powers[n & (kPowers - 1)];
   const double w = __builtin_bit_cast(
-      double, __builtin_bit_cast(uint64_t, p) + ((uint64_t)(uint32_t)(some ? n + 43 : 0) << 52));
+      double, __builtin_bit_cast(uint64_t, p) + ((uint64_t)(uint32_t)((n >> 7) + 43) << 52));
+  static_assert(kPowers == 1 << 7, "the shift");
   const uint64_t whole = __builtin_bit_cast(uint64_t, w + 0x1p52) & ((1ull << 52) - 1);
   return some ? whole : 0;
 }
@@ -123,7 +132,7 @@ DNX_DEV uint64_t at_least(uint64_t w, const Request& r) { return w >= r.least ? 
 // the same for every chunk of a row. Far-off values are as the last ones (no
 // difference of two is then an infinity).
 DNX_DEV float scaled(float l, float inv) {
-  return __builtin_amdgcn_fmed3f(l * inv, -1e37f, 1e37f) * (float)kBinsPerUnit;
+  return __builtin_amdgcn_fmed3f(l * inv, -1e38f, 1e38f);
 }
 // The bin below the one that the row's (or the chunk's) largest logit lies in;
 // kBins and more: no weight.
@@ -297,7 +306,7 @@ DNX_DEV void find_cuts(const SampleArgs& a, int row) {
     uint64_t ws = 0, ns = 0, all, tokens;
 #pragma unroll
     for (int k = 0; k < P; k++) {
-      w[k] = (uint64_t)((double)w[k] * exp((double)(P * tid + k) * (-1.0 / kBinsPerUnit)) * 0x1p15);
+      w[k] = (uint64_t)((double)w[k] * __builtin_amdgcn_exp2f((float)(P * tid + k) * (-1.44269504f / kBinsPerUnit)) * 0x1p15);
       ws += w[k];
       ns += n[k];
     }
@@ -351,7 +360,8 @@ constexpr int unit_found(int E) { return E == 16 ? 128 : 64; }
 // min_p), and the keys of the tokens in them. The next unit is requested before
 // the present one is weighed.
 template <int E>
-DNX_DEV void weigh_units(const SampleArgs& a, int row, int first, int step) {
+DNX_DEV void weigh_units(const SampleArgs& a, int row, int first, int step,
+                         const double* powers) {
   if (first >= a.units) return;
   const int lane = threadIdx.x & 63;
   float l[E], next[E];
@@ -361,6 +371,9 @@ DNX_DEV void weigh_units(const SampleArgs& a, int row, int first, int step) {
   const Request r = request(a, row);
   const float top = row_top(a, row);
   const float place = floorf(scaled(top, r.inv));
+  // Without a cut every token's weight counts; without one by rank every bin's.
+  const float f_lo = lo < kBins ? (float)lo : INFINITY, f_hi = lo < kBins ? (float)hi : -1.0f;
+  const float f_k = bin_k < kBins ? (float)bin_k : INFINITY;
 #pragma unroll 1
   for (int unit = first; unit < a.units; unit += step) {
 #pragma unroll
@@ -371,30 +384,35 @@ DNX_DEV void weigh_units(const SampleArgs& a, int row, int first, int step) {
     uint32_t found = 0;
 #pragma unroll
     for (int e = 0; e < E; e += 4) {
-      int b[4];
-      bool weighs = false, asked = false, here[4];
+      bool first[4], weighs[4], here[4], some = false, asked = false;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        b[i] = r.cut ? bin_of(l[e + i], top, place, r.inv) : l[e + i] > -INFINITY ? 0 : kBins;
-        here[i] = b[i] < kBins && ((b[i] >= lo && b[i] <= hi) || b[i] == bin_k);
-        weighs |= b[i] < bin_k;
+        const float x = l[e + i], d = place - floorf(scaled(x, r.inv));   // its bin
+        const bool one = x > -INFINITY;
+        here[i] = one && ((d >= f_lo && d <= f_hi) || d == f_k);
+        weighs[i] = one && d < f_k;
+        first[i] = d < f_lo;
+        some |= weighs[i];
         asked |= here[i];
       }
-      if (__any(weighs)) {       // four at once: their series are independent
+      if (__any(some)) {       // four at once: their series are independent
         uint64_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = weight(l[e + i], top, r.rate);
+        for (int i = 0; i < 4; i++) w[i] = weight(l[e + i], top, r.rate, powers);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          before_k += b[i] < bin_k ? w[i] : 0;
-          before_lo += b[i] < lo ? w[i] : 0;
-          kept += b[i] < lo ? at_least(w[i], r) : 0;
+          w[i] = weighs[i] ? w[i] : 0;
+          before_k += w[i];
+          w[i] = first[i] ? w[i] : 0;
+          before_lo += w[i];
+          kept += at_least(w[i], r);
         }
       }
       if (!__any(asked)) continue;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const uint64_t with = __ballot(here[i]);
+        if (with == 0) continue;
         const uint32_t at_i =
             found + __builtin_amdgcn_mbcnt_hi((uint32_t)(with >> 32),
                                               __builtin_amdgcn_mbcnt_lo((uint32_t)with, 0));
@@ -440,6 +458,7 @@ static_assert(kFound <= kParts && kFound <= kThreads, "upto serves both, a threa
 struct PickShared {
   uint64_t list[kListed], keys[kFound], upto[kParts];
   uint32_t count[kParts];
+  double powers[kPowers];
   uint64_t part[kWaves], ends[2];
   unsigned long long sums[kMaxUnits];
   int begin[kMaxUnits + 1], at[2], n, unit;
@@ -451,7 +470,7 @@ DNX_DEV void order_keys(PickShared& sh, int n, float top, const Request& r) {
   const int tid = threadIdx.x;
   sort_keys(sh.keys, n);
   uint64_t all;
-  const uint64_t w = tid < n ? weight(of_key((uint32_t)(sh.keys[tid] >> 32)), top, r.rate) : 0;
+  const uint64_t w = tid < n ? weight(of_key((uint32_t)(sh.keys[tid] >> 32)), top, r.rate, sh.powers) : 0;
   const uint64_t before = block_before(w, sh.part, all);
   if (tid < n) sh.upto[tid] = before + w;
   __syncthreads();
@@ -503,7 +522,7 @@ DNX_DEV bool find_key(PickShared& sh, Each each, float top, const Request& r, in
       const int i = (int)((k - first) >> shift);
       atomicAdd(&count[i], 1u);
       atomicAdd((unsigned long long*)&sh.upto[i],
-                (unsigned long long)weight(of_key((uint32_t)(k >> 32)), top, r.rate));
+                (unsigned long long)weight(of_key((uint32_t)(k >> 32)), top, r.rate, sh.powers));
     });
     __syncthreads();
     constexpr int P = kParts / kThreads;
@@ -573,6 +592,7 @@ DNX_DEV void pick(const SampleArgs& a, int row) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* x = a.logits + row * a.stride;
   const int64_t base = (int64_t)row * a.units;
+  fill_powers(sh.powers);
   const int32_t* cut = a.cuts + 4 * (int64_t)row;
   const int lo = cut[0], hi = cut[1], bin_k = cut[2];
   // A thread's units: U in a row. All is requested before the first wait.
@@ -706,7 +726,7 @@ DNX_DEV void pick(const SampleArgs& a, int row) {
       __syncthreads();
       for (int i = tid; i < n && !whole; i += kThreads) {
         const uint64_t k = sh.list[i];
-        const uint64_t w = k <= within ? at_least(weight(of_key((uint32_t)(k >> 32)), top, r.rate), r) : 0;
+        const uint64_t w = k <= within ? at_least(weight(of_key((uint32_t)(k >> 32)), top, r.rate, sh.powers), r) : 0;
         if (w > 0) atomicAdd(&sh.sums[(uint32_t)k / kUnit], (unsigned long long)w);
       }
     }
@@ -719,7 +739,7 @@ DNX_DEV void pick(const SampleArgs& a, int row) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
       w[e] = order_key(l[e], index_of(unit * kUnit, lane, 64, e)) <= within
-                 ? at_least(weight(l[e], top, r.rate), r) : 0;
+                 ? at_least(weight(l[e], top, r.rate, sh.powers), r) : 0;
       sum += w[e];
     }
     return sum;
@@ -775,8 +795,11 @@ __global__ void __launch_bounds__(kThreads) cuts_kernel(SampleArgs a) { find_cut
 constexpr int kUnitWaves = 4;
 template <int E>
 __global__ void __launch_bounds__(64 * kUnitWaves) weigh_kernel(SampleArgs a) {
+  __shared__ double powers[kPowers];
+  fill_powers(powers);
+  __syncthreads();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  weigh_units<E>(a, blockIdx.x, blockIdx.y * kUnitWaves + wave, gridDim.y * kUnitWaves);
+  weigh_units<E>(a, blockIdx.x, blockIdx.y * kUnitWaves + wave, gridDim.y * kUnitWaves, powers);
 }
 template <int E>
 __global__ void __launch_bounds__(kThreads) pick_kernel(SampleArgs a) {
@@ -788,8 +811,11 @@ __global__ void __launch_bounds__(kThreads) row_kernel(SampleArgs a) {
   __syncthreads();
   find_cuts(a, blockIdx.x);
   __syncthreads();
+  __shared__ double powers[kPowers];
+  fill_powers(powers);
+  __syncthreads();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  weigh_units<16>(a, blockIdx.x, wave, kWaves);
+  weigh_units<16>(a, blockIdx.x, wave, kWaves, powers);
   __syncthreads();
   pick<16>(a, blockIdx.x);
 }
