@@ -90,14 +90,14 @@ DNX_DEV float query_digits(const float* q, int dim, int step, float scale, uint4
     uint32_t w[3][4];
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
-      // The float 3 2^22 + 0x8080 + q 2^(22 - e): its third byte is 64 more than
-      // the signed digit.
+      // The float 3 2^22 + q 2^(22 - e) holds the whole number in its lower bits, from
+      // 2^23 to 2^24; the 0x8080 would leave that range.
       uint32_t y[4], t[3];
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        y[i] = __float_as_uint(__builtin_amdgcn_ldexpf(x[d][j + i], 22 - e) + (12582912.0f + kMiddle));
+        y[i] = __float_as_uint(__builtin_amdgcn_ldexpf(x[d][j + i], 22 - e) + 12582912.0f) -
+               0x4b400000u + kMiddle;
       bytes_of(y, t);
-      t[2] = ((t[2] & 0x7f7f7f7fu) + 0x40404040u) ^ ((t[2] ^ 0xc0c0c0c0u) & kSigns);   // + 192, bytewise
 #pragma unroll
       for (int k = 0; k < 3; k++) w[k][j / 4] = t[k];
     }

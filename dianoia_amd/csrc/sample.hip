@@ -128,7 +128,7 @@ DNX_DEV uint64_t weight(float l, float top, double rate, const double* powers) {
 }
 DNX_DEV uint64_t at_least(uint64_t w, const Request& r) { return w >= r.least ? w : 0; }
 
-// Bins of l / T, an eighth wide: whole numbers that do not fall as logits rise,
+// Bins of l / T, 1 / kBinsPerUnit wide: whole numbers that do not fall as logits rise,
 // the same for every chunk of a row. Far-off values are as the last ones (no
 // difference of two is then an infinity).
 DNX_DEV float scaled(float l, float inv) {

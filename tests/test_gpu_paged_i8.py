@@ -504,6 +504,26 @@ def test_weights_of_nothing_and_much(gpu_ready):
         b.check()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("counts", [[1, 3], [150]])
+def test_next_to_powers_of_two(gpu_ready, counts, hd):
+    """Queries and weights whose digits are the largest there are: values at a
+    power of two, next to it, and some thousandths below it."""
+    edges = np.float32([1, -1, np.nextafter(np.float32(1), np.float32(0)),
+                        -np.nextafter(np.float32(1), np.float32(0)), 0.9925, -0.9925, 0.9921, -0.9921,
+                        0.998, -0.9999, 1 + 2.0 ** -23, 0.5, -0.25])
+    rng = np.random.default_rng(hd)
+    for fill in (1.0, 0.05):
+        b = Batch8(43, counts, [200, 90][:len(counts)], 70, 8, 2, hd, 32)
+        q = rng.choice(edges, tuple(b.q.shape)) * np.where(rng.random(tuple(b.q.shape)) < fill, 1, 0.1)
+        q *= 2.0 ** rng.integers(-3, 2, (*b.q.shape[:2], 1))
+        b.q.copy_(torch.from_numpy(q.astype(np.float32)))
+        b.value_scales.copy_(torch.from_numpy(np.abs(rng.choice(edges, tuple(b.value_scales.shape)))))
+        b.keys.copy_((b.keys.float() / 16).round().to(torch.int8))     # weights of nearly one
+        b.take()
+        b.check()
+
+
 def test_far_tail(gpu_ready):
     """One key that outweighs every other, and a long tail that together weighs
     as much: none of it is lost."""
