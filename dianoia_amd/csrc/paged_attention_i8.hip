@@ -5,10 +5,11 @@
 //   out = sum_j e^(s_j - m) vs_j d_j / sum_j e^(s_j - m).
 //
 // Both products run on the int8 matrix cores, on the codes as they lie in the
-// cache. The other operand is a whole number of at most 22 bits in three
-// digits of base 256 (the lower two from -128 to 127), a product each:
-// * a query row is q = 2^(e - 22) (65536 a + 256 b + c), 2^e the power of two
-//   above its largest value, so that q is off by half a unit, 2^-23 of 2^e;
+// cache. The other operand is a whole number of at most 23 bits in three
+// digits of base 256 from -128 to 127 (the highest up to 127), a product each:
+// * a query row is q = 2^(e - 23) (65536 a + 256 b + c), 2^e the power of two
+//   above 1.004 times its largest value, so that q is off by half a unit, 2^-24
+//   of 2^e;
 // * so are the weights e^(s_j - m) vs_j of a row and step, 2^e above the largest
 //   of that step: relative to the step, not to the running maximum, so that a
 //   long tail of small weights is kept.
@@ -43,6 +44,8 @@ DNX_DEV float power2(int e) { return __int_as_float((e + 127) << 23); }
 // The lower two digits are bytes less 128: 0x80 in both, taken off by an xor.
 constexpr int kMiddle = 0x8080;
 constexpr uint32_t kSigns = 0x80808080u;
+// 127 65536 + 127 256 + 127 is the largest number of three digits: 2^23 / 1.00394.
+constexpr float kRoom = 1.004f;
 
 // Word k of the result holds byte k of each of four words; of the lower two bytes
 // the digits.
@@ -84,19 +87,17 @@ DNX_DEV float query_digits(const float* q, int dim, int step, float scale, uint4
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false,
                                                   false);
   top = abs_max(__uint_as_float(b[0]), __uint_as_float(b[1]));
+  top *= kRoom;
   const int e = __builtin_amdgcn_frexp_expf(top);
 #pragma unroll
   for (int d = 0; d < ND; d++) {
     uint32_t w[3][4];
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
-      // The float 3 2^22 + q 2^(22 - e) holds the whole number in its lower bits, from
-      // 2^23 to 2^24; the 0x8080 would leave that range.
       uint32_t y[4], t[3];
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        y[i] = __float_as_uint(__builtin_amdgcn_ldexpf(x[d][j + i], 22 - e) + 12582912.0f) -
-               0x4b400000u + kMiddle;
+        y[i] = (uint32_t)((int)rintf(__builtin_amdgcn_ldexpf(x[d][j + i], 23 - e)) + kMiddle);
       bytes_of(y, t);
 #pragma unroll
       for (int k = 0; k < 3; k++) w[k][j / 4] = t[k];
@@ -104,11 +105,11 @@ DNX_DEV float query_digits(const float* q, int dim, int step, float scale, uint4
 #pragma unroll
     for (int k = 0; k < 3; k++) qd[d][k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
   }
-  return __builtin_amdgcn_ldexpf(scale * 1.44269504088896341f, e - 22) + (top - top);
+  return __builtin_amdgcn_ldexpf(scale * 1.44269504088896341f, e - 23) + (top - top);
 }
 
-// The digits of four weights below 2^e, word k those of place k: the float 2^23 +
-// 0x8080 + w 2^(22 - e) has them as its bytes.
+// The digits of four weights up to 2^e / kRoom, unit = 2^(23 - e), word k those of
+// place k: the float 2^23 + 0x8080 + w 2^(23 - e), below 2^24, has them as its bytes.
 DNX_DEV void weight_digits(const float* w, float unit, uint32_t* d) {
   uint32_t y[4];
 #pragma unroll
@@ -226,8 +227,9 @@ DNX_DEV float step_weights(v4f* s, float c, const float4* vs, bool edge, F sees,
   const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false,
                                                   false);
   top = abs_max(__uint_as_float(y[0]), __uint_as_float(y[1]));
+  top *= kRoom;
   const int e = max(__builtin_amdgcn_frexp_expf(top), -100);
-  const float unit = power2(22 - e);
+  const float unit = power2(23 - e);
 #pragma unroll
   for (int u = 0; u < 4; u++) {
     const float w[4] = {s[u][0], s[u][1], s[u][2], s[u][3]};
@@ -235,7 +237,7 @@ DNX_DEV float step_weights(v4f* s, float c, const float4* vs, bool edge, F sees,
     weight_digits(w, unit, t);
     d[0][u] = t[0], d[1][u] = t[1], d[2][u] = t[2];
   }
-  return power2(e - 22) + (top - top);   // NaN where a weight is no finite number
+  return power2(e - 23) + (top - top);   // NaN where a weight is no finite number
 }
 
 // ---- 16 rows a workgroup, each wave other keys, 64 a step.
