@@ -149,12 +149,10 @@ inline void paged_fit(PagedSplit& s, int64_t seqs, int64_t tokens, int64_t group
 }
 
 // int8 at head size 64: a line of the cache holds two heads. Where the runs are
-// whole rounds of the XCDs, or many, all heads of one go to the same XCD.
-inline void paged_together(PagedPart& p, int64_t sets, int64_t kv_heads, int64_t blocks,
-                           int64_t& items) {
-  const int64_t rounds = (sets + 7) / 8, all = rounds * 8 * kv_heads * blocks;
-  p.together = (sets % 8 == 0 || sets >= 64) && all <= kPagedItems / 2;
-  if (p.together) items = all;
+// whole rounds of the XCDs, or many, all heads of one go to the same XCD: the
+// workgroups that this takes, or 0.
+inline int64_t paged_together(int64_t sets, int64_t kv_heads, int64_t blocks) {
+  return sets > 0 && (sets % 8 == 0 || sets >= 64) ? (sets + 7) / 8 * 8 * kv_heads * blocks : 0;
 }
 
 // i8: the head size of an int8 cache, else 0.
@@ -191,9 +189,17 @@ inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, 
   }
   paged_fit(s, seqs, tokens, group, kv_heads, prefix_len, max_len);
   if (i8 == 64) {
-    paged_together(s.prefix, s.prefix.runs, kv_heads, s.prefix.blocks, s.prefix_items);
-    paged_together(s.own, (s.slots > 0 ? s.slots : seqs) * s.own.runs, kv_heads,
-                   s.slots > 0 ? 1 : s.own.blocks, s.own_items);
+    const int64_t prefix = paged_together(s.prefix.runs, kv_heads, s.prefix.blocks);
+    if (prefix > 0 && prefix + s.own_items <= kPagedItems) {
+      s.prefix.together = true;
+      s.prefix_items = prefix;
+    }
+    const int64_t own = paged_together((s.slots > 0 ? s.slots : seqs) * s.own.runs, kv_heads,
+                                       s.slots > 0 ? 1 : s.own.blocks);
+    if (own > 0 && s.prefix_items + own <= kPagedItems) {
+      s.own.together = true;
+      s.own_items = own;
+    }
   }
   return s;
 }

@@ -24,6 +24,7 @@ from scipy.ndimage import maximum_filter1d
 
 from dianoia_amd import device as D
 from gpu_util import host
+from test_gpu_sample import answers
 from test_gpu_paged import CASES, EPS, U, Batch, ints, rope_table, rotated
 
 pytestmark = pytest.mark.gpu
@@ -567,6 +568,145 @@ def test_same_bits_again_on_another_stream(gpu_ready):
     b.run(stream=side)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(b.out, first)
+
+
+def test_most_rows(gpu_ready):
+    """As many rows as a call may have, nearly all of them padding."""
+    rows, heads, kv = 1082401, 62, 31             # 2^26 - 2 rows of the result
+    b = Batch8(14, [3], [40], 500, heads, kv, 64, 16)
+    batch = D.PagedBatch(b.starts, b.lens_d, b.tables, rows, 3, 40,
+                         prefix_pages=b.batch.prefix_pages, prefix_len=500)
+    ws = D.paged_attention_workspace(b.cache, batch, heads)
+    q, out = (torch.empty(rows, heads, 64, device="cuda") for _ in range(2))
+    q[:3] = b.q
+    out.fill_(3.25)
+    D.paged_attention(b.cache, batch, q, out, ws)
+    want, room = b.expected()
+    assert (np.abs(host(out[:3]) - want) <= room).all()
+    assert not bool((out[3:] != 3.25).any())
+
+
+def test_steps_to_tokens_eager_and_captured(gpu_ready):
+    """Decode steps as a server runs them: append, attention, the int8 rows of its
+    output, their product with a head of 3001 tokens, and a token for each
+    sequence, over growing sequences; once eagerly and once as one captured graph
+    whose arrays change, with the program's own work between the replays. The
+    prefix is read back and written to another cache, which holds the same."""
+    seqs, prefix, heads, kv, hd, page, steps, vocab = 5, 75, 8, 2, 64, 16, 6, 3001
+    rows, width = seqs + 3, 6
+    rng = np.random.default_rng(13)
+    g = torch.Generator(device="cuda").manual_seed(13)
+    pages = 8 + seqs * width
+    order = rng.permutation(pages).astype(np.int32)
+    shared, tables_h = order[:5], order[5:5 + seqs * width].reshape(seqs, width)
+    rope = torch.from_numpy(rope_table(512, hd)).cuda()
+    w = 1 + 0.1 * torch.randn(hd, device="cuda", generator=g)
+    head = torch.randn(vocab, heads * hd, device="cuda", generator=g)
+    head_q = torch.empty(vocab, heads * hd, dtype=torch.int8, device="cuda")
+    head_s = torch.empty(vocab, device="cuda")
+    D.quantize_i8r(head, head_q, head_s, vocab, heads * hd, heads * hd)
+    step_qkv = [torch.randn(rows, (heads + 2 * kv) * hd, device="cuda", generator=g)
+                for _ in range(steps)]
+    step_u = torch.rand(steps, rows, device="cuda", generator=g)
+    par = [torch.tensor(x, device="cuda") for x in ([0.9, 1.0, 0.0, 1.2, 0.7, 1.0, 1.0, 1.0],
+                                                    [0.9, 1.0, 1.0, 0.95, 0.5, 1.0, 1.0, 1.0])]
+    top_k = ints([40, 0, 0, 200, 0, 0, 0, 0])
+    begin = [3, 17, 40, 15, 60]
+    history = [torch.randn(n, 2 * kv * hd, device="cuda", generator=g) for n in [prefix] + begin]
+
+    def play(captured):
+        kept = empty_cache(pages, page, kv, hd)
+        cache = D.PagedCache(*kept)
+        for i, x in enumerate(history):     # prompts, appended many tokens at once
+            n = x.shape[0]
+            table = shared if i == 0 else tables_h[i - 1]
+            own = np.arange(n)
+            D.paged_append(cache, x[:, :kv * hd].view(n, kv, hd), x[:, kv * hd:].view(n, kv, hd),
+                           ints(own + (0 if i == 0 else prefix)),
+                           ints(table[own // page] * page + own % page), rope=rope, k_norm=w)
+        starts, lens, tables = ints(list(range(seqs + 1))), ints(begin), ints(tables_h)
+        positions, slots = ints([0] * rows), ints([-1] * rows)
+        qkv = torch.empty(rows, (heads + 2 * kv) * hd, device="cuda")
+        q = qkv[:, :heads * hd].view(rows, heads, hd)
+        k = qkv[:, heads * hd:(heads + kv) * hd].view(rows, kv, hd)
+        v = qkv[:, (heads + kv) * hd:].view(rows, kv, hd)
+        q_rot, out = (torch.zeros(rows, heads, hd, device="cuda") for _ in range(2))
+        out_q = torch.empty(rows, heads * hd, dtype=torch.int8, device="cuda")
+        out_s, u = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+        logits = torch.empty(rows, vocab, device="cuda")
+        tokens = torch.full((rows,), -9, dtype=torch.int32, device="cuda")
+        batch = D.PagedBatch(starts, lens, tables, rows, 1, width * page, prefix_pages=ints(shared),
+                             prefix_len=prefix)
+        ws, sample_ws = D.paged_attention_workspace(cache, batch, heads), D.sample_workspace(rows, vocab)
+
+        def step():
+            D.paged_append(cache, k, v, positions, slots, rope=rope, q=q, q_out=q_rot, q_norm=w,
+                           k_norm=w)
+            D.paged_attention(cache, batch, q_rot, out, ws)
+            D.quantize_i8r(out, out_q, out_s, rows, heads * hd, heads * hd)
+            D.gemm_i8r(head_q, head_s, out_q, out_s, logits, vocab, heads * hd, rows)
+            D.sample(logits, u, tokens, sample_ws, temperature=par[0], top_k=top_k, top_p=par[1])
+
+        graph, got = None, []
+        for i in range(steps):
+            at = np.array(begin) + i
+            lens.copy_(ints(at + 1))
+            positions[:seqs] = ints(prefix + at)
+            slots[:seqs] = ints(tables_h[np.arange(seqs), at // page] * page + at % page)
+            qkv.copy_(step_qkv[i])
+            u.copy_(step_u[i])
+            if captured:
+                if graph is None:           # capture runs nothing
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph):
+                        step()
+                graph.replay()
+            else:
+                step()
+            got.append((out.clone(), logits.clone(), tokens.clone()))
+            torch.cuda.synchronize()
+        return cache, kept, q_rot.clone(), got
+
+    cache, kept, q_rot, eager = play(False)
+    _, kept2, _, replayed = play(True)
+    for a, b in zip(eager, replayed):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert all(torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0)) for x, y in zip(kept, kept2))
+    # Each step's tokens against the definition on its logits.
+    for i, (_, logits, tokens) in enumerate(eager):
+        for r in range(seqs):
+            want = answers(host(logits[r]), float(step_u[i, r]), float(par[0][r]), int(top_k[r]),
+                           float(par[1][r]), 0.0)
+            assert int(tokens[r]) in want, (i, r)
+    # The last step's attention against the formula on what the cache holds.
+    flat = [stored(kept[j], kept[2 + j]) for j in (0, 1)]
+    q = q_rot.double().cpu().numpy()
+    for b in range(seqs):
+        n = begin[b] + steps
+        places = np.concatenate([shared[np.arange(prefix) // page] * page + np.arange(prefix) % page,
+                                 tables_h[b][np.arange(n) // page] * page + np.arange(n) % page])
+        kk, vv = flat[0][places], flat[1][places]
+        assert np.isfinite(kk).all() and np.isfinite(vv).all()
+        for h in range(heads):
+            k1, v1 = kk[:, h // 4], vv[:, h // 4]
+            s = k1 @ q[b, h] / np.sqrt(hd)
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            e = (4 * U * np.abs(q[b, h]).max() * np.abs(k1).sum(1) / np.sqrt(hd) + 8 * U * np.abs(s)).max() + 2 * U
+            top = np.abs(v1).max(1)
+            of_step = maximum_filter1d(p * top, 255, mode="constant")
+            room = (2 * e + 2 * (len(k1) + 64) * U) * (p @ np.abs(v1)) + 4 * U * (of_step / top) @ np.abs(v1)
+            assert (np.abs(eager[-1][0][b, h].double().cpu().numpy() - p @ v1) <= room).all()
+    # The prefix moved to another cache: read back, appended, the same again.
+    at = ints(shared[np.arange(prefix) // page] * page + np.arange(prefix) % page)
+    back = [torch.empty(prefix, kv, hd, device="cuda") for _ in range(2)]
+    D.paged_read(cache, at, *back)
+    other = D.PagedCache(*empty_cache(pages, page, kv, hd))
+    D.paged_append(other, *back, None, at)
+    again = [torch.empty(prefix, kv, hd, device="cuda") for _ in range(2)]
+    D.paged_read(other, at, *again)
+    for x, y in zip(back, again):          # the largest code is 127 again: its scale moves by a rounding
+        assert bool(((x - y).abs() <= 2 * U * x.abs()).all())
 
 
 def test_refusals(gpu_ready):

@@ -190,6 +190,32 @@ def test_rows_of_any_stride(gpu_ready):
         view.fill_(50.0)
 
 
+@pytest.mark.parametrize("rows,vocab", [(40, 9000), (64, 151936), (300, 8192), (2000, 700), (65536, 3)])
+def test_many_rows(gpu_ready, rows, vocab):
+    """Shapes of every division into chunks and units, requests of every kind."""
+    rng = np.random.default_rng(rows)
+    l = logits_of(rng, rows, vocab)
+    r = Rows(l, rng.random(rows), t=rng.choice([0.0, 0.5, 1.0, 1.4], rows), k=rng.choice([0, 1, 50, 5000], rows),
+             p=rng.choice([0.3, 0.9, 1.0], rows), low=rng.choice([0.0, 0.02], rows))
+    got = r.run()
+    for i in rng.choice(rows, min(rows, 60), replace=False):
+        want = answers(l[i], r.u[i], *(x[i] for x in r.par))
+        assert int(got[i]) in want, (i, int(got[i]), want)
+
+
+@pytest.mark.parametrize("spread", [0.0, 1e-3, 0.05, 0.3])
+@pytest.mark.parametrize("vocab", [3000, 60000])
+def test_cuts_among_many_near_logits(gpu_ready, vocab, spread):
+    """More tokens in the bins in question than are listed or sorted at once."""
+    rng = np.random.default_rng(vocab)
+    l = (spread * rng.standard_normal((8, vocab))).astype(np.float32)
+    u, p = rng.random(8), np.array([0.01, 0.1, 0.3, 0.5, 0.77, 0.9, 0.999, 1.0])
+    k = np.array([0, 100, vocab // 3, 0, vocab - 7, 5000, 0, vocab // 2])
+    Rows(l, u, p=p).check()
+    Rows(l, u, t=0.3, k=k).check()
+    Rows(l, u, t=2.0, k=k, p=p, low=0.9).check()
+
+
 def test_large_vocabulary(gpu_ready):
     rng = np.random.default_rng(9)
     l = logits_of(rng, 2, 1 << 20)
@@ -268,4 +294,6 @@ def test_refusals(gpu_ready):
         D.sample_workspace(3, (1 << 20) + 1)
     with pytest.raises(RuntimeError):
         D.sample(l.expand(3, 100)[:1].expand(3, 100), u, out, ws)      # rows on top of each other
+    with pytest.raises(RuntimeError):
+        D.sample(l, u, out, ws[:-1])
     D.sample(torch.zeros(0, 100, device="cuda"), u[:0], out[:0], ws)
