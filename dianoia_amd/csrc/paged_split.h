@@ -164,13 +164,18 @@ inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, 
   const int64_t least = prefix_len == 0 && max_len <= 256 ? 256 : kPagedStep;
   const int64_t max_runs = tokens * group * kv_heads >= kPagedManyRows ? kPagedRuns
                            : prefix_len > 0 ? kPagedMaxRuns / 2 : kPagedMaxRuns;
+  const PagedPart own =
+      paged_part(max_tokens, group, seqs * kv_heads, max_len, f32, least, 2048, max_runs);
   // int8: a wide block's partial results are as many bytes as 256 of its keys and
-  // values (64 sequences of 128 to 4096 keys after 1000 shared ones, 32 / 8 heads,
-  // hd 128: prefix runs of 64 keys at least 92 us, 128 90, 256 84, 512 88).
+  // values. Where the sequences' own workgroups fill the card, the prefix has runs of
+  // that many at least (64 sequences of 128 to 4096 keys after 1000 shared ones, 32
+  // / 8 heads, hd 128: 64 92 us, 128 90, 256 84, 512 88); where not, its runs have
+  // to (6 sequences of up to 37 tokens after 777, 12 / 4 heads, hd 64, window 512:
+  // 64 15.3, 256 22.4).
+  const bool filled = i8 > 0 && seqs * kv_heads * own.blocks * own.runs >= 512;
   const int64_t prefix_least =
-      i8 > 0 && paged_wide(tokens * group, kv_heads, prefix_len, f32) ? 256 : kPagedStep;
-  PagedSplit s{paged_part(tokens, group, kv_heads, prefix_len, f32, prefix_least, 1 << 20, max_runs),
-               paged_part(max_tokens, group, seqs * kv_heads, max_len, f32, least, 2048, max_runs),
+      filled && paged_wide(tokens * group, kv_heads, prefix_len, f32) ? 256 : kPagedStep;
+  PagedSplit s{paged_part(tokens, group, kv_heads, prefix_len, f32, prefix_least, 1 << 20, max_runs), own,
                0, 0, 0, 0};
   // A short prefix is joined to them where a CU for each workgroup is left: its
   // keys are then read once for each block of rows, but without the second
