@@ -257,6 +257,12 @@ DNX_DEV float step_weights(v4f* s, float c, const float4* vs, bool edge, F sees,
 // .., V as dims 16 (l % 8) .. of key 16 u + 4 g + l / 8 % 2 (+ 2). At hd 64 the
 // lines hold two heads: those of a run run on one XCD, through one L2 (64
 // sequences of 1088 keys, 28 -> 19.5 us; at hd 128 3% slower).
+//
+// 64 sequences, 32 / 8 heads, hd 128, of 4096 keys 113 us, 4.9 TB/s (reading alone
+// 98), of 1088 34 us, 4.4; one of 131072 61, of which 5 are the second launch. A
+// step of 64 keys takes about 500 vector instructions (the bf16 form of
+// paged_attention.hip 1000 for as many), which cover half of the reading's time;
+// forming the products of one part beside the sums of another gained nothing.
 template <int HD>
 struct Raw {
   uint4 k[4][HD / 64];
@@ -453,6 +459,12 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
 // Keys as [16 dims][key], values as [quarter][dim], 16 bytes each: the bytes of
 // a quarter and dim are those of its sixteen keys, turned on the way. The next
 // tile is in registers meanwhile.
+//
+// 4096 tokens of a prompt, 32 / 8 heads, hd 128: 323 us, 248 TFLOP/s of the formula's
+// products; 2047 of 4099, 16 / 8 heads, 117 us. Vector instructions bound it, about
+// 450 for a wave's 64 keys of 16 rows: 16 a score (digits to a float, exp2, float to
+// digits) and 5 a sum (digits to a float, into the running sum), beside 48 matrix
+// instructions; tiles of 128 keys would halve the latter and are not tried.
 template <int HD>
 struct WideTile {
   static constexpr int KT = 64, KC = HD / 16;      // 16-byte chunks of a key

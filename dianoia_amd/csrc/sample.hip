@@ -11,6 +11,20 @@
 //
 // Weights are whole multiples of 2^-43, formed in 64 bits: whole numbers' sums
 // do not depend on their order, whatever deals them to threads.
+//
+// Nothing is sorted but what lies at a cut. Four launches: (1) of each chunk of a row
+// its largest logit and, in bins of l / T, the tokens and a rough weight; (2) of each
+// row the bins in which the cuts lie; (3) of each unit (a wave's tokens) the exact
+// weights before those bins and the tokens in them; (4) of each row these tokens in
+// order, the cuts, the total, the unit and the token. A row of up to 8192 tokens takes
+// one launch. The logits are read twice, the second time mostly from the caches.
+//
+// 64 rows of 151936, a mix of requests: 59 us (traced 15 + 6 + 23 + 16), where reading
+// the logits once takes 8: the third step's 64-bit series (25 instructions a token) and
+// the fourth's ten or so waits in turn for memory and for its workgroup. One row of
+// 128000 with top-k and top-p 21, 13 rows of 32003 without filters 13: four launches,
+// one to three load latencies each. Rows of nearly equal logits, whose bins hold more
+// than lists do, 92 (32003) to 480 (64 of 151936).
 
 #include <algorithm>
 
@@ -820,9 +834,10 @@ __global__ void __launch_bounds__(kThreads) row_kernel(SampleArgs a) {
   pick<16>(a, blockIdx.x);
 }
 
-// Tokens of a thread in a chunk: 32 where that many workgroups are on the card at
-// once (64 rows of 151936: COUNT32), else 16. Tokens of a lane in a unit: 4
-// where 16 would leave SIMDs without a wave.
+// Tokens of a thread in a chunk: 32 where 16 would make more workgroups than the card
+// holds at once (64 rows of 151936 logits: the first two steps take 19.4 us, with 16
+// 21.4), else 16 (one row of 128000: 10.7; with 4 18). Tokens of a lane in a unit: 4
+// where 16 would leave SIMDs without a wave (one row of 128000: 4.1 us).
 struct Shape {
   int64_t chunks, units;
   int counted, tokens;

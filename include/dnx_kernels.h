@@ -636,7 +636,13 @@ typedef struct {
 // float32, of values times weights of up to 2^8. Where the bf16 matrix cores are
 // used (bf16 caches, and float32 ones where more than 32 rows share keys), each
 // float32 operand is taken as three pieces, whose sum it is down to 2^-110: of
-// values of 2^-118 5e-6 is lost, of 2^-125 6e-4.
+// values of 2^-118 5e-6 is lost, of 2^-125 6e-4. On an int8 cache the codes are taken
+// as they are (scales not below zero) and the other operand as a whole number of 23
+// bits, relative to a query row's largest value and to the largest weight times value
+// scale among 64 keys of a row: within 6e-7 of the formula at ordinary values. There a
+// query row that holds an infinity or NaN (or 3.3e38) is NaN, and so is a head that
+// sees a key scale of NaN or a value scale that is no finite number; of value scales
+// below 2^-100 2^-123 may be lost.
 // workspace: dnx_paged_attention_workspace_bytes of device memory (the partial
 // results of runs of keys), 16-byte aligned; calls that overlap need one each.
 // Batches of up to 2^22 key heads (seqs * kv_heads) are served whatever their
