@@ -887,25 +887,37 @@ def paged_append(cache: PagedCache, k, v, positions, slots, rope=None, q=None, q
         _check(rc, "dnx_paged_append")
 
 
+def _strided(name: str, t, heads: int, hd: int) -> int:
+    """The stride of rows [n][heads][hd] whose heads are dense."""
+    if t.dim() != 3 or t.stride(2) != 1 or (heads != 1 and t.stride(1) != hd):
+        raise ValueError(f"{name}: rows [n][heads][hd] with dense heads")
+    return t.stride(0) if t.shape[0] > 1 else heads * hd
+
+
 def paged_read(cache: PagedCache, slots, k=None, v=None, stream=None) -> None:
     """Places `slots` of the cache as float32 into k and v [n][kv_heads][hd]
     (dnx_paged_read); either may be left out, and both may be views of one
     tensor's rows. A row whose slot lies outside the cache is left as it is."""
     d = cache.check_device()
     n, kv_heads, hd = slots.numel(), cache.kv_heads, cache.hd
-    at = []
-    for t in (k, v):
-        if t is None:
-            at += [None, 0]
-            continue
-        s0, s1, s2 = t.stride() if t.dim() == 3 else (0, 0, 0)
-        if (t.shape != (n, kv_heads, hd) or t.dtype is not _F32 or s2 != 1
-                or (kv_heads != 1 and s1 != hd) or t.get_device() != d):
-            raise ValueError("paged_read: k and v are float32 [n][kv_heads][hd] with dense heads, "
-                             "on the cache's device")
-        at += [t.data_ptr(), s0 if n > 1 else kv_heads * hd]
-    rc = _lib.load().dnx_paged_read(cache.ref, _numbers("slots", slots, d, n, _I32), *at, n,
-                                    _on(d, stream))
+    dense = kv_heads * hd
+    kp = vp = None
+    ks = vs = dense
+    if k is not None:
+        if not k.is_contiguous():
+            ks = _strided("paged_read", k, kv_heads, hd)
+        if k.shape != (n, kv_heads, hd) or k.dtype is not _F32 or k.get_device() != d:
+            raise ValueError("paged_read: k is float32 [n][kv_heads][hd], on the cache's device")
+        kp = k.data_ptr()
+    if v is not None:
+        if not v.is_contiguous():
+            vs = _strided("paged_read", v, kv_heads, hd)
+        if v.shape != (n, kv_heads, hd) or v.dtype is not _F32 or v.get_device() != d:
+            raise ValueError("paged_read: v is float32 [n][kv_heads][hd], on the cache's device")
+        vp = v.data_ptr()
+    rc = (_lib._lib or _lib.load()).dnx_paged_read(
+        cache.ref, _numbers("slots", slots, d, n, _I32), kp, ks, vp, vs, n,
+        _raw_stream(d) if stream is None else stream.cuda_stream)
     if rc:
         _check(rc, "dnx_paged_read")
 
@@ -963,14 +975,13 @@ def sample(logits, u, out, workspace, temperature=None, top_k=None, top_p=None, 
     if inner != 1 and vocab != 1:
         raise ValueError("sample: the logits of a row lie side by side")
 
-    def given(what, t, dtype):
-        return None if t is None else _numbers(what, t, d, rows, dtype)
-
-    rc = _lib.load().dnx_sample(
+    rc = (_lib._lib or _lib.load()).dnx_sample(
         logits.data_ptr(), stride if rows > 1 else vocab, _numbers("u", u, d, rows, _F32),
-        given("temperature", temperature, _F32), given("top_k", top_k, _I32),
-        given("top_p", top_p, _F32), given("min_p", min_p, _F32),
+        None if temperature is None else _numbers("temperature", temperature, d, rows, _F32),
+        None if top_k is None else _numbers("top_k", top_k, d, rows, _I32),
+        None if top_p is None else _numbers("top_p", top_p, d, rows, _F32),
+        None if min_p is None else _numbers("min_p", min_p, d, rows, _F32),
         _numbers("out", out, d, rows, _I32), rows, vocab, _at(workspace, d), workspace.nbytes,
-        _on(d, stream))
+        _raw_stream(d) if stream is None else stream.cuda_stream)
     if rc:
         _check(rc, "dnx_sample")
