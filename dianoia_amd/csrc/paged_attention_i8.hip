@@ -162,8 +162,8 @@ DNX_DEV Block block_at(const PagedArgs& a, const Item& w, int kt, int page) {
   return b;
 }
 
-// The running sums of a wave's 16 rows: o[c][v] of row l % 16 at dim EV (4 g +
-// v) + c, l the lane's part of the row's sum.
+// The running sums of a wave's 16 rows: o[c][v] of row l % 16 at the dim that row 4
+// g + v of product c is of, l the lane's part of the row's sum.
 template <int HD>
 struct Sums {
   float m, l;
@@ -175,7 +175,7 @@ struct Sums {
 // the weights' digits, whose word u of digit k is d[k][u]; the running sums
 // are scaled anew where the maximum has grown by 2^kSlack, and the factor is
 // returned that takes this step's sums of products to theirs.
-// bad: where the step holds keys that some row does not see.
+// edge: the step holds keys that some row does not see.
 template <int HD, typename F>
 DNX_DEV float step_weights(v4f* s, float c, const float4* vs, bool edge, F sees, Sums<HD>& a,
                            uint32_t (*d)[4]) {

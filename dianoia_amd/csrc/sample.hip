@@ -92,7 +92,6 @@ DNX_DEV Request request(const SampleArgs& a, int row) {
 }
 
 // Keys that rise as logits fall (+0 and -0 are one, NaN is -inf).
-constexpr uint32_t kNothing = 0xff800000u;   // of -inf
 DNX_DEV uint32_t falling_key(float v) {
   uint32_t b = __float_as_uint(v);
   if (v == 0.0f) b = 0;
