@@ -345,7 +345,9 @@ DNX_DEV void find_cuts(const SampleArgs& a, int row) {
       const double slack = 0x1p-17 + fabs((double)place) * 0x1p-27;
       const double least = (double)(bin_k == kBins ? all : bin_k == 0 ? 0 : mass[bin_k - 1]);
       const double most = (double)(bin_k == kBins ? all : mass[bin_k]);
-      const double from = r.top_p * least * (1.0 - slack), to = r.top_p * most * (1.0 + slack);
+      // Where |l / T| is so large that a float of it is wider than the bins' weights hold
+      // for (from 2^22 on), the cut may lie in any bin up to the last.
+      const double from = r.top_p * least * fmax(1.0 - slack, 0.0), to = r.top_p * most * (1.0 + slack);
 #pragma unroll
       for (int k = 0; k < P; k++) {
         const int b = P * tid + k;
@@ -707,7 +709,7 @@ DNX_DEV void pick(const SampleArgs& a, int row) {
       }
     }
     if (!done) {
-      whole = n <= 0 || n > kListed;
+      whole = n <= kFound || n > kListed;     // up to kFound were put into sh.keys, not sh.list
       const auto any = [&](auto f) {
         for (int j0 = tid; j0 < a.vocab; j0 += 8 * kThreads) {
           float l[8];
