@@ -63,11 +63,28 @@ DNX_DEV float abs_max(float x, float y) {
   return __builtin_elementwise_maximum(fabsf(x), fabsf(y));
 }
 
+// What takes a sum of products of a query row's digits to a score in units of
+// log2: `first` before the key's scale, where `far` (of any of the wave's rows,
+// else it is 1), and `c` after it. Rows of small values have two factors: the
+// product of both, 2^(e - 23), may be too small for a float, and the sum times a
+// large key's scale too large. A score up to 2^60 is so reached from any row and
+// any scale; c and first are normal numbers.
+struct QueryFactor {
+  float c, first;
+  bool far;
+};
+constexpr int kNear = -32, kFirst = -120;   // 2^37, the largest sum, 2^kFirst is normal
+DNX_DEV QueryFactor query_factor(float scale, int e, float nan) {
+  const int a = max(min(e - 23, 0), kFirst);
+  const bool far = __any(e < kNear);
+  return {__builtin_amdgcn_ldexpf(scale * 1.44269504088896341f, far ? e - 23 - a : e - 23) + nan,
+          power2(a), far};
+}
+
 // The digits of a query row at the lane's dims, 16 from `dim` on and each `step`
-// further, and the factor that takes a sum of products of theirs to a score in
-// units of log2. A row with an infinity or NaN: a factor of NaN.
+// further. A row with an infinity or NaN: a factor of NaN.
 template <int HD>
-DNX_DEV float query_digits(const float* q, int dim, int step, float scale, uint4 (*qd)[3]) {
+DNX_DEV QueryFactor query_digits(const float* q, int dim, int step, float scale, uint4 (*qd)[3]) {
   constexpr int ND = HD / 64;
   float x[ND][16], top = 0.0f;
 #pragma unroll
@@ -105,7 +122,21 @@ DNX_DEV float query_digits(const float* q, int dim, int step, float scale, uint4
 #pragma unroll
     for (int k = 0; k < 3; k++) qd[d][k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
   }
-  return __builtin_amdgcn_ldexpf(scale * 1.44269504088896341f, e - 23) + (top - top);
+  return query_factor(scale, e, top - top);
+}
+
+// Sums of products to scores over c: times `first` where far, times the keys' scales.
+DNX_DEV void to_scores(v4f* s, const QueryFactor& f, const float4* ks) {
+  if (f.far) {
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+      for (int v = 0; v < 4; v++) s[u][v] *= f.first;
+  }
+#pragma unroll
+  for (int u = 0; u < 4; u++)
+#pragma unroll
+    for (int v = 0; v < 4; v++) s[u][v] *= (&ks[u].x)[v];
 }
 
 // The digits of four weights up to 2^e / kRoom, unit = 2^(23 - e), word k those of
@@ -346,7 +377,7 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
     return at;
   };
   uint4 qd[ND][3];
-  float c = 0.0f;
+  QueryFactor factor{};
   const int first = w.k_lo + KS * wave;
   int kt = next(first), after = kt;
   if (kt < w.k_hi) {
@@ -361,8 +392,8 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
     request_values();
     after = next(kt + kStride);
     pages(after);
-    c = ND == 2 ? query_digits<HD>(qp, 32 * g4, 16, a.scale, qd)
-                : query_digits<HD>(qp, 16 * g4, 64, a.scale, qd);
+    factor = ND == 2 ? query_digits<HD>(qp, 32 * g4, 16, a.scale, qd)
+                     : query_digits<HD>(qp, 16 * g4, 64, a.scale, qd);
   }
   while (kt < w.k_hi) {
     int end[4];
@@ -388,8 +419,9 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
         for (int d = 0; d < ND; d++) t[k] = mfma8(x.k[u][d], qd[d][k], t[k]);
       }
 #pragma unroll
-      for (int v = 0; v < 4; v++) s[u][v] = of_digits(t[2][v], t[1][v], t[0][v]) * (&x.ks[u].x)[v];
+      for (int v = 0; v < 4; v++) s[u][v] = of_digits(t[2][v], t[1][v], t[0][v]);
     }
+    to_scores(s, factor, x.ks);
     request_keys();
     bool edge = __any(see.lo > kt || see.hi < kt + KS);
 #pragma unroll
@@ -399,7 +431,7 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
       return key >= see.lo && key < see.hi && key < end[u];
     };
     uint32_t pd[3][4];
-    const float beta = step_weights<HD>(s, c, x.vs, edge, sees, sums, pd);
+    const float beta = step_weights<HD>(s, factor.c, x.vs, edge, sees, sums, pd);
     if constexpr (ND == 2) {       // (key of b8, its first dims) for (first key, own dims)
 #pragma unroll
       for (int u = 0; u < 4; u++)
@@ -601,7 +633,7 @@ DNX_DEV void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
     load_tile(from);
     pages(from + KT);
   }
-  const float c = query_digits<HD>(qp, 16 * g4, 64, a.scale, qd);
+  const QueryFactor factor = query_digits<HD>(qp, 16 * g4, 64, a.scale, qd);
   Sums<HD> sums;
   sums.m = -INFINITY;
   sums.l = 0.0f;
@@ -618,10 +650,10 @@ DNX_DEV void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
     }
     if (!live || wave_lo >= kt + KT || wave_hi <= kt) continue;
     v4f s[4];
-    float4 vs[4];
+    float4 ks[4], vs[4];
 #pragma unroll
     for (int u = 0; u < 4; u++) {
-      const float4 ks = *(const float4*)&scales[16 * u + 4 * g4];
+      ks[u] = *(const float4*)&scales[16 * u + 4 * g4];
       vs[u] = *(const float4*)&scales[KT + 16 * u + 4 * g4];
       v4i t[3] = {v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}};
 #pragma unroll
@@ -631,15 +663,16 @@ DNX_DEV void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
         for (int k = 0; k < 3; k++) t[k] = mfma8(kf, qd[d][k], t[k]);
       }
 #pragma unroll
-      for (int v = 0; v < 4; v++) s[u][v] = of_digits(t[2][v], t[1][v], t[0][v]) * (&ks.x)[v];
+      for (int v = 0; v < 4; v++) s[u][v] = of_digits(t[2][v], t[1][v], t[0][v]);
     }
+    to_scores(s, factor, ks);
     const bool edge = there != 15u || kt + KT > w.k_hi || __any(see.lo > kt || see.hi < kt + KT);
     auto sees = [&](int u, int v) {
       const int key = kt + 16 * u + 4 * g4 + v;
       return (there >> u & 1) && key >= see.lo && key < see.hi && key < w.k_hi;
     };
     uint32_t pd[3][4];
-    const float beta = step_weights<HD>(s, c, vs, edge, sees, sums, pd);
+    const float beta = step_weights<HD>(s, factor.c, vs, edge, sees, sums, pd);
 #pragma unroll
     for (int e = 0; e < NE; e++) {
       const uint4 vf = *(const uint4*)(Vp + (g4 * HD + v_slot(16 * e + l16)) * 16);

@@ -642,7 +642,8 @@ typedef struct {
 // scale among 64 keys of a row: within 6e-7 of the formula at ordinary values. There a
 // query row that holds an infinity or NaN (or 3.3e38) is NaN, and so is a head that
 // sees a key scale of NaN or a value scale that is no finite number; of value scales
-// below 2^-100 2^-123 may be lost.
+// below 2^-100 2^-123 may be lost; scores hold up to 2^60, however small the queries
+// and large the key scales are.
 // workspace: dnx_paged_attention_workspace_bytes of device memory (the partial
 // results of runs of keys), 16-byte aligned; calls that overlap need one each.
 // Batches of up to 2^22 key heads (seqs * kv_heads) are served whatever their
