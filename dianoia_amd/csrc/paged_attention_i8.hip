@@ -5,14 +5,18 @@
 //   out = sum_j e^(s_j - m) vs_j d_j / sum_j e^(s_j - m).
 //
 // Both products run on the int8 matrix cores, on the codes as they lie in the
-// cache. The other operand is a whole number of at most 23 bits in three
-// digits of base 256 from -128 to 127 (the highest up to 127), a product each:
-// * a query row is q = 2^(e - 23) (65536 a + 256 b + c), 2^e the power of two
-//   above 1.004 times its largest value, so that q is off by half a unit, 2^-24
-//   of 2^e;
-// * so are the weights e^(s_j - m) vs_j of a row and step, 2^e above the largest
-//   of that step: relative to the step, not to the running maximum, so that a
-//   long tail of small weights is kept.
+// cache. The other operand is a whole number in digits of base 256 from -128 to 127
+// (the highest up to 127), a product each:
+// * a query row is a number of 31 bits in four digits, in units of 2^(e - 31), 2^e
+//   the power of two above 1.004 times its largest value: off by half a unit, 2^-32
+//   of 2^e. With three digits a row with one channel 3000 times the others, whose
+//   keys are as much smaller, is off by 1.2e-4 (2000 keys, hd 128), with four by
+//   5e-7; the fourth costs nothing that could be measured.
+// * the weights e^(s_j - m) vs_j of a row and step are numbers of 23 bits in three,
+//   2^e above the largest of that step: relative to the step, not to the running
+//   maximum, so that a long tail of small weights is kept. 64 keys times half a
+//   unit times codes of 127 are 2^-9 of half a code of that largest one, which
+//   is what its value was rounded by when it was appended.
 // The int32 sums are exact (128 products of 7 by 8 bits are below 2^21). A bf16
 // form would convert every code (1.5 instructions each) and take three
 // products of half the depth.
@@ -33,7 +37,12 @@ DNX_DEV v4i mfma8(const uint4& x, const uint4& y, v4i acc) {
                                                acc, 0, 0, 0);
 }
 
-// 65536 a + 256 b + c of sums of products of digits.
+// Sums of products of digits as one number: 2^24 a + 65536 b + 256 c + d.
+DNX_DEV float of_digits(int a, int b, int c, int d) {
+  return fmaf((float)(int)(((uint32_t)a << 8) + (uint32_t)b), 65536.0f,
+              (float)(int)(((uint32_t)c << 8) + (uint32_t)d));
+}
+// 65536 a + 256 b + c.
 DNX_DEV float of_digits(int a, int b, int c) {
   return fmaf((float)a, 65536.0f, (float)(int)(((uint32_t)b << 8) + (uint32_t)c));
 }
@@ -41,11 +50,25 @@ DNX_DEV float of_digits(int a, int b, int c) {
 // 2^e for -126 <= e <= 127.
 DNX_DEV float power2(int e) { return __int_as_float((e + 127) << 23); }
 
-// The lower two digits are bytes less 128: 0x80 in both, taken off by an xor.
-constexpr int kMiddle = 0x8080;
+// The digits below the highest are bytes less 128: 0x80 in each, taken off by an xor.
+constexpr int kMiddle = 0x8080, kMiddle4 = 0x808080;
 constexpr uint32_t kSigns = 0x80808080u;
-// 127 65536 + 127 256 + 127 is the largest number of three digits: 2^23 / 1.00394.
+// 127 (65536 + 256 + 1) is the largest number of three digits: 2^23 / 1.00394; of
+// four 2^31 / 1.00394.
 constexpr float kRoom = 1.004f;
+constexpr int kQ = 4, kQBits = 31;   // digits of a query's values, bits of them
+
+// Bytes of four words turned: word c of the result holds byte c of each.
+DNX_DEV void turn4(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, uint32_t* y) {
+  const uint32_t a = __builtin_amdgcn_perm(x1, x0, 0x05010400u);
+  const uint32_t b = __builtin_amdgcn_perm(x3, x2, 0x05010400u);
+  const uint32_t c = __builtin_amdgcn_perm(x1, x0, 0x07030602u);
+  const uint32_t d = __builtin_amdgcn_perm(x3, x2, 0x07030602u);
+  y[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+  y[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  y[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+  y[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
 
 // Word k of the result holds byte k of each of four words; of the lower two bytes
 // the digits.
@@ -66,25 +89,25 @@ DNX_DEV float abs_max(float x, float y) {
 // What takes a sum of products of a query row's digits to a score in units of
 // log2: `first` before the key's scale, where `far` (of any of the wave's rows,
 // else it is 1), and `c` after it. Rows of small values have two factors: the
-// product of both, 2^(e - 23), may be too small for a float, and the sum times a
+// product of both, 2^(e - kQBits), may be too small for a float, and the sum times a
 // large key's scale too large. A score up to 2^60 is so reached from any row and
 // any scale; c and first are normal numbers.
 struct QueryFactor {
   float c, first;
   bool far;
 };
-constexpr int kNear = -32, kFirst = -120;   // 2^37, the largest sum, 2^kFirst is normal
+constexpr int kNear = -32, kFirst = -120;
 DNX_DEV QueryFactor query_factor(float scale, int e, float nan) {
-  const int a = max(min(e - 23, 0), kFirst);
+  const int a = max(min(e - kQBits, 0), kFirst);
   const bool far = __any(e < kNear);
-  return {__builtin_amdgcn_ldexpf(scale * 1.44269504088896341f, far ? e - 23 - a : e - 23) + nan,
-          power2(a), far};
+  const int b = far ? e - kQBits - a : e - kQBits;
+  return {__builtin_amdgcn_ldexpf(scale * 1.44269504088896341f, b) + nan, power2(a), far};
 }
 
 // The digits of a query row at the lane's dims, 16 from `dim` on and each `step`
 // further. A row with an infinity or NaN: a factor of NaN.
 template <int HD>
-DNX_DEV QueryFactor query_digits(const float* q, int dim, int step, float scale, uint4 (*qd)[3]) {
+DNX_DEV QueryFactor query_digits(const float* q, int dim, int step, float scale, uint4 (*qd)[kQ]) {
   constexpr int ND = HD / 64;
   float x[ND][16], top = 0.0f;
 #pragma unroll
@@ -108,19 +131,19 @@ DNX_DEV QueryFactor query_digits(const float* q, int dim, int step, float scale,
   const int e = __builtin_amdgcn_frexp_expf(top);
 #pragma unroll
   for (int d = 0; d < ND; d++) {
-    uint32_t w[3][4];
+    uint32_t w[kQ][4];
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
-      uint32_t y[4], t[3];
+      uint32_t y[4], t[kQ];
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        y[i] = (uint32_t)((int)rintf(__builtin_amdgcn_ldexpf(x[d][j + i], 23 - e)) + kMiddle);
-      bytes_of(y, t);
+        y[i] = (uint32_t)(int)rintf(__builtin_amdgcn_ldexpf(x[d][j + i], kQBits - e)) + kMiddle4;
+      turn4(y[0], y[1], y[2], y[3], t);
 #pragma unroll
-      for (int k = 0; k < 3; k++) w[k][j / 4] = t[k];
+      for (int k = 0; k < kQ; k++) w[k][j / 4] = k < kQ - 1 ? t[k] ^ kSigns : t[k];
     }
 #pragma unroll
-    for (int k = 0; k < 3; k++) qd[d][k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+    for (int k = 0; k < kQ; k++) qd[d][k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
   }
   return query_factor(scale, e, top - top);
 }
@@ -146,18 +169,6 @@ DNX_DEV void weight_digits(const float* w, float unit, uint32_t* d) {
 #pragma unroll
   for (int i = 0; i < 4; i++) y[i] = __float_as_uint(fmaf(w[i], unit, 8388608.0f + kMiddle));
   bytes_of(y, d);
-}
-
-// Bytes of four words turned: word c of the result holds byte c of each.
-DNX_DEV void turn4(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, uint32_t* y) {
-  const uint32_t a = __builtin_amdgcn_perm(x1, x0, 0x05010400u);
-  const uint32_t b = __builtin_amdgcn_perm(x3, x2, 0x05010400u);
-  const uint32_t c = __builtin_amdgcn_perm(x1, x0, 0x07030602u);
-  const uint32_t d = __builtin_amdgcn_perm(x3, x2, 0x07030602u);
-  y[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
-  y[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-  y[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
-  y[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
 // 16 keys of an item from kt on, as paged_attention.hip's blocks: where their
@@ -376,7 +387,7 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
     while (at < w.k_hi && !__any(see.lo < at + KS && see.hi > at)) at += kStride;
     return at;
   };
-  uint4 qd[ND][3];
+  uint4 qd[ND][kQ];
   QueryFactor factor{};
   const int first = w.k_lo + KS * wave;
   int kt = next(first), after = kt;
@@ -411,15 +422,15 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
         trade8(x.k[u][0].z, x.k[u][1].z);
         trade8(x.k[u][0].w, x.k[u][1].w);
       }
-      v4i t[3];
+      v4i t[kQ];
 #pragma unroll
-      for (int k = 0; k < 3; k++) {
+      for (int k = 0; k < kQ; k++) {
         t[k] = v4i{0, 0, 0, 0};
 #pragma unroll
         for (int d = 0; d < ND; d++) t[k] = mfma8(x.k[u][d], qd[d][k], t[k]);
       }
 #pragma unroll
-      for (int v = 0; v < 4; v++) s[u][v] = of_digits(t[2][v], t[1][v], t[0][v]);
+      for (int v = 0; v < 4; v++) s[u][v] = of_digits(t[3][v], t[2][v], t[1][v], t[0][v]);
     }
     to_scores(s, factor, x.ks);
     request_keys();
@@ -627,7 +638,7 @@ DNX_DEV void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
     if (wave < 2) scales[tid] = sr;
   };
 
-  uint4 qd[ND][3];
+  uint4 qd[ND][kQ];
   if (from < to) {
     pages(from);
     load_tile(from);
@@ -655,15 +666,15 @@ DNX_DEV void wide(const PagedArgs& a, const Item& w, uint8_t* lds) {
     for (int u = 0; u < 4; u++) {
       ks[u] = *(const float4*)&scales[16 * u + 4 * g4];
       vs[u] = *(const float4*)&scales[KT + 16 * u + 4 * g4];
-      v4i t[3] = {v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}};
+      v4i t[kQ] = {};
 #pragma unroll
       for (int d = 0; d < ND; d++) {
         const uint4 kf = *(const uint4*)(Kp + (4 * d + g4) * T::KS + (16 * u + l16) * 16);
 #pragma unroll
-        for (int k = 0; k < 3; k++) t[k] = mfma8(kf, qd[d][k], t[k]);
+        for (int k = 0; k < kQ; k++) t[k] = mfma8(kf, qd[d][k], t[k]);
       }
 #pragma unroll
-      for (int v = 0; v < 4; v++) s[u][v] = of_digits(t[2][v], t[1][v], t[0][v]);
+      for (int v = 0; v < 4; v++) s[u][v] = of_digits(t[3][v], t[2][v], t[1][v], t[0][v]);
     }
     to_scores(s, factor, ks);
     const bool edge = there != 15u || kt + KT > w.k_hi || __any(see.lo > kt || see.hi < kt + KT);

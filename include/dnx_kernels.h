@@ -637,9 +637,10 @@ typedef struct {
 // used (bf16 caches, and float32 ones where more than 32 rows share keys), each
 // float32 operand is taken as three pieces, whose sum it is down to 2^-110: of
 // values of 2^-118 5e-6 is lost, of 2^-125 6e-4. On an int8 cache the codes are taken
-// as they are (scales not below zero) and the other operand as a whole number of 23
-// bits, relative to a query row's largest value and to the largest weight times value
-// scale among 64 keys of a row: within 6e-7 of the formula at ordinary values. There a
+// as they are (scales not below zero) and the other operand as a whole number: a
+// query row's values of 31 bits, relative to its largest, and weights times value
+// scales of 23 bits, relative to the largest among 64 keys of a row (at most 2^-9 of
+// half a code of that one): within 6e-7 of the formula at ordinary values. There a
 // query row that holds an infinity or NaN (or 3.3e38) is NaN, and so is a head that
 // sees a key scale of NaN or a value scale that is no finite number; of value scales
 // below 2^-100 2^-123 may be lost; scores hold up to 2^60, however small the queries

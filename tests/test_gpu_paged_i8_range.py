@@ -1,16 +1,15 @@
 """dnx_paged_attention over int8 caches at the ends of the float range, against
 the formula in 64 bits, with bounds that follow the digits it is made of.
 
-Tolerances, with u = 2^-24. A query row is in multiples of 2^(e - 23), 2^e the power
-of two above 1.004 times its largest value and at most 2.008 times it: an element is
-off by half a unit, 1.004 u times that largest value (plus u for the rounding of
-1.004 times it: 1.01 u), where the kernel's digits are three; more digits only
-lower that. Sums of products with codes are exact; made floats by two roundings
-and scaled by four, so a score is off by 1.01 u max|q| sum|k| / sqrt(hd) + 8 u |s|,
-and exp2 adds 2 u. A weight times its value's scale is off by 1.01 u of the largest
-of its step in the same way; a step is 64 keys, so the largest lies within 63 keys
-of it. The normalised weights are off by twice the scores' error, the sums over N
-keys add 2 (N + 64) u of the sum of |weight v|, the gate 4 u."""
+Tolerances, with u = 2^-24. A query row is in multiples of 2^(e - 31), 2^e the power
+of two above 1.004 times its largest value and so at most 2.008 times that value (the
+rounding of 1.004 times it: 2.01): an element is off by half a unit at most, 2.01 2^-32
+times the row's largest. Sums of products with codes are exact; made floats by two
+roundings and scaled by four, so a score is off by 2.01 2^-32 max|q| sum|k| / sqrt(hd) +
+8 u |s|, and exp2 adds 2 u. A weight times its value's scale is a multiple of 2^(e - 23)
+in the same way, off by 2.01 u of the largest of its step; a step is 64 keys, so the
+largest lies within 63 keys of it. The normalised weights are off by twice the scores'
+error, the sums over N keys add 2 (N + 64) u of the sum of |weight v|, the gate 4 u."""
 
 import numpy as np
 import pytest
@@ -25,7 +24,7 @@ pytestmark = pytest.mark.gpu
 
 
 class Tight(Batch8):
-    query = 1.01 * U          # an element's error in parts of the row's largest
+    query = 2.01 * 2.0 ** -32    # an element's error in parts of the row's largest
 
     def take(self):
         super().take()
@@ -65,7 +64,7 @@ class Tight(Batch8):
                     codes = np.abs(vv) / np.where(vs > 0, vs, 1)[:, None]
                     want[t, h] = w @ vv
                     room[t, h] = ((2 * e + 2 * (len(kk) + 64) * U) * (w @ np.abs(vv))
-                                  + 1.01 * U * of_step @ codes)
+                                  + 2.01 * U * of_step @ codes)
                     if gate is not None:
                         g = 1 / (1 + np.exp(-gate[t, h]))
                         room[t, h] = (room[t, h] + 4 * U * np.abs(want[t, h])) * g
@@ -142,3 +141,19 @@ def test_subnormal_queries_on_the_largest_keys(gpu_ready):
             b.check()
             q = host(b.q)
             assert (np.abs(q).max() < 2.0 ** -120) and (q != 0).any()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_one_large_query_channel(gpu_ready, shape, hd):
+    """A channel that is large in the queries and small in the keys, as models have
+    them: the others keep their bits."""
+    for by in (30.0, 300.0, 3000.0, 1e5, 1e6):
+        b = batch(55, SHAPES[shape], hd, gate=by > 1000)
+        rng = np.random.default_rng(int(by))
+        at = int(rng.integers(hd))
+        b.q[..., at] *= by
+        b.keys[..., at] = (b.keys[..., at].float() / by).round().to(torch.int8)
+        b.take()
+        b.check()
+        b.check(70)
