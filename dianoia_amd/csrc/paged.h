@@ -18,6 +18,16 @@ inline bool cache_ok(const dnx_paged_cache* c) {
            (((uintptr_t)c->key_scales | (uintptr_t)c->value_scales) & 15) == 0));
 }
 
+// An int8 cache's scales; the fields are not touched for other types, whose callers
+// may hold the struct as it was without them.
+struct CacheScales {
+  float *keys, *values;
+};
+inline CacheScales cache_scales(const dnx_paged_cache* c) {
+  if (c->type != DNX_I8) return {nullptr, nullptr};
+  return {c->key_scales, c->value_scales};
+}
+
 inline bool batch_ok(const dnx_paged_batch* b) {
   return b != nullptr && b->seqs > 0 && b->seqs <= (1 << 20) && b->tokens >= 0 &&
          b->tokens <= (1 << 22) && b->max_tokens > 0 && b->max_tokens <= (1 << 22) &&

@@ -267,9 +267,10 @@ int dnx_paged_append(const dnx_paged_cache* cache, const float* q, int64_t q_str
                         q_stride % 4 != 0))) {
     return DNX_EINVAL;
   }
+  const CacheScales scales = cache_scales(cache);
   const AppendArgs a{q, k, v, q_norm, k_norm, rope, q_out, positions, slots, q_stride, k_stride,
                      v_stride, rope_rows, cache->pages * cache->page, cache->keys, cache->values,
-                     cache->key_scales, cache->value_scales, (int)n, (int)heads, cache->kv_heads,
+                     scales.keys, scales.values, (int)n, (int)heads, cache->kv_heads,
                      __builtin_ctz((unsigned)cache->page), eps};
   const int64_t units = n * ((q != nullptr ? heads : 0) + 2 * cache->kv_heads);
   const int64_t per = kThreads / (cache->hd / 8);
@@ -294,7 +295,8 @@ int dnx_paged_read(const dnx_paged_cache* cache, const int32_t* slots, float* k,
       (v != nullptr && (v_stride < kv_dim || v_stride % 4 != 0))) {
     return DNX_EINVAL;
   }
-  const ReadArgs a{cache->keys, cache->values, cache->key_scales, cache->value_scales, slots, k, v,
+  const CacheScales scales = cache_scales(cache);
+  const ReadArgs a{cache->keys, cache->values, scales.keys, scales.values, slots, k, v,
                    k_stride, v_stride, cache->pages * cache->page, (int)n, cache->kv_heads,
                    __builtin_ctz((unsigned)cache->page)};
   const int64_t grid = (n * kv_dim / 4 + kThreads - 1) / kThreads;

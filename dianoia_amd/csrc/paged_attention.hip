@@ -1121,8 +1121,8 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
   a.pages = (int)cache->pages;
   a.page_bits = __builtin_ctz((unsigned)cache->page);
   a.row_bytes = cache->kv_heads * cache->hd * (cache->type == DNX_F32 ? 4 : cache->type == DNX_BF16 ? 2 : 1);
-  a.key_scales = cache->key_scales;
-  a.value_scales = cache->value_scales;
+  a.key_scales = cache_scales(cache).keys;
+  a.value_scales = cache_scales(cache).values;
   a.kv_heads = cache->kv_heads;
   a.heads = (int)heads;
   a.group = (int)(heads / cache->kv_heads);
