@@ -839,15 +839,16 @@ __global__ void __launch_bounds__(kThreads) row_kernel(SampleArgs a) {
 // holds at once (64 rows of 151936 logits: the first two steps take 19.4 us, with 16
 // 21.4), else 16 (one row of 128000: 10.7; with 4 18). Tokens of a lane in a unit: 4
 // where 16 would leave SIMDs without a wave (one row of 128000: 4.1 us).
+constexpr int kManyChunks = 1024, kManyUnits = 1024;   // of all rows, by 16 tokens a thread or lane
 struct Shape {
   int64_t chunks, units;
   int counted, tokens;
 };
 Shape shape_of(int64_t rows, int64_t vocab) {
   const auto parts = [&](int64_t size) { return (vocab + size - 1) / size; };
-  const int counted = rows * parts(kThreads * 16) > 1024 && vocab > kThreads * 16 ? 32 : 16;
+  const int counted = rows * parts(kThreads * 16) > kManyChunks && vocab > kThreads * 16 ? 32 : 16;
   const int64_t chunks = parts(kThreads * counted);
-  const bool few = chunks > 1 && rows * parts(64 * 16) < 1024 && parts(64 * 4) <= kMaxUnits;
+  const bool few = chunks > 1 && rows * parts(64 * 16) < kManyUnits && parts(64 * 4) <= kMaxUnits;
   return {chunks, parts(64 * (few ? 4 : 16)), counted, few ? 4 : 16};
 }
 
@@ -857,8 +858,15 @@ extern "C" {
 
 int64_t dnx_sample_workspace_bytes(int64_t rows, int64_t vocab) {
   if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab) return -1;
-  const Shape s = shape_of(rows, vocab);
-  return rows * (s.chunks * (8 * kBins + 4) + s.units * (8 * (3 + unit_found(s.tokens)) + 4) + 16);
+  // What the most demanding call of up to that many rows and tokens takes: few rows
+  // are in more chunks and units each than many are.
+  const auto parts = [&](int64_t size) { return (vocab + size - 1) / size; };
+  const auto unit = [](int64_t e) { return 8 * (3 + unit_found((int)e)) + 4; };
+  const int64_t chunks = std::max(rows * parts(kThreads * 32),
+                                  std::min<int64_t>(rows * parts(kThreads * 16), kManyChunks));
+  const int64_t units = std::max(rows * parts(64 * 16) * unit(16),
+                                 std::min<int64_t>(rows * parts(64 * 4), 4 * kManyUnits) * unit(4));
+  return chunks * (8 * kBins + 4) + units + rows * 16;
 }
 
 int dnx_sample(const float* logits, int64_t stride, const float* u, const float* temperature,

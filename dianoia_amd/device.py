@@ -953,7 +953,7 @@ def paged_attention(cache: PagedCache, batch: PagedBatch, q, out, workspace, win
 
 
 def sample_workspace(rows: int, vocab: int, device="cuda") -> torch.Tensor:
-    """Device workspace of sample for that many rows of logits."""
+    """Device workspace of sample for up to that many rows of up to that many logits."""
     nbytes = int(_lib.load().dnx_sample_workspace_bytes(rows, vocab))
     if nbytes < 0:
         raise RuntimeError(f"dnx_sample_workspace_bytes({rows}, {vocab}) refused the shape")

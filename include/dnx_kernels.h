@@ -676,7 +676,8 @@ int dnx_paged_attention(const dnx_paged_cache* cache, const dnx_paged_batch* bat
 // sums exact: the same logits give the same token, however they are dealt to
 // threads. Row i at logits + i * stride floats, vocab up to 2^20, rows to 2^16;
 // pointers 4-byte aligned. workspace: dnx_sample_workspace_bytes of device
-// memory, 16-byte aligned; calls that overlap need one each.
+// memory, 16-byte aligned; one for the most rows and the largest vocabulary serves
+// all calls of less; calls that overlap need one each.
 int64_t dnx_sample_workspace_bytes(int64_t rows, int64_t vocab);
 int dnx_sample(const float* logits, int64_t stride, const float* u, const float* temperature,
                const int32_t* top_k, const float* top_p, const float* min_p, int32_t* out,

@@ -10,6 +10,7 @@ import numpy as np
 import pytest
 import torch
 
+from dianoia_amd import device as D
 from test_gpu_sample import Rows, logits_of
 
 pytestmark = pytest.mark.gpu
@@ -85,3 +86,20 @@ def test_temperatures_of_nearly_nothing(gpu_ready, t):
             l[r, rng.permutation(vocab)[:4]] = l[r].max()
         for par in (dict(k=3, p=0.7), dict(k=50, p=0.4, low=0.1), dict(p=0.9), dict(k=2)):
             Rows(l, rng.random(12), t=np.float32(t), **par).check()
+
+
+@pytest.mark.parametrize("rows,vocab", [(32, 32003), (114, 9000), (257, 32003), (54, 151936), (9, 128000)])
+def test_fewer_rows_and_tokens_in_the_same_workspace(gpu_ready, rows, vocab):
+    """A server's workspace is that of its largest batch; nothing behind it is written."""
+    rng = np.random.default_rng(rows)
+    n = D.sample_workspace(rows, vocab).nbytes
+    memory = torch.full((n + 4096,), 0xff, dtype=torch.uint8, device="cuda")
+    l = logits_of(rng, rows, vocab)
+    for fewer in {rows, rows - 1, rows // 2, 1}:
+        for tokens in {vocab, vocab - 1, vocab // 2 + 3, 8193, 700}:
+            r = Rows(l[:fewer, :tokens], rng.random(fewer), t=0.8, k=rng.choice([0, 40], fewer), p=0.9)
+            out = torch.full((fewer,), -9, dtype=torch.int32, device="cuda")
+            t, k, p, _ = (None if x is None else torch.from_numpy(x).cuda() for x in r.par)
+            D.sample(r.logits, torch.from_numpy(r.u).cuda(), out, memory[:n], temperature=t, top_k=k, top_p=p)
+            assert (out.cpu().numpy() == r.run()).all()
+    assert bool((memory[n:] == 0xff).all())
