@@ -87,21 +87,16 @@ DNX_DEV float abs_max(float x, float y) {
 }
 
 // What takes a sum of products of a query row's digits to a score in units of
-// log2: `first` before the key's scale, where `far` (of any of the wave's rows,
-// else it is 1), and `c` after it. Rows of small values have two factors: the
-// product of both, 2^(e - kQBits), may be too small for a float, and the sum times a
-// large key's scale too large. A score up to 2^60 is so reached from any row and
-// any scale; c and first are normal numbers.
+// log2: `first` before the key's scale and `c` after it, powers of two but for c's
+// part of the formula. Their product may be too small for a float (rows of small
+// values), and a sum times a large key's scale too large: with both, which are
+// normal numbers, a score up to 2^60 is reached from any row and any scale.
 struct QueryFactor {
   float c, first;
-  bool far;
 };
-constexpr int kNear = -32, kFirst = -120;
 DNX_DEV QueryFactor query_factor(float scale, int e, float nan) {
-  const int a = max(min(e - kQBits, 0), kFirst);
-  const bool far = __any(e < kNear);
-  const int b = far ? e - kQBits - a : e - kQBits;
-  return {__builtin_amdgcn_ldexpf(scale * 1.44269504088896341f, b) + nan, power2(a), far};
+  const int a = max(min(e - kQBits, 0), -120);
+  return {__builtin_amdgcn_ldexpf(scale * 1.44269504088896341f, e - kQBits - a) + nan, power2(a)};
 }
 
 // The digits of a query row at the lane's dims, 16 from `dim` on and each `step`
@@ -148,18 +143,12 @@ DNX_DEV QueryFactor query_digits(const float* q, int dim, int step, float scale,
   return query_factor(scale, e, top - top);
 }
 
-// Sums of products to scores over c: times `first` where far, times the keys' scales.
+// Sums of products to scores over c.
 DNX_DEV void to_scores(v4f* s, const QueryFactor& f, const float4* ks) {
-  if (f.far) {
-#pragma unroll
-    for (int u = 0; u < 4; u++)
-#pragma unroll
-      for (int v = 0; v < 4; v++) s[u][v] *= f.first;
-  }
 #pragma unroll
   for (int u = 0; u < 4; u++)
 #pragma unroll
-    for (int v = 0; v < 4; v++) s[u][v] *= (&ks[u].x)[v];
+    for (int v = 0; v < 4; v++) s[u][v] = s[u][v] * f.first * (&ks[u].x)[v];
 }
 
 // The digits of four weights up to 2^e / kRoom, unit = 2^(23 - e), word k those of
