@@ -57,6 +57,25 @@ inline bool paged_wide(int64_t rows, int64_t units, int64_t keys, bool f32) {
   return rows > 128 || rows * keys * units > (f32 ? 1200000 : 4000000);
 }
 
+// int8: a wide block takes the keys' products for 64 rows one step after another,
+// with two barriers each; narrow ones have no barrier in a step, but join four
+// waves' sums for every 16 rows. So wide where the card is full of them and the
+// keys are no more than they are: there what a narrow block costs besides its steps
+// is felt. And wide on a prefix of up to four key heads that narrow blocks would
+// read in as many runs, of one XCD each. us, narrow / wide, 32 / 8 heads, hd 128: 1
+// sequence of 64 new tokens and 256 keys 9.9 / 19.7, 1 of 512 and 2048 keys 60 /
+// 67 (16 / 8: 36 / 67), 1 of 2048 and 2048 161 / 145, 16 of 256 and 256 139 / 76, 64
+// of 64 and 64 115 / 49, of 64 and 1024 324 / 321; 256 tokens over 1000 shared keys 55 /
+// 57, 512 over 16384 on 8 heads over one 834 / 275, 128 68 / 67. At hd 64, 12 / 4: 16 of
+// 64 and 64 11.7 / 8.7, 1 of 1024 and 16384 266 / 334. (544 calls, geometric mean:
+// narrow alone 43.9 us, wide alone 50.5, bf16's rule 49.1, this one 40.9, the better
+// of both 40.8; 128 or 256 workgroups at least 41.0.)
+inline bool paged_wide_i8(int64_t rows, int64_t units, int64_t keys, bool prefix) {
+  if (rows <= 32) return false;
+  return units * ((rows + kPagedWide - 1) / kPagedWide) >= std::max<int64_t>(192, keys) ||
+         (prefix && units <= 4 && rows >= 1024);
+}
+
 // At most that many runs of whole steps.
 inline void paged_deal(PagedPart& p, int64_t keys, int64_t runs) {
   p.keys = ((keys + runs - 1) / runs + kPagedStep - 1) / kPagedStep * kPagedStep;
@@ -69,11 +88,11 @@ inline int64_t paged_items(const PagedPart& p, int64_t units) {
   return (units * p.runs + 7) / 8 * 8 * p.blocks;
 }
 
-inline PagedPart paged_part(int64_t tokens, int64_t group, int64_t units, int64_t keys, bool f32,
-                            int64_t least, int64_t most, int64_t max_runs) {
+inline PagedPart paged_part(int64_t tokens, int64_t group, int64_t units, int64_t keys, bool wide,
+                            bool f32, int64_t least, int64_t most, int64_t max_runs) {
   PagedPart p{};
   const int64_t rows = tokens * group;
-  p.wide = paged_wide(rows, units, keys, f32);
+  p.wide = wide;
   p.few = !f32 || tokens > 1 || rows > 4 ? 0 : rows <= 2 ? 2 : 4;
   const int64_t block = p.wide ? kPagedWide : kPagedNarrow;
   p.blocks = (rows + block - 1) / block;
@@ -81,7 +100,7 @@ inline PagedPart paged_part(int64_t tokens, int64_t group, int64_t units, int64_
   if (keys <= 0 || units <= 0 || rows <= 0) return p;
   // Runs that make about 256 workgroups, of `least` to `most` keys (49 calls,
   // geometric mean: 13.7 us; with 192 or 384 workgroups 13.9 and 14.0, with 128
-  // keys at least 14.1).
+  // keys at least 14.1; int8, 44 calls: 10.7, with 192 10.8, 384 and 512 10.9).
   const int64_t wgs = units * p.blocks;
   int64_t runs = (256 + wgs - 1) / wgs;
   runs = std::min(std::max(runs, (keys + most - 1) / most), std::max<int64_t>(1, keys / least));
@@ -160,29 +179,29 @@ inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, 
                               int64_t kv_heads, int64_t prefix_len, int64_t max_len, bool f32,
                               int i8 = 0) {
   // Without a prefix, keys that one workgroup walks in about the time of the
-  // second launch (3 us) stay in one run: up to 256.
+  // second launch (3 us) stay in one run: up to 256 (int8, 63 calls of up to 512
+  // keys, geometric mean: 8.2 us; up to 64 9.0, 128 8.7, 384 and 512 8.3).
   const int64_t least = prefix_len == 0 && max_len <= 256 ? 256 : kPagedStep;
   const int64_t max_runs = tokens * group * kv_heads >= kPagedManyRows ? kPagedRuns
                            : prefix_len > 0 ? kPagedMaxRuns / 2 : kPagedMaxRuns;
+  const auto wide = [&](int64_t rows, int64_t units, int64_t keys, bool prefix) {
+    return i8 > 0 ? paged_wide_i8(rows, units, keys, prefix) : paged_wide(rows, units, keys, f32);
+  };
+  const bool own_wide = wide(max_tokens * group, seqs * kv_heads, max_len, false);
+  const bool prefix_wide = wide(tokens * group, kv_heads, prefix_len, true);
   const PagedPart own =
-      paged_part(max_tokens, group, seqs * kv_heads, max_len, f32, least, 2048, max_runs);
-  // int8: a wide block's partial results are as many bytes as 256 of its keys and
-  // values. Where the sequences' own workgroups fill the card, the prefix has runs of
-  // that many at least (64 sequences of 128 to 4096 keys after 1000 shared ones, 32
-  // / 8 heads, hd 128: 64 92 us, 128 90, 256 84, 512 88); where not, its runs have
-  // to (6 sequences of up to 37 tokens after 777, 12 / 4 heads, hd 64, window 512:
-  // 64 15.3, 256 22.4).
-  const bool filled = i8 > 0 && seqs * kv_heads * own.blocks * own.runs >= 512;
-  const int64_t prefix_least =
-      filled && paged_wide(tokens * group, kv_heads, prefix_len, f32) ? 256 : kPagedStep;
-  PagedSplit s{paged_part(tokens, group, kv_heads, prefix_len, f32, prefix_least, 1 << 20, max_runs), own,
-               0, 0, 0, 0};
+      paged_part(max_tokens, group, seqs * kv_heads, max_len, own_wide, f32, least, 2048, max_runs);
+  PagedSplit s{paged_part(tokens, group, kv_heads, prefix_len, prefix_wide, f32, kPagedStep, 1 << 20,
+                          max_runs),
+               own, 0, 0, 0, 0};
   // A short prefix is joined to them where a CU for each workgroup is left: its
   // keys are then read once for each block of rows, but without the second
   // launch. Up to 384 keys, or 256 where the float32 matrix cores take 16 rows
   // (us, apart against joined: 1 sequence of 83 keys after 238, f32 hd 64, 8.1 /
   // 6.8; 31 tokens each of 6 after 235, bf16 hd 128, 11.9 / 8.8; 6 tokens each of
-  // 12 after 276, f32 hd 128, 11.3 / 15.4; limits of 512 keys change nothing).
+  // 12 after 276, f32 hd 128, 11.3 / 15.4; limits of 512 keys change nothing). int8,
+  // 216 calls, geometric mean: apart 9.6, up to 256 keys 8.6, up to 384 8.6 (hd 128, 32
+  // sequences of 60 keys after 250, 32 / 8 heads, 12.5 / 11.5, one of them 10.1 / 10.9).
   const auto steps = [](int64_t keys) { return (keys + kPagedStep - 1) / kPagedStep * kPagedStep; };
   const int64_t joined = steps(prefix_len), keys = joined + steps(max_len);
   if (joined > 0 && s.own.runs > 0 && !s.own.wide && keys <= (f32 && s.own.few == 0 ? 256 : 384) &&
