@@ -193,8 +193,9 @@ DNX_DEV bool unseen(const PagedArgs& a, const Item& w, int end) {
 // mean: 9.11 us against 8.98).
 // Body: the blocks of one cache type and head size. kKeys: of a wave's step in a
 // block of 16. kTogether: paged_together's order. kLastFirst: a prompt's last rows,
-// which see the most keys, begin first (int8, 4096 tokens, 32 / 8 heads, hd 128: 366
-// -> 328 us; 2047 of 4099, 16 / 8 141 -> 118).
+// which see the most keys, begin first (int8, hd 128: 4096 tokens, 32 / 8 heads, 632
+// -> 610 us; four prompts of 1024 190 -> 160, sixteen of 512 222 -> 226; 725 tokens of
+// 4099 keys, 16 / 8 heads, 111 -> 107).
 template <typename Body, bool kPacked>
 DNX_DEV void paged_workgroup(const PagedArgs& a, uint8_t* lds) {
   Item w;

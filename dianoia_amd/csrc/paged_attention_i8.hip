@@ -11,7 +11,7 @@
 //   the power of two above 1.004 times its largest value: off by half a unit, 2^-32
 //   of 2^e. With three digits a row with one channel 3000 times the others, whose
 //   keys are as much smaller, is off by 1.2e-4 (2000 keys, hd 128), with four by
-//   5e-7; the fourth costs nothing that could be measured.
+//   5e-7; the fourth takes 3% of a prompt's time and none of a decode step's.
 // * the weights e^(s_j - m) vs_j of a row and step are numbers of 23 bits in three,
 //   2^e above the largest of that step: relative to the step, not to the running
 //   maximum, so that a long tail of small weights is kept. 64 keys times half a
@@ -289,11 +289,14 @@ DNX_DEV float step_weights(v4f* s, float c, const float4* vs, bool edge, F sees,
 // lines hold two heads: those of a run run on one XCD, through one L2 (64
 // sequences of 1088 keys, 28 -> 19.5 us; at hd 128 3% slower).
 //
-// 64 sequences, 32 / 8 heads, hd 128, of 4096 keys 113 us, 4.9 TB/s (reading alone
-// 98), of 1088 34 us, 4.4; one of 131072 61, of which 5 are the second launch. A
-// step of 64 keys takes about 500 vector instructions (the bf16 form of
-// paged_attention.hip 1000 for as many), which cover half of the reading's time;
-// forming the products of one part beside the sums of another gained nothing.
+// 64 sequences, 32 / 8 heads, hd 128, of 4096 keys 108 us, 5.1 TB/s (reading alone
+// 98), of 1088 32 us, 4.6; one of 131072 56, of which 5 are the second launch. A
+// step of 64 keys takes about 630 vector instructions and 56 matrix ones (the bf16
+// form of paged_attention.hip 1000 vector ones for as many), which a decode step
+// hides behind the reading; forming the products of one part beside the sums of
+// another gained nothing. In a prompt they are what bounds it: 4096 tokens, 32 / 8
+// heads, hd 128, 610 us, 225 TFLOP/s of the formula's products; 725 of 4099 keys, 16 /
+// 8 heads, 107.
 template <int HD>
 struct Raw {
   uint4 k[4][HD / 64];
@@ -492,11 +495,15 @@ DNX_DEV void narrow(const PagedArgs& a, const Item& w, uint8_t* lds) {
 // a quarter and dim are those of its sixteen keys, turned on the way. The next
 // tile is in registers meanwhile.
 //
-// 4096 tokens of a prompt, 32 / 8 heads, hd 128: 323 us, 248 TFLOP/s of the formula's
-// products; 2047 of 4099, 16 / 8 heads, 117 us. Vector instructions bound it, about
-// 450 for a wave's 64 keys of 16 rows: 16 a score (digits to a float, exp2, float to
-// digits) and 5 a sum (digits to a float, into the running sum), beside 48 matrix
-// instructions; tiles of 128 keys would halve the latter and are not tried.
+// Sixteen prompts of 512 tokens, 32 / 8 heads, hd 128: 226 us, 152 TFLOP/s of the
+// formula's products; 64 of 64 tokens 48 us. For a wave's 64 keys of 16 rows it takes
+// about 450 vector instructions, 18 a score (digits to a float, exp2, float to digits)
+// and 5 a sum (digits to a float, into the running sum), beside 56 matrix ones, and
+// about 60 to stage its part of the tile: the four blocks of a tile lie in scratch
+// memory (112 bytes a lane), since a load's block is chosen at run time, and the
+// loads' addresses wait for it. That, the two barriers and the digits bound it; a
+// staging that looks up a wave's own block alone and tiles of 128 keys (half the sums)
+// are not tried.
 template <int HD>
 struct WideTile {
   static constexpr int KT = 64, KC = HD / 16;      // 16-byte chunks of a key
