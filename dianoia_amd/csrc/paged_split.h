@@ -59,9 +59,10 @@ inline bool paged_wide(int64_t rows, int64_t units, int64_t keys, bool f32) {
 
 // int8: a wide block takes the keys' products for 64 rows one step after another,
 // with two barriers each; narrow ones have no barrier in a step, but join four
-// waves' sums for every 16 rows. So wide where the card is full of them and the
-// keys are no more than they are: there what a narrow block costs besides its steps
-// is felt. And wide on a prefix of up to four key heads that narrow blocks would
+// waves' sums for every 16 rows. So wide where all rows together fill the card with
+// them and the keys are no more than they are: there what a narrow block costs
+// besides its steps is felt. (All rows, not the bound on a sequence's: 64 sequences, one
+// of 20 new tokens and the others of one, 200 keys, 8 / 2 heads, hd 128, 9.5 / 15.3.) And wide on a prefix of up to four key heads that narrow blocks would
 // read in as many runs, of one XCD each. us, narrow / wide, 32 / 8 heads, hd 128: 1
 // sequence of 64 new tokens and 256 keys 9.9 / 19.7, 1 of 512 and 2048 keys 60 /
 // 67 (16 / 8: 36 / 67), 1 of 2048 and 2048 161 / 145, 16 of 256 and 256 139 / 76, 64
@@ -70,10 +71,11 @@ inline bool paged_wide(int64_t rows, int64_t units, int64_t keys, bool f32) {
 // 64 and 64 11.7 / 8.7, 1 of 1024 and 16384 266 / 334. (544 calls, geometric mean:
 // narrow alone 43.9 us, wide alone 50.5, bf16's rule 49.1, this one 40.9, the better
 // of both 40.8; 128 or 256 workgroups at least 41.0.)
-inline bool paged_wide_i8(int64_t rows, int64_t units, int64_t keys, bool prefix) {
+// rows: of a unit; all: of a key head in all sequences.
+inline bool paged_wide_i8(int64_t rows, int64_t all, int64_t kv_heads, int64_t keys, bool prefix) {
   if (rows <= 32) return false;
-  return units * ((rows + kPagedWide - 1) / kPagedWide) >= std::max<int64_t>(192, keys) ||
-         (prefix && units <= 4 && rows >= 1024);
+  return kv_heads * ((all + kPagedWide - 1) / kPagedWide) >= std::max<int64_t>(192, keys) ||
+         (prefix && kv_heads <= 4 && rows >= 1024);
 }
 
 // At most that many runs of whole steps.
@@ -184,11 +186,11 @@ inline PagedSplit paged_split(int64_t seqs, int64_t tokens, int64_t max_tokens, 
   const int64_t least = prefix_len == 0 && max_len <= 256 ? 256 : kPagedStep;
   const int64_t max_runs = tokens * group * kv_heads >= kPagedManyRows ? kPagedRuns
                            : prefix_len > 0 ? kPagedMaxRuns / 2 : kPagedMaxRuns;
-  const auto wide = [&](int64_t rows, int64_t units, int64_t keys, bool prefix) {
-    return i8 > 0 ? paged_wide_i8(rows, units, keys, prefix) : paged_wide(rows, units, keys, f32);
-  };
-  const bool own_wide = wide(max_tokens * group, seqs * kv_heads, max_len, false);
-  const bool prefix_wide = wide(tokens * group, kv_heads, prefix_len, true);
+  const int64_t rows = tokens * group, own_rows = max_tokens * group;
+  const bool own_wide = i8 > 0 ? paged_wide_i8(own_rows, rows, kv_heads, max_len, false)
+                               : paged_wide(own_rows, seqs * kv_heads, max_len, f32);
+  const bool prefix_wide = i8 > 0 ? paged_wide_i8(rows, rows, kv_heads, prefix_len, true)
+                                  : paged_wide(rows, kv_heads, prefix_len, f32);
   const PagedPart own =
       paged_part(max_tokens, group, seqs * kv_heads, max_len, own_wide, f32, least, 2048, max_runs);
   PagedSplit s{paged_part(tokens, group, kv_heads, prefix_len, prefix_wide, f32, kPagedStep, 1 << 20,

@@ -16,23 +16,25 @@ pytestmark = pytest.mark.gpu
 
 
 def ragged(seqs, most, tokens, seed):
-    """Lengths up to `most` with borders of steps among them, new tokens up to `tokens`."""
+    """Lengths up to `most` with borders of steps among them; one new token in every
+    sixth sequence, about `tokens` in the others."""
     rng = np.random.default_rng(seed)
-    lens = rng.choice([1, 63, 64, 65, 100, 127, 128, most - 1, most, most // 2], seqs)
-    lens = np.minimum(np.maximum(lens, 1), most)
-    counts = np.minimum(rng.choice([1, tokens, tokens - 1, tokens // 2], seqs), lens)
-    lens[0], counts[0], lens[-1], counts[-1] = most, min(tokens, most), most, 1
+    lens = rng.choice([63, 64, 65, 100, 127, 128, 129, most - 1, most, most], seqs)
+    lens = np.minimum(lens, most)
+    counts = np.minimum([1 if i % 6 == 5 else tokens - i % 2 for i in range(seqs)], lens)
+    lens[0], counts[0], lens[-1], counts[-1] = most, min(tokens, most), 1, 1
     return counts.tolist(), lens.tolist()
 
 
 # counts, lens, prefix, heads, kv, page
-OWN = [(*ragged(24, 190, 33, 1), 0, 8, 8, 16), (*ragged(50, 200, 12, 2), 0, 12, 4, 32),
-       (*ragged(24, 190, 40, 3), 70, 8, 8, 64), (*ragged(100, 190, 9, 4), 300, 8, 2, 16),
+OWN = [(*ragged(48, 190, 45, 1), 0, 8, 8, 16), (*ragged(60, 200, 25, 2), 0, 12, 4, 32),
+       (*ragged(24, 190, 100, 3), 70, 8, 8, 64), (*ragged(160, 190, 12, 4), 300, 8, 2, 16),
        (*ragged(3, 130, 130, 5), 0, 64, 32, 64)]
 PREFIX = [([1] * 257, [1 + i % 40 for i in range(257)], 100, 4, 1, 16), ([260, 3], [290, 200], 65, 4, 1, 64),
           ([37, 1, 100, 0, 128], [40, 9, 100, 7, 500], 2100, 8, 2, 32), ([1] * 350, [3] * 350, 1, 9, 3, 16),
           ([130] * 3, [130, 200, 400], 640, 12, 4, 128)]
 SHAPES = OWN + PREFIX
+BOUNDED = [190] * 4 + [1] * 60 + [2, 0, 33], [190] * 4 + [3 * i + 1 for i in range(60)] + [7, 0, 180]
 
 
 def batch(seed, i, hd, **more):
@@ -119,9 +121,9 @@ def test_next_to_powers_of_two(gpu_ready):
 def test_bounds_above_the_batch(gpu_ready, window):
     """Every sequence might have as many tokens and keys as the largest: its blocks lie in
     a row, and most runs hold no key."""
-    counts, lens = [33] + [1] * 60 + [2, 0, 33], [190] + [5 * i % 190 + 1 for i in range(60)] + [7, 0, 180]
+    counts, lens = BOUNDED
     b = Tight(77, counts, lens, 0, 16, 8, 64, 16, pad=3)
-    b.batch = D.PagedBatch(b.starts, b.lens_d, b.tables, b.live + 3, 100, 190)
+    b.batch = D.PagedBatch(b.starts, b.lens_d, b.tables, b.live + 3, 700, 190)
     b.ws = D.paged_attention_workspace(b.cache, b.batch, b.heads)
     b.ws.fill_(0xff)
     b.check(window)

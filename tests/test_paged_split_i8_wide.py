@@ -7,7 +7,7 @@ import subprocess
 
 import pytest
 
-from test_gpu_paged_i8_wide import OWN, PREFIX
+from test_gpu_paged_i8_wide import BOUNDED, OWN, PREFIX
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -51,5 +51,10 @@ def test_shapes_of_the_gpu_tests(kinds):
         for hd in (64, 128):
             kind = kinds(len(counts), sum(counts), max(counts), heads // kv, kv, prefix, max(lens), hd)
             assert kind & (1 if i < len(OWN) else 2) and kind < 4, (i, kind)
-    for tokens in (sum([33] + [1] * 60 + [2, 0, 33]) + 3,):     # test_bounds_above_the_batch
-        assert kinds(64, tokens, 100, 2, 8, 0, 190, 64) == 1
+    assert kinds(len(BOUNDED[0]), sum(BOUNDED[0]) + 3, 700, 2, 8, 0, 190, 64) == 1
+
+
+def test_bounds_of_sequences_do_not_count_as_rows(kinds):
+    """Up to 20 new tokens of each of 64 sequences, 83 in all."""
+    assert kinds(64, 83, 20, 4, 2, 0, 200, 128) == 0
+    assert kinds(64, 64 * 20, 20, 4, 8, 0, 200, 128) == 1
