@@ -61,14 +61,15 @@ inline bool paged_wide(int64_t rows, int64_t units, int64_t keys, bool f32) {
 // with two barriers each; narrow ones have no barrier in a step, but join four
 // waves' sums for every 16 rows. So wide where all rows together fill the card with
 // them and the keys are no more than they are: there what a narrow block costs
-// besides its steps is felt. (All rows, not the bound on a sequence's: 64 sequences, one
-// of 20 new tokens and the others of one, 200 keys, 8 / 2 heads, hd 128, 9.5 / 15.3.) And wide on a prefix of up to four key heads that narrow blocks would
-// read in as many runs, of one XCD each. us, narrow / wide, 32 / 8 heads, hd 128: 1
-// sequence of 64 new tokens and 256 keys 9.9 / 19.7, 1 of 512 and 2048 keys 60 /
-// 67 (16 / 8: 36 / 67), 1 of 2048 and 2048 161 / 145, 16 of 256 and 256 139 / 76, 64
-// of 64 and 64 115 / 49, of 64 and 1024 324 / 321; 256 tokens over 1000 shared keys 55 /
-// 57, 512 over 16384 on 8 heads over one 834 / 275, 128 68 / 67. At hd 64, 12 / 4: 16 of
-// 64 and 64 11.7 / 8.7, 1 of 1024 and 16384 266 / 334. (544 calls, geometric mean:
+// besides its steps is felt. (All rows, not the bound on a sequence's: 64 sequences,
+// one of 20 new tokens and the others of one, 200 keys, 8 / 2 heads, hd 128, 9.5 us
+// narrow, 15.3 wide.) And wide on a prefix of up to four key heads that narrow blocks
+// would read in as many runs, of one XCD each. us, narrow / wide, 32 / 8 heads, hd
+// 128: 1 sequence of 64 new tokens and 256 keys 9.9 / 19.7, 1 of 512 and 2048 keys 67 /
+// 113 (16 / 8: 36 / 67), 1 of 2048 and 2048 161 / 145, 16 of 256 and 256 139 / 76, 64
+// of 64 and 64 115 / 49, of 64 and 1024 324 / 321; 256 tokens over 1000 shared keys 55
+// / 57, 512 over 16384 on 8 heads over one 834 / 275, 128 68 / 67. At hd 64, 12 / 4:
+// 16 of 64 and 64 11.7 / 8.7, 1 of 1024 and 16384 266 / 334. (544 calls, geometric mean:
 // narrow alone 43.9 us, wide alone 50.5, bf16's rule 49.1, this one 40.9, the better
 // of both 40.8; 128 or 256 workgroups at least 41.0.)
 // rows: of a unit; all: of a key head in all sequences.
